@@ -235,7 +235,7 @@ def _adamw(s):
         s["exp_avg_sq"].copy_(v)
         return [s["param"], s["exp_avg"], s["exp_avg_sq"]]
     key = _mixed(_mixed(torch.tensor(s["seed"] & 0xFFFFFFFF, device=g.device)) ^ (t & 0xFFFFFFFF))
-    h = _mixed(_mixed(torch.arange(s["total"], device=g.device) & 0xFFFFFFFF) ^ key)
+    h = _mixed((torch.arange(s["total"], device=g.device) & 0xFFFFFFFF) ^ key)
     for name, value, dither, top in (("exp_avg", m, h & 0xFFFF, 8), ("exp_avg_sq", v, h >> 16, 15)):
         code, scale = _squeeze(value, top, 0x600000, dither.float() * 2.0 ** -16)
         s[name].copy_(code)
