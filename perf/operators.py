@@ -144,8 +144,8 @@ def _prepare_adamw(case, seed):
     if own:
         from pin_slam_amd import ops
         params = [param[a:a + v] for v, a in zip(sizes, starts)]
-        s["grads"] = [grad[a:a + v] for v, a in zip(sizes, starts)]
-        s["optimizer"] = ops.AdamW(params, lr=LR, betas=(BETA1, BETA2), eps=EPS, weight_decay=DECAY, state_bits=case["bits"], seed=s["seed"])
+        grads = [grad[a:a + v] for v, a in zip(sizes, starts)]
+        s["optimizer"] = ops.AdamW(params, grads, lr=LR, betas=(BETA1, BETA2), eps=EPS, weight_decay=DECAY, state_bits=case["bits"], seed=s["seed"])
         s["optimizer"].load_state_dict({"step": s["step"], **{k: s[k] for k in s if k.startswith("exp_avg")}})
     return s
 
@@ -259,7 +259,7 @@ def run(state):
         return _predict(state["x"], state["weight"], state["bias"], torch.float32)
     if own:
         opt = state["optimizer"]
-        opt.step(state["grads"])
+        opt.step()
         if case["bits"] == 32:
             return [state["param"], opt.exp_avg, opt.exp_avg_sq]
         return [state["param"], opt.exp_avg, opt.exp_avg_sq, opt.exp_avg_scale, opt.exp_avg_sq_scale]
