@@ -6,7 +6,7 @@ R=$(cd "$(dirname "$0")/.." && pwd)
 N=$1; shift
 O=$R/pin_slam_amd/_variants/obj_$N; mkdir -p $O
 for f in $R/pin_slam_amd/csrc/*.hip; do
-  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-result "$@" -c $f -o $O/$(basename ${f%.hip}).o &
+  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops "$@" -c $f -o $O/$(basename ${f%.hip}).o &
 done
 wait
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -ldl -o $R/pin_slam_amd/_variants/libpinhip_$N.so $O/*.o
