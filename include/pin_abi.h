@@ -58,7 +58,7 @@ typedef struct pin_sample_params {
 extern "C" {
 #endif
 
-#define PIN_ABI_VERSION 18
+#define PIN_ABI_VERSION 19
 #define PIN_FEATURE_DIM 8          /* config.feature_dim (utils/config.py:103) */
 #define PIN_MLP_IN (PIN_FEATURE_DIM + 3)
 #define PIN_MAX_K 8                /* query_nn_k: 6 default, 8 in the benchmark configs */
@@ -1099,6 +1099,45 @@ int pin_dp_cert_apply(float* certainty, const float* certainty0, const float* de
  * one RCCL group.  scratch [n] floats. */
 int pin_dp_sync_side_effects(void* comm, float* certainty, const float* certainty0, float* scratch,
                              int32_t* ts_update, int32_t n, void* stream);
+
+/* ---- an optimiser step over many tensors (csrc/adamw.hip) ---------------------------------------------------------------------
+ * AdamW (decoupled weight decay) as torch.optim.Adam is configured by setup_optimizer (utils/tools.py:153-203, whose groups carry a
+ * weight_decay), for any number of tensors in one call and with moments of 32 or 8 bits:
+ *   t += 1;  m += (g - m)(1 - beta1);  v = v beta2 + (1 - beta2) g g
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * The moments of all tensors lie in ONE layout, each tensor from a multiple of PIN_ADAMW_BLOCK elements on.  state_bits 8: exp_avg
+ * holds e4m3 and exp_avg_sq e5m2 codes (OCP), value = code * scale[element / PIN_ADAMW_BLOCK], scales powers of two; codes are
+ * rounded up with the probability of the remainder, the dither a hash of (seed, step, element): the same call gives the same bits.
+ * A moment that is not finite makes the scale of its block NaN. */
+#define PIN_F32 0
+#define PIN_BF16 1
+#define PIN_F16 2
+#define PIN_ADAMW_BLOCK 256
+#define PIN_ADAMW_CLOCK_DOUBLES 8  /* t, beta1^t, beta2^t, lr, and at PIN_ADAMW_CLOCK_TICKET a 64-bit counter (0 between calls) */
+#define PIN_ADAMW_CLOCK_TICKET 4
+typedef struct pin_adamw_tensor {
+    void* param;             /* [n] updated in place */
+    void* grad;              /* [n]; cleared in the same pass with zero_grad */
+    int64_t n;               /* 0 = nothing to do */
+    int64_t offset;          /* first element in the moments' layout, a multiple of PIN_ADAMW_BLOCK */
+    int32_t param_dtype, grad_dtype;  /* PIN_F32, PIN_BF16, PIN_F16: rounded to nearest from the fp32 arithmetic */
+    float weight_decay;
+    int32_t reserved;
+} pin_adamw_tensor;
+typedef struct pin_adamw_state {
+    void* exp_avg;           /* [total] float, or uint8 e4m3 codes */
+    void* exp_avg_sq;        /* [total] float, or uint8 e5m2 codes */
+    float* exp_avg_scale;    /* [total / PIN_ADAMW_BLOCK], state_bits 8 only */
+    float* exp_avg_sq_scale;
+    double* clock;           /* [PIN_ADAMW_CLOCK_DOUBLES] DEVICE: the step count lives here and is set by the call, so that a captured
+                              * call counts on with every replay; lr is read from here */
+    int64_t total;           /* elements of the layout, a multiple of PIN_ADAMW_BLOCK */
+    int32_t state_bits;      /* 32 or 8 */
+    int32_t zero_grad;
+} pin_adamw_state;
+/* tensors_host is a HOST array, read before the call returns.  At least one tensor must have elements. */
+int pin_adamw_step(const pin_adamw_tensor* tensors_host, int32_t n_tensors, const pin_adamw_state* st, float beta1, float beta2,
+                   float eps, uint32_t seed, void* stream);
 
 #ifdef __cplusplus
 }

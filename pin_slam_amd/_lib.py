@@ -19,9 +19,12 @@ PIN_NONLOCAL = -2
 PIN_NBR_QUIRK_BIT = 0x40000000
 PIN_GN_NSUMS = 32
 PIN_GN_REPLICAS = 16
-PIN_ABI_VERSION = 18
+PIN_ABI_VERSION = 19
 PIN_ADAM_ROW_EXCLUDED = -(1 << 31)
 PIN_COMM_ID_BYTES = 128
+PIN_F32, PIN_BF16, PIN_F16 = 0, 1, 2
+PIN_ADAMW_BLOCK = 256
+PIN_ADAMW_CLOCK_DOUBLES = 8
 
 vp = C.c_void_p
 
@@ -149,6 +152,16 @@ class TrainColorParams(C.Structure):
 class SemParams(C.Structure):
     _fields_ = [("n_main", C.c_int32), ("heads", C.c_int32), ("weight_s", C.c_float), ("reserved", C.c_int32), ("labels", vp),
                 ("selected", vp), ("count", vp)]
+
+
+class AdamwTensor(C.Structure):
+    _fields_ = [("param", vp), ("grad", vp), ("n", C.c_int64), ("offset", C.c_int64), ("param_dtype", C.c_int32), ("grad_dtype", C.c_int32),
+                ("weight_decay", C.c_float), ("reserved", C.c_int32)]
+
+
+class AdamwState(C.Structure):
+    _fields_ = [("exp_avg", vp), ("exp_avg_sq", vp), ("exp_avg_scale", vp), ("exp_avg_sq_scale", vp), ("clock", vp), ("total", C.c_int64),
+                ("state_bits", C.c_int32), ("zero_grad", C.c_int32)]
 
 
 class PreprocessParams(C.Structure):
@@ -292,6 +305,7 @@ SIGNATURES = {
     "pin_dp_cert_delta": (i32, [vp, vp, vp, i32, vp]),
     "pin_dp_cert_apply": (i32, [vp, vp, vp, i32, vp]),
     "pin_dp_sync_side_effects": (i32, [vp, vp, vp, vp, vp, i32, vp]),
+    "pin_adamw_step": (i32, [P(AdamwTensor), i32, P(AdamwState), f32, f32, f32, C.c_uint32, vp]),
 }
 
 _lib = None

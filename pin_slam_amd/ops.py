@@ -74,6 +74,24 @@ def _stream():
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
+class _device_of:
+    """Makes `device` current for a call whose tensors live there (nothing to do, and nothing spent, where it already is)."""
+
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self):
+        now = torch._C._cuda_getDevice()
+        self.back = now if self.index is not None and now != self.index else None
+        if self.back is not None:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.back is not None:
+            torch.cuda.set_device(self.back)
+        return False
+
+
 def spatial_sort(points: torch.Tensor, cell: float, return_perm: bool = False):
     """points [n,3] in ascending Morton order of floor(p / cell) (pin_spatial_sort); optionally the permutation."""
     L = _lib.lib()
@@ -862,3 +880,153 @@ def gather_rows(src: torch.Tensor, index: torch.Tensor, out: Optional[torch.Tens
     check(_lib.lib().pin_gather_rows(_ptr(src, torch.float32), width, _ptr(index, torch.int32), index.numel(), _ptr(out),
                                      _stream()), "pin_gather_rows")
     return out
+
+
+# ------------------------------------------------------------------------------- AdamW over many tensors (csrc/adamw.hip)
+_DTYPE_CODES = {torch.float32: _lib.PIN_F32, torch.bfloat16: _lib.PIN_BF16, torch.float16: _lib.PIN_F16}
+
+
+class AdamW:
+    """One AdamW step over many tensors per call (pin_adamw_step): decoupled weight decay, moments of 32 or of 8 bits.
+
+    params: contiguous device tensors, float32 / bfloat16 / float16, updated in place.  grads: their gradient buffers, of the same
+    sizes, float32 / bfloat16 / float16 (they may be None: ``step(grads)`` then brings them).  weight_decay: a number, or one for
+    every tensor.  state_bits 32: float32 moments; with weight decay 0 a step is bit for bit ``adam_step``.  state_bits 8: the
+    moments take 2 bytes an element instead of 8 -- ``exp_avg`` float8_e4m3fn and ``exp_avg_sq`` float8_e5m2 with a power-of-two
+    scale per 256 elements, rounded by a dither that depends on (seed, step, element) alone, so that a run repeats bit for bit.
+
+    ``exp_avg`` / ``exp_avg_sq`` [total] (and ``*_scale`` [total / 256]) hold the moments of all tensors, tensor i from element
+    ``offsets[i]`` on (a multiple of 256).  The step count lives on the device: a captured ``step()`` counts on when its graph is
+    replayed; ``lr`` is read on the device too, and setting it takes effect with the next step, replayed ones included."""
+
+    def __init__(self, params, grads=None, lr=0.01, betas=(0.9, 0.99), eps=1e-15, weight_decay=0.0, state_bits=32, seed=0):
+        self.params = list(params)
+        if not self.params:
+            raise ValueError("no parameters")
+        if state_bits not in (8, 32):
+            raise ValueError("state_bits must be 32 or 8")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0 and eps >= 0.0):
+            raise ValueError("betas must lie in [0, 1), eps must not be negative")
+        decay = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else [float(weight_decay)] * len(self.params)
+        if len(decay) != len(self.params):
+            raise ValueError("weight_decay: one number, or one for every parameter")
+        self.betas, self.eps, self.state_bits, self.seed = (float(betas[0]), float(betas[1])), float(eps), int(state_bits), int(seed) & 0xFFFFFFFF
+        self.device = self.params[0].device
+        self.offsets, total = [], 0
+        self._table = (_lib.AdamwTensor * len(self.params))()
+        for i, p in enumerate(self.params):
+            _ptr(p)
+            if p.dtype not in _DTYPE_CODES:
+                raise RuntimeError(f"parameter {i}: float32, bfloat16 or float16, got {p.dtype}")
+            if p.device != self.device:
+                raise RuntimeError(f"parameter {i} is on {p.device}, the first one on {self.device}")
+            self.offsets.append(total)
+            t = self._table[i]
+            t.n, t.offset, t.param_dtype, t.weight_decay = p.numel(), total, _DTYPE_CODES[p.dtype], float(decay[i])
+            total += -(-p.numel() // _lib.PIN_ADAMW_BLOCK) * _lib.PIN_ADAMW_BLOCK
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in self.params if p.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise RuntimeError("two parameters share memory: they would be updated twice, in no order")
+        self.total = total
+        kinds = (torch.float32, torch.float32) if state_bits == 32 else (torch.float8_e4m3fn, torch.float8_e5m2)
+        self.exp_avg, self.exp_avg_sq = (torch.zeros(total, dtype=torch.uint8 if state_bits == 8 else torch.float32, device=self.device).view(k)
+                                         for k in kinds)
+        self.exp_avg_scale = self.exp_avg_sq_scale = None
+        if state_bits == 8:
+            self.exp_avg_scale, self.exp_avg_sq_scale = (torch.ones(total // _lib.PIN_ADAMW_BLOCK, device=self.device) for _ in range(2))
+        self._clock = torch.zeros(_lib.PIN_ADAMW_CLOCK_DOUBLES, dtype=torch.float64, device=self.device)
+        self._clock[1:3] = 1.0
+        self.lr = lr
+        self._state = _lib.AdamwState(self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(),
+                                      None if state_bits == 32 else self.exp_avg_scale.data_ptr(),
+                                      None if state_bits == 32 else self.exp_avg_sq_scale.data_ptr(), self._clock.data_ptr(), total,
+                                      self.state_bits, 0)
+        self.grads = None
+        self._addresses = None
+        if grads is not None:
+            self._bind(list(grads))
+
+    @property
+    def lr(self):
+        return self._lr
+
+    @lr.setter
+    def lr(self, lr):
+        self._lr = float(lr)
+        self._clock[3:4].fill_(float(np.float32(lr)))
+
+    @property
+    def steps(self) -> int:
+        """Steps taken so far (reads the device's count: synchronises)."""
+        return int(self._clock[0].item())
+
+    def _bind(self, grads):
+        if len(grads) != len(self.params):
+            raise RuntimeError(f"{len(grads)} gradients for {len(self.params)} parameters")
+        for i, (p, g) in enumerate(zip(self.params, grads)):
+            t = self._table[i]
+            t.n, t.param, t.grad = (0, None, None) if g is None else (p.numel(), p.data_ptr(), _ptr(g))
+            if g is None:  # (no gradient: neither the parameter nor its moments move, as in torch.optim)
+                continue
+            _ptr(p)
+            if g.dtype not in _DTYPE_CODES:
+                raise RuntimeError(f"gradient {i}: float32, bfloat16 or float16, got {g.dtype}")
+            if g.numel() != p.numel() or g.device != self.device:
+                raise RuntimeError(f"gradient {i}: {tuple(g.shape)} on {g.device} for a parameter {tuple(p.shape)} on {self.device}")
+            t.grad_dtype = _DTYPE_CODES[g.dtype]
+        self.grads = grads
+        self._bound = self.params + [g for g in grads if g is not None]
+        self._addresses = [t.data_ptr() for t in self._bound]
+        self._any = any(t.n for t in self._table)
+
+    def step(self, grads=None, zero_grad: bool = False):
+        """Update every parameter that has a gradient.  zero_grad: clear the gradients in the same pass (kernels that ADD into their
+        gradient buffers).  Without an element to update the step does not count."""
+        if grads is not None:
+            self._bind(list(grads))
+        elif self.grads is None:
+            raise RuntimeError("no gradients: pass them to AdamW() or to step()")
+        elif [t.data_ptr() for t in self._bound] != self._addresses:  # (a buffer was replaced behind its tensor, e.g. by .data = ...)
+            self._bind(self.grads)
+        if not self._any:
+            return
+        self._state.zero_grad = int(bool(zero_grad))
+        with _device_of(self.device):
+            check(_lib.lib().pin_adamw_step(self._table, len(self.params), C.byref(self._state), self.betas[0], self.betas[1], self.eps,
+                                            self.seed, _stream()), "pin_adamw_step")
+
+    def moments(self, i: int):
+        """(exp_avg, exp_avg_sq) of parameter i as float32 tensors of its shape: views of the moments (32 bits) or the values that the
+        codes stand for (8 bits)."""
+        p, a = self.params[i], self.offsets[i]
+        if self.state_bits == 32:
+            return tuple(m[a:a + p.numel()].view(p.shape) for m in (self.exp_avg, self.exp_avg_sq))
+        b = a + -(-p.numel() // _lib.PIN_ADAMW_BLOCK) * _lib.PIN_ADAMW_BLOCK
+        return tuple((m[a:b].float().view(-1, _lib.PIN_ADAMW_BLOCK) * s[a // _lib.PIN_ADAMW_BLOCK:b // _lib.PIN_ADAMW_BLOCK, None])
+                     .view(-1)[:p.numel()].view(p.shape) for m, s in ((self.exp_avg, self.exp_avg_scale), (self.exp_avg_sq, self.exp_avg_sq_scale)))
+
+    def state_dict(self) -> dict:
+        """Moments, step count and settings, as a checkpoint stores them (the tensors are copies; synchronises)."""
+        d = {"step": self.steps, "lr": self.lr, "seed": self.seed, "state_bits": self.state_bits}
+        for k in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"):
+            if getattr(self, k) is not None:
+                d[k] = getattr(self, k).clone()
+        return d
+
+    def load_state_dict(self, d: dict):
+        """Take over what state_dict() gave (lr, seed and state_bits may be missing)."""
+        if int(d.get("state_bits", self.state_bits)) != self.state_bits:
+            raise ValueError(f"the state has {d['state_bits']}-bit moments, this optimiser {self.state_bits}-bit ones")
+        names = [k for k in ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale") if getattr(self, k) is not None]
+        for k in names:
+            if d[k].shape != getattr(self, k).shape or d[k].dtype != getattr(self, k).dtype:
+                raise ValueError(f"{k}: {tuple(d[k].shape)} {d[k].dtype}, expected {tuple(getattr(self, k).shape)} {getattr(self, k).dtype}")
+        step = int(d["step"])
+        if step < 0:
+            raise ValueError("step must not be negative")
+        for k in names:
+            getattr(self, k).view(torch.uint8).copy_(d[k].to(self.device).view(torch.uint8))
+        b1, b2 = (float(np.float32(b)) for b in self.betas)
+        self._clock[:3].copy_(torch.tensor([float(step), b1 ** step, b2 ** step], dtype=torch.float64))
+        self.seed = int(d.get("seed", self.seed)) & 0xFFFFFFFF
+        self.lr = d.get("lr", self.lr)

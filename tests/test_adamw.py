@@ -1,0 +1,353 @@
+"""AdamW over many tensors (pin_adamw_step, ops.AdamW): against the formula in 64 bits, against adam_step bit for bit, the 8-bit codes
+against a table of the formats' values, and what a program does around it (graphs, streams, checkpoints, refusals)."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from pin_slam_amd import _lib, ops
+
+BLOCK = _lib.PIN_ADAMW_BLOCK
+gpu = pytest.mark.gpu
+F32 = 2.0 ** -24  # half a step of float32
+
+
+# ------------------------------------------------------------------------------------------------ refusals (no GPU needed)
+@pytest.fixture
+def host(monkeypatch):
+    """Host tensors pass for device tensors: the argument checks run, no launch is reached."""
+    monkeypatch.setattr(ops, "_ptr", lambda t, dtype=None: None if t is None else t.data_ptr())
+
+
+def test_cpu_tensors_are_refused():
+    with pytest.raises(RuntimeError, match="device"):
+        ops.AdamW([torch.zeros(4)], [torch.zeros(4)])
+
+
+@pytest.mark.parametrize("kw, word", [
+    (dict(params=[]), "no parameters"),
+    (dict(state_bits=16), "state_bits"),
+    (dict(betas=(1.0, 0.9)), "betas"),
+    (dict(eps=-1.0), "eps"),
+    (dict(weight_decay=[0.1, 0.2]), "weight_decay"),
+    (dict(params=[torch.zeros(4, dtype=torch.float64)]), "float64"),
+    (dict(grads=[]), "0 gradients"),
+    (dict(grads=[torch.zeros(5)]), "gradient 0"),
+    (dict(grads=[torch.zeros(4, dtype=torch.int32)]), "gradient 0"),
+])
+def test_refusals(host, kw, word):
+    kw = {"params": [torch.zeros(4)], **kw}
+    with pytest.raises((RuntimeError, ValueError), match=word):
+        ops.AdamW(kw.pop("params"), kw.pop("grads", None), **kw)
+
+
+def test_shared_memory_and_missing_gradients_are_refused(host):
+    flat = torch.zeros(10)
+    with pytest.raises(RuntimeError, match="share memory"):
+        ops.AdamW([flat[:6], flat[4:]])
+    opt = ops.AdamW([flat[:6], flat[6:]])
+    with pytest.raises(RuntimeError, match="no gradients"):
+        opt.step()
+    with pytest.raises(ValueError, match="32-bit"):
+        opt.load_state_dict({"state_bits": 8, "step": 1})
+    with pytest.raises(ValueError, match="exp_avg"):
+        opt.load_state_dict({"step": 1, "exp_avg": torch.zeros(3), "exp_avg_sq": torch.zeros(3)})
+    opt.step([None, None])  # nothing to update: no launch, no step
+
+
+def test_layout_and_state_dict(host):
+    ps = [torch.zeros(1), torch.zeros(0), torch.zeros(257, dtype=torch.bfloat16), torch.zeros(16, 16)]
+    opt = ops.AdamW(ps, state_bits=8)
+    assert opt.offsets == [0, 256, 256, 768] and opt.total == 1024
+    assert opt.exp_avg.dtype == torch.float8_e4m3fn and opt.exp_avg_sq.dtype == torch.float8_e5m2 and opt.exp_avg_scale.shape == (4,)
+    other = ops.AdamW(ps, state_bits=8, seed=3)
+    opt.exp_avg.view(torch.uint8).fill_(0x38)
+    opt.exp_avg_scale.fill_(0.5)
+    opt._clock[0] = 7
+    other.load_state_dict(opt.state_dict())
+    assert other.steps == 7 and other.seed == 0 and other._clock[1].item() == float(np.float32(0.9)) ** 7
+    assert torch.equal(other.moments(2)[0], torch.full((257,), 0.5))  # code 0x38 of e4m3 is 1
+
+
+def test_entry_point_refuses_bad_arguments():
+    """The C entry point's own checks (host code: no GPU is needed to be refused)."""
+    L = _lib.lib()
+    t = (_lib.AdamwTensor * 1)()
+    st = _lib.AdamwState(1 << 20, 1 << 20, 1 << 20, 1 << 20, 1 << 20, 512, 32, 0)
+    t[0].param = t[0].grad = 1 << 20
+    t[0].n, t[0].offset = 300, 0
+
+    def call(**kw):
+        s = _lib.AdamwState.from_buffer_copy(st)
+        row = (_lib.AdamwTensor * 1).from_buffer_copy(t)
+        for k, v in kw.items():
+            if hasattr(s, k):
+                setattr(s, k, v)
+            elif hasattr(row[0], k):
+                setattr(row[0], k, v)
+        return L.pin_adamw_step(row, 1, C.byref(s), kw.get("beta1", 0.9), 0.99, 1e-15, 0, None)
+    for bad in (dict(state_bits=16), dict(clock=None), dict(exp_avg=None), dict(beta1=1.0), dict(n=600), dict(n=-1), dict(offset=128),
+                dict(offset=256), dict(param=None), dict(grad=None), dict(param_dtype=3), dict(grad_dtype=-1), dict(total=256), dict(n=0)):
+        assert call(**bad) < 0, bad
+        assert _lib.lib().pin_last_error()
+    assert call(state_bits=8, exp_avg_scale=None) < 0
+
+
+# ------------------------------------------------------------------------------------------------ on the GPU
+SIZES = [1, 255, 256, 257, 2047, 2049, 70001]
+
+
+def _tensors(sizes, dtype, seed, scale=1.0, shift=0):
+    """Views of one buffer; with `shift` they begin at odd elements (no 16-byte border)."""
+    gen = torch.Generator().manual_seed(seed)
+    at, starts = shift, []
+    for n in sizes:
+        starts.append(at)
+        at += n + (shift if (n + shift) % 2 else 0)
+    flat = (torch.randn(at + 8, generator=gen) * scale).to(dtype).cuda()
+    return [flat[a:a + n] for a, n in zip(starts, sizes)]
+
+
+@gpu
+@pytest.mark.parametrize("shift", [0, 1, 3])
+def test_fp32_without_decay_is_adam_step_bit_for_bit(shift):
+    ps, gs = _tensors(SIZES, torch.float32, 1, shift=shift), _tensors(SIZES, torch.float32, 2, 1e-3, shift)
+    opt = ops.AdamW(ps, gs)
+    ref = [[p.clone(), torch.zeros_like(p), torch.zeros_like(p)] for p in ps]
+    for t in range(1, 5):
+        opt.step()
+        for r, g in zip(ref, gs):
+            ops.adam_step(r[0], g.clone(), r[1], r[2], t)
+    for i, r in enumerate(ref):
+        m, v = opt.moments(i)
+        assert torch.equal(ps[i], r[0]) and torch.equal(m, r[1]) and torch.equal(v, r[2]), SIZES[i]
+    assert opt.steps == 4
+
+
+def _formula(p, g, m, v, t, lr, b1, b2, eps, wd):
+    b1, b2, lr = (float(np.float32(x)) for x in (b1, b2, lr))
+    m = m + (g - m) * (1 - b1)
+    v = v * b2 + (1 - b2) * g * g
+    step = lr / (1 - b1 ** t) * m / (v.sqrt() / math.sqrt(1 - b2 ** t) + eps)
+    return p * (1 - lr * float(np.float32(wd))) - step, m, v, step
+
+
+@gpu
+@pytest.mark.parametrize("pd", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("gd", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_types_against_the_formula(pd, gd, shift):
+    """fp32 arithmetic: m and v carry 3 roundings a step; the step itself 5 more; p two of its own and, stored, half a step of its type."""
+    ps, gs = _tensors(SIZES, pd, 3, shift=shift), _tensors(SIZES, gd, 4, 1e-2, shift)
+    decay = [0.1 * (i % 3) for i in range(len(ps))]
+    before = [p.clone().double() for p in ps]
+    opt = ops.AdamW(ps, gs, lr=0.02, betas=(0.8, 0.95), eps=1e-8, weight_decay=decay)
+    opt.step()
+    for i, (p, b, g) in enumerate(zip(ps, before, gs)):
+        want, m, v, step = _formula(b, g.double(), torch.zeros_like(b), torch.zeros_like(b), 1, 0.02, 0.8, 0.95, 1e-8, decay[i])
+        gm, gv = opt.moments(i)
+        assert ((gm.double() - m).abs() <= 3 * F32 * m.abs()).all()
+        assert ((gv.double() - v).abs() <= 4 * F32 * v.abs()).all()
+        # (fp16: below its smallest normal number half a step is 2^-25)
+        tol = torch.finfo(pd).eps / 2 * want.abs() + (2.0 ** -25 if pd == torch.float16 else 0) + 4 * F32 * b.abs() + 12 * F32 * step.abs()
+        assert ((p.double() - want).abs() <= tol).all(), (i, ((p.double() - want).abs() / tol).max())
+
+
+def _values(dtype):
+    """The format's non-negative finite values in order of their codes."""
+    v = torch.arange(128, dtype=torch.uint8).view(dtype).double().numpy()
+    return v[np.isfinite(v)]
+
+
+def _mixed(h):
+    h = np.asarray(h, np.uint64)
+    h = h ^ (h >> np.uint64(16))
+    h = (h * np.uint64(0x9E3779B1)) & np.uint64(0xFFFFFFFF)
+    h = h ^ (h >> np.uint64(15))
+    h = (h * np.uint64(0xB7E15163)) & np.uint64(0xFFFFFFFF)
+    return h ^ (h >> np.uint64(16))
+
+
+def _codes(value, dtype, dither):
+    """(value the code stands for over its scale, scale, undecided): value between two numbers of the format goes up where the part
+    of the way it has come plus the dither reach 1.  undecided: within the rounding of that sum (float32 below 16) of the border."""
+    table = _values(dtype)
+    size = np.abs(value).reshape(-1, BLOCK)
+    largest = size.max(1, keepdims=True)
+    with np.errstate(divide="ignore"):
+        e = np.ceil(np.log2(largest / table[-1]))
+    e = np.maximum(np.where(largest == 0, -100, e), -100)
+    scale = 2.0 ** e
+    x = (size / scale).reshape(-1)
+    lo = np.searchsorted(table, x, side="right") - 1
+    hi = np.minimum(lo + 1, len(table) - 1)
+    gap = np.where(hi > lo, table[hi] - table[lo], 1.0)
+    part = (x - table[lo]) / gap + dither
+    code = np.where(part >= 1, hi, lo)
+    if dtype == torch.float8_e5m2:
+        code = np.where((value > 0) & (code == 0), 1, code)
+    return np.sign(value) * table[code], scale.reshape(-1), np.abs(part - 1) < 2.0 ** -19
+
+
+@gpu
+@pytest.mark.parametrize("spread", [0.0, 3.0])
+def test_8_bit_codes_against_the_table_of_their_values(spread):
+    rng = np.random.RandomState(5)
+    sizes = [1, 300, 4096, 5000]
+    ps = _tensors(sizes, torch.float32, 6)
+    gs = _tensors(sizes, torch.float32, 7)
+    for g in gs:
+        g.mul_(torch.from_numpy(np.exp(spread * rng.randn(g.numel())).astype(np.float32)).cuda())
+    gs[2][::7] = 0
+    opt = ops.AdamW(ps, gs, state_bits=8, seed=77)
+    n = opt.total
+    inside = np.zeros(n, bool)
+    for a, s in zip(opt.offsets, sizes):
+        inside[a:a + s] = True
+    b1, b2 = np.float32(0.9), np.float32(0.99)
+    g = np.zeros(n, np.float32)
+    for a, x in zip(opt.offsets, gs):
+        g[a:a + x.numel()] = x.cpu().numpy()
+    for t in range(1, 4):
+        m = (opt.exp_avg.float().cpu().numpy().reshape(-1, BLOCK) * opt.exp_avg_scale.cpu().numpy()[:, None]).reshape(-1)
+        v = (opt.exp_avg_sq.float().cpu().numpy().reshape(-1, BLOCK) * opt.exp_avg_sq_scale.cpu().numpy()[:, None]).reshape(-1)
+        opt.step()
+        m = m + (g - m) * (np.float32(1) - b1)
+        v = v * b2 + (np.float32(1) - b2) * g * g
+        h = _mixed(np.arange(n) ^ int(_mixed(int(_mixed(77)) ^ t)))
+        for x, got, scale, dtype, u in ((m, opt.exp_avg, opt.exp_avg_scale, torch.float8_e4m3fn, h & np.uint64(0xFFFF)),
+                                        (v, opt.exp_avg_sq, opt.exp_avg_sq_scale, torch.float8_e5m2, h >> np.uint64(16))):
+            want, s, open_ = _codes(x.astype(np.float64), dtype, u.astype(np.float64) / 65536)
+            assert np.array_equal(scale.cpu().numpy(), s)
+            same = got.double().cpu().numpy() == want
+            assert (same | open_).all() and open_.mean() < 1e-3
+        assert not opt.exp_avg.float().cpu().numpy()[~inside].any() and not opt.exp_avg_sq.float().cpu().numpy()[~inside].any()
+        assert (opt.exp_avg_sq.float().cpu().numpy()[v > 0] > 0).all()
+
+
+@gpu
+def test_8_bit_rounding_is_unbiased_and_repeats():
+    """The mean of the decoded moments of N equal elements: each is one of two neighbours, so its deviation is at most half their
+    distance, and the mean's 1 / sqrt(N) of that; 6 of those are allowed.  (The first element of a block sets the scale.)"""
+    n = 256 * 2000
+    def run(seed):
+        p = torch.zeros(n, device="cuda")
+        g = torch.full((n,), 0.37, device="cuda")
+        g[::256] = 1.0
+        opt = ops.AdamW([p], [g], state_bits=8, seed=seed)
+        opt.step()
+        return opt, p
+    a, pa = run(1)
+    b, pb = run(1)
+    c, _ = run(2)
+    assert torch.equal(a.exp_avg.view(torch.uint8), b.exp_avg.view(torch.uint8)) and torch.equal(pa, pb)
+    assert torch.equal(a.exp_avg_sq.view(torch.uint8), b.exp_avg_sq.view(torch.uint8))
+    assert not torch.equal(a.exp_avg.view(torch.uint8), c.exp_avg.view(torch.uint8))
+    keep = torch.ones(n, dtype=torch.bool, device="cuda")
+    keep[::256] = False
+    for got, want in zip(a.moments(0), (0.37 * (1 - float(np.float32(0.9))), 0.37 ** 2 * (1 - float(np.float32(0.99))))):
+        x = got[keep].double()
+        kinds = x.unique()
+        assert kinds.numel() == 2 and kinds[0] < want < kinds[1]
+        assert abs(x.mean().item() - want) < 6 * 0.5 * (kinds[1] - kinds[0]).item() / math.sqrt(x.numel()) + 4 * F32 * want
+
+
+@gpu
+@pytest.mark.parametrize("bits", [8, 32])
+def test_many_tensors_of_mixed_types_count_one_step(bits):
+    """150 tensors of all type pairs, some empty, some without a gradient: several launches, one step."""
+    kinds = [torch.float32, torch.bfloat16, torch.float16]
+    sizes = [(i * 37) % 600 for i in range(150)]
+    ps = [torch.randn(n, device="cuda").to(kinds[i % 3]) for i, n in enumerate(sizes)]
+    gs = [None if i % 11 == 5 else ((torch.rand(n, device="cuda") + 0.5) * torch.randn(n, device="cuda").sign()).to(kinds[(i // 3) % 3]) for i, n in enumerate(sizes)]
+    before = [p.clone() for p in ps]
+    opt = ops.AdamW(ps, gs, state_bits=bits)
+    opt.step()
+    opt.step()
+    assert opt.steps == 2 and opt._clock[_lib.PIN_ADAMW_CLOCK_DOUBLES - 4].item() == 0
+    for p, b, g in zip(ps, before, gs):
+        if g is None:
+            assert torch.equal(p, b)
+        else:  # step 1 of Adam moves every element by lr, whatever its gradient; two equal gradients by 2 lr
+            off = (b.double() - 0.02 * g.double().sign() - p.double()).abs()
+            # (the 8-bit moments' second step: m and sqrt(v) are each within a code's spacing, 1/8 and 1/4 / 2)
+            assert (off <= torch.finfo(p.dtype).eps * (b.double().abs() + 0.02) + 2.0 ** -24 + (0.01 * 0.4 if bits == 8 else 1e-6)).all()
+
+
+@gpu
+def test_zero_grad_and_replaced_buffers():
+    p, g = torch.ones(1000, device="cuda"), torch.ones(1000, device="cuda")
+    opt = ops.AdamW([p], [g], state_bits=8)
+    opt.step(zero_grad=True)
+    assert not g.any()
+    g.data = torch.full((1000,), 2.0, device="cuda")  # another buffer behind the same tensor
+    opt.step()
+    assert (g == 2).all() and (opt.moments(0)[0] > 0.1).all()
+    opt.step([torch.full((1000,), -4.0, device="cuda")])
+    assert opt.steps == 3 and (opt.moments(0)[0] < 0.1).all()
+
+
+@gpu
+@pytest.mark.parametrize("bits", [8, 32])
+def test_captured_step_counts_on(bits):
+    """Replays of a captured step, with eager work and changes of lr between them, equal the eager steps bit for bit."""
+    def make():
+        torch.manual_seed(3)
+        ps = [torch.randn(n, device="cuda") for n in (5, 1000, 70000)]
+        gs = [torch.randn_like(p) for p in ps]
+        return ps, gs, ops.AdamW(ps, gs, state_bits=bits, weight_decay=0.1, seed=9)
+    pe, ge, eager = make()
+    pc, gc, captured = make()
+    graph = torch.cuda.CUDAGraph()
+    captured.step()
+    eager.step()
+    with torch.cuda.graph(graph):
+        captured.step()
+    for k in range(4):
+        if k == 2:
+            eager.lr = captured.lr = 0.003
+        for a, b in zip(ge, gc):
+            a.mul_(1.5)
+            b.mul_(1.5)
+        graph.replay()
+        eager.step()
+        torch.cuda.synchronize()
+        assert captured.steps == eager.steps == k + 2
+        for a, b in zip(pe, pc):
+            assert torch.equal(a, b), k
+        assert torch.equal(eager.exp_avg_sq.view(torch.uint8), captured.exp_avg_sq.view(torch.uint8))
+
+
+@gpu
+@pytest.mark.parametrize("bits", [8, 32])
+def test_checkpoint_resumes_on_another_stream(bits):
+    torch.manual_seed(4)
+    p, g = torch.randn(3000, device="cuda"), torch.randn(3000, device="cuda")
+    a = ops.AdamW([p], [g], state_bits=bits, seed=5, lr=0.02)
+    a.step()
+    q, d = p.clone(), a.state_dict()
+    a.step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        b = ops.AdamW([q], [g], state_bits=bits)
+        b.load_state_dict(d)
+        b.step()
+    side.synchronize()
+    assert torch.equal(p, q) and torch.equal(a.exp_avg.view(torch.uint8), b.exp_avg.view(torch.uint8)) and a.steps == b.steps == 2
+
+
+@gpu
+def test_a_gradient_that_is_not_finite_is_seen():
+    """32 bits: the element alone.  8 bits: its block of 256 from the next step on (they share a scale), never silently a number."""
+    for bits in (32, 8):
+        p, g = torch.ones(600, device="cuda"), torch.ones(600, device="cuda")
+        g[300] = float("nan")
+        opt = ops.AdamW([p], [g], state_bits=bits)
+        opt.step()
+        assert p.isnan().nonzero().flatten().tolist() == [300]
+        g[300] = 1.0
+        opt.step()
+        assert p.isnan().nonzero().flatten().tolist() == ([300] if bits == 32 else list(range(256, 512)))
