@@ -368,6 +368,7 @@ const char* pin_last_error(void);
  * read-back (PIN_GN_STATE_STATUS), so Tracker.tracking hears about a flag without an extra read-back. */
 #define PIN_STATUS_FP16_RANGE 1  /* pin_stage_decoder met a decoder parameter of magnitude >= 65504 or a non-finite one: the
                                   * split-fp16 image cannot hold it (mlp_h2.h); PIN_MLP=f32 selects the fp32 image */
+#define PIN_STATUS_LABEL_RANGE 2 /* pin_vocab_nll* met a label that is not below the number of labels: its nll is NaN, its gradient 0 */
 int         pin_status(int32_t* flags_out, int32_t clear, void* stream);
 
 /* host helper: cand_off_host[c] = (dx.primes) mod buffer_size, primes = (73856093,
@@ -1138,6 +1139,40 @@ typedef struct pin_adamw_state {
 /* tensors_host is a HOST array, read before the call returns.  At least one tensor must have elements. */
 int pin_adamw_step(const pin_adamw_tensor* tensors_host, int32_t n_tensors, const pin_adamw_state* st, float beta1, float beta2,
                    float eps, uint32_t seed, void* stream);
+
+/* ---- a linear head over a LARGE label set (csrc/vocab.hip) ---------------------------------------------------------------------
+ * What pin_train_sem_step / pin_sem_query do for 2..32 heads of the map's decoder (Decoder.sem_label_prob, model/decoder.py:100-103;
+ * the NLL term, utils/mapper.py:782-800), for any features x [n][dim] and any number of labels: s = x W^T + b, log-softmax,
+ * NLL and its gradients, or the most probable label -- without the n x vocab logits in memory.
+ * x, weight and bias are of one type (PIN_F32, PIN_BF16, PIN_F16); sums, maxima and statistics are fp32.  A bias of -inf (or
+ * below -1e30) switches a label off.  A row whose labels are all switched off has lse -inf, nll +inf, gradient 0 and the label -1. */
+#define PIN_VOCAB_MAX (1 << 24)      /* largest n, vocab */
+#define PIN_VOCAB_MAX_DIM (1 << 16)  /* largest dim */
+typedef struct pin_vocab_head {
+    const void* x;           /* [n][dim], row stride x_stride elements */
+    const void* weight;      /* [vocab][dim], row stride weight_stride */
+    const void* bias;        /* [vocab] or NULL */
+    int64_t x_stride, weight_stride;
+    int32_t n, vocab, dim, dtype;
+} pin_vocab_head;
+/* bytes of the workspace of the calls below (device memory, from a multiple of 256 on); gradients: 0 for pin_vocab_nll and
+ * pin_vocab_predict, 1 for pin_vocab_nll_grad and pin_vocab_nll_step.  -1: a size that is not supported. */
+int64_t pin_vocab_workspace_bytes(int32_t n, int32_t vocab, int32_t dim, int32_t dtype, int32_t gradients);
+/* nll_out[i] = lse_i - s_i,labels[i] (0 where labels[i] < 0: no label), lse_out[i] = log sum_v exp s_iv.  A label >= vocab gives
+ * nll NaN and raises PIN_STATUS_LABEL_RANGE. */
+int pin_vocab_nll(const pin_vocab_head* h, const int32_t* labels, float* nll_out, float* lse_out, void* workspace, int64_t workspace_bytes,
+                  void* stream);
+/* Gradients of sum_i grad_nll[i] nll_i, with the lse of pin_vocab_nll: dx [n][dim], dweight [vocab][dim], dbias [vocab] (or NULL),
+ * contiguous, of the head's type, WRITTEN (not added).  Rows without a label take no part, whatever they hold. */
+int pin_vocab_nll_grad(const pin_vocab_head* h, const int32_t* labels, const float* lse, const float* grad_nll, void* dx, void* dweight,
+                       void* dbias, void* workspace, int64_t workspace_bytes, void* stream);
+/* The two in one call (the operands are laid out once); the same bits. */
+int pin_vocab_nll_step(const pin_vocab_head* h, const int32_t* labels, const float* grad_nll, float* nll_out, float* lse_out, void* dx,
+                       void* dweight, void* dbias, void* workspace, int64_t workspace_bytes, void* stream);
+/* label_out[i] = the lowest label of the largest logit, logprob_out[i] = its log-probability; a row without a finite sum of
+ * exponentials (all labels switched off, a logit that is NaN or +inf) has the label -1. */
+int pin_vocab_predict(const pin_vocab_head* h, int32_t* label_out, float* logprob_out, void* workspace, int64_t workspace_bytes,
+                      void* stream);
 
 #ifdef __cplusplus
 }

@@ -24,6 +24,8 @@ PIN_ADAM_ROW_EXCLUDED = -(1 << 31)
 PIN_COMM_ID_BYTES = 128
 PIN_F32, PIN_BF16, PIN_F16 = 0, 1, 2
 PIN_ADAMW_BLOCK = 256
+PIN_VOCAB_MAX = 1 << 24
+PIN_VOCAB_MAX_DIM = 1 << 16
 PIN_ADAMW_CLOCK_DOUBLES = 8
 
 vp = C.c_void_p
@@ -84,6 +86,7 @@ class GnLoopParams(C.Structure):
 PIN_GN_STATE_DOUBLES = 80
 PIN_GN_STATE_STATUS = 61
 PIN_STATUS_FP16_RANGE = 1
+PIN_STATUS_LABEL_RANGE = 2
 
 
 class MapArrays(C.Structure):
@@ -162,6 +165,11 @@ class AdamwTensor(C.Structure):
 class AdamwState(C.Structure):
     _fields_ = [("exp_avg", vp), ("exp_avg_sq", vp), ("exp_avg_scale", vp), ("exp_avg_sq_scale", vp), ("clock", vp), ("total", C.c_int64),
                 ("state_bits", C.c_int32), ("zero_grad", C.c_int32)]
+
+
+class VocabHead(C.Structure):
+    _fields_ = [("x", vp), ("weight", vp), ("bias", vp), ("x_stride", C.c_int64), ("weight_stride", C.c_int64), ("n", C.c_int32),
+                ("vocab", C.c_int32), ("dim", C.c_int32), ("dtype", C.c_int32)]
 
 
 class PreprocessParams(C.Structure):
@@ -305,6 +313,11 @@ SIGNATURES = {
     "pin_dp_cert_delta": (i32, [vp, vp, vp, i32, vp]),
     "pin_dp_cert_apply": (i32, [vp, vp, vp, i32, vp]),
     "pin_dp_sync_side_effects": (i32, [vp, vp, vp, vp, vp, i32, vp]),
+    "pin_vocab_workspace_bytes": (i64, [i32, i32, i32, i32, i32]),
+    "pin_vocab_nll": (i32, [P(VocabHead), vp, vp, vp, vp, i64, vp]),
+    "pin_vocab_nll_grad": (i32, [P(VocabHead), vp, vp, vp, vp, vp, vp, vp, i64, vp]),
+    "pin_vocab_nll_step": (i32, [P(VocabHead), vp, vp, vp, vp, vp, vp, vp, vp, i64, vp]),
+    "pin_vocab_predict": (i32, [P(VocabHead), vp, vp, vp, i64, vp]),
     "pin_adamw_step": (i32, [P(AdamwTensor), i32, P(AdamwState), f32, f32, f32, C.c_uint32, vp]),
 }
 

@@ -64,6 +64,9 @@ def raise_on_status(flags: int):
     if flags & _lib.PIN_STATUS_FP16_RANGE:
         status(clear=True)
         raise RuntimeError(FP16_RANGE_MESSAGE)
+    if flags & _lib.PIN_STATUS_LABEL_RANGE:
+        status(clear=True)
+        raise RuntimeError("a label is not below the number of labels of its head (vocab_nll / vocab_nll_step: its nll is NaN, its gradient 0)")
 
 
 def _stream():
@@ -882,10 +885,122 @@ def gather_rows(src: torch.Tensor, index: torch.Tensor, out: Optional[torch.Tens
     return out
 
 
-# ------------------------------------------------------------------------------- AdamW over many tensors (csrc/adamw.hip)
+# ------------------------------------------------------------------------------- a head over a large label set (csrc/vocab.hip)
 _DTYPE_CODES = {torch.float32: _lib.PIN_F32, torch.bfloat16: _lib.PIN_BF16, torch.float16: _lib.PIN_F16}
 
 
+def _vocab_head(x, weight, bias):
+    """The head's struct after the checks of its tensors.  Rows may be strided (the columns not)."""
+    if x.dim() != 2 or weight.dim() != 2 or x.shape[1] != weight.shape[1]:
+        raise RuntimeError(f"x [n, dim] and weight [vocab, dim] are needed, got {tuple(x.shape)} and {tuple(weight.shape)}")
+    if weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise RuntimeError("a head needs at least one label and one feature")
+    if x.dtype not in _DTYPE_CODES:
+        raise RuntimeError(f"float32, bfloat16 or float16 is needed, got {x.dtype}")
+    tensors = [("weight", weight)] + ([("bias", bias)] if bias is not None else [])
+    for name, t in tensors:
+        if t.dtype != x.dtype or t.device != x.device:
+            raise RuntimeError(f"{name} is {t.dtype} on {t.device}, x is {x.dtype} on {x.device}")
+    if bias is not None and bias.shape != (weight.shape[0],):
+        raise RuntimeError(f"bias {tuple(bias.shape)} for {weight.shape[0]} labels")
+    n, dim = x.shape
+    for name, t in (("x", x), ("weight", weight)):
+        if not t.is_cuda:
+            raise RuntimeError("libpinhip needs device (HIP) tensors; there is no CPU path")
+        if t.shape[0] > 1 and (t.stride(0) < dim or (dim > 1 and t.stride(1) != 1)) or (t.shape[0] == 1 and dim > 1 and t.stride(1) != 1):
+            raise RuntimeError(f"{name}: the features of a row must be contiguous and its rows must not overlap, got strides {t.stride()}")
+    if max(n, weight.shape[0]) > _lib.PIN_VOCAB_MAX or dim > _lib.PIN_VOCAB_MAX_DIM:
+        raise RuntimeError(f"at most {_lib.PIN_VOCAB_MAX} rows and labels and {_lib.PIN_VOCAB_MAX_DIM} features")
+    h = _lib.VocabHead()
+    h.x, h.weight, h.bias = x.data_ptr(), weight.data_ptr(), _ptr(bias)
+    h.x_stride, h.weight_stride = max(x.stride(0), dim) if n > 1 else dim, max(weight.stride(0), dim) if weight.shape[0] > 1 else dim
+    h.n, h.vocab, h.dim, h.dtype = n, weight.shape[0], dim, _DTYPE_CODES[x.dtype]
+    return h
+
+
+def _vocab_rows(name, t, x, dtype):
+    if t.shape != (x.shape[0],) or t.device != x.device:
+        raise RuntimeError(f"{name} {tuple(t.shape)} on {t.device} for {x.shape[0]} rows on {x.device}")
+    return _ptr(t, dtype)
+
+
+def _vocab_workspace(h, gradients, ws, device):
+    need = int(_lib.lib().pin_vocab_workspace_bytes(h.n, h.vocab, h.dim, h.dtype, int(gradients)))
+    if ws is None:
+        return torch.empty((max(need, 1),), dtype=torch.uint8, device=device)
+    if ws.dtype != torch.uint8 or ws.device != device or ws.numel() < need:
+        raise RuntimeError(f"the workspace must hold {need} bytes (uint8) on {device}")
+    return ws
+
+
+def vocab_workspace(n: int, vocab: int, dim: int, dtype=torch.float32, gradients: bool = True, device="cuda") -> torch.Tensor:
+    """A workspace for vocab_* calls of these sizes, for callers that keep one (one call at a time may use it)."""
+    need = int(_lib.lib().pin_vocab_workspace_bytes(int(n), int(vocab), int(dim), _DTYPE_CODES[dtype], int(bool(gradients))))
+    if need < 0:
+        raise ValueError("sizes out of range")
+    return torch.empty((max(need, 1),), dtype=torch.uint8, device=device)
+
+
+def vocab_nll(x, weight, bias, labels, ws=None):
+    """Negative log-likelihood of a linear head over a large label set: (nll [n], lse [n]) float32 with
+    lse_i = log sum_v exp(x_i . weight_v + bias_v) and nll_i = lse_i - logit of labels[i]; 0 where labels[i] < 0 (no label).
+    x [n, dim], weight [vocab, dim], bias [vocab] or None: one of float32 / bfloat16 / float16; labels int32.  The logits are
+    never held.  A bias of -inf (or below -1e30) switches a label off; a row without any label left has lse -inf, nll inf.
+    A label >= vocab gives nll NaN and raises a flag that raise_on_status(status()) turns into an error."""
+    h = _vocab_head(x, weight, bias)
+    lab = _vocab_rows("labels", labels, x, torch.int32)
+    nll, lse = (torch.empty((h.n,), dtype=torch.float32, device=x.device) for _ in range(2))
+    with _device_of(x.device):
+        ws = _vocab_workspace(h, False, ws, x.device)
+        check(_lib.lib().pin_vocab_nll(C.byref(h), lab, nll.data_ptr(), lse.data_ptr(), ws.data_ptr(), ws.numel(), _stream()), "pin_vocab_nll")
+    return nll, lse
+
+
+def _vocab_gradients(x, weight, bias):
+    return (torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty(weight.shape, dtype=x.dtype, device=x.device),
+            None if bias is None else torch.empty(bias.shape, dtype=x.dtype, device=x.device))
+
+
+def vocab_nll_grad(x, weight, bias, labels, lse, grad_nll, ws=None):
+    """Gradients of sum_i grad_nll[i] nll_i (float32 [n]) with the lse of vocab_nll: (dx, dweight, dbias), of the head's type,
+    contiguous, written anew.  Rows without a label (labels < 0) take no part, whatever they hold."""
+    h = _vocab_head(x, weight, bias)
+    lab, l, g = _vocab_rows("labels", labels, x, torch.int32), _vocab_rows("lse", lse, x, torch.float32), _vocab_rows("grad_nll", grad_nll, x, torch.float32)
+    dx, dw, db = _vocab_gradients(x, weight, bias)
+    with _device_of(x.device):
+        ws = _vocab_workspace(h, True, ws, x.device)
+        check(_lib.lib().pin_vocab_nll_grad(C.byref(h), lab, l, g, dx.data_ptr(), dw.data_ptr(), _ptr(db), ws.data_ptr(), ws.numel(), _stream()),
+              "pin_vocab_nll_grad")
+    return dx, dw, db
+
+
+def vocab_nll_step(x, weight, bias, labels, grad_nll, ws=None):
+    """vocab_nll and vocab_nll_grad in one call (the operands are laid out once; the same bits): (nll, lse, dx, dweight, dbias)."""
+    h = _vocab_head(x, weight, bias)
+    lab, g = _vocab_rows("labels", labels, x, torch.int32), _vocab_rows("grad_nll", grad_nll, x, torch.float32)
+    nll, lse = (torch.empty((h.n,), dtype=torch.float32, device=x.device) for _ in range(2))
+    dx, dw, db = _vocab_gradients(x, weight, bias)
+    with _device_of(x.device):
+        ws = _vocab_workspace(h, True, ws, x.device)
+        check(_lib.lib().pin_vocab_nll_step(C.byref(h), lab, g, nll.data_ptr(), lse.data_ptr(), dx.data_ptr(), dw.data_ptr(), _ptr(db),
+                                            ws.data_ptr(), ws.numel(), _stream()), "pin_vocab_nll_step")
+    return nll, lse, dx, dw, db
+
+
+def vocab_predict(x, weight, bias=None, ws=None):
+    """The most probable label of every row (int32, the lowest of equal ones) and its log-probability (float32): (label [n],
+    logprob [n]).  Types and switched-off labels as in vocab_nll; a row without a finite sum of exponentials has the label -1."""
+    h = _vocab_head(x, weight, bias)
+    label = torch.empty((h.n,), dtype=torch.int32, device=x.device)
+    logprob = torch.empty((h.n,), dtype=torch.float32, device=x.device)
+    with _device_of(x.device):
+        ws = _vocab_workspace(h, False, ws, x.device)
+        check(_lib.lib().pin_vocab_predict(C.byref(h), label.data_ptr(), logprob.data_ptr(), ws.data_ptr(), ws.numel(), _stream()),
+              "pin_vocab_predict")
+    return label, logprob
+
+
+# ------------------------------------------------------------------------------- AdamW over many tensors (csrc/adamw.hip)
 class AdamW:
     """One AdamW step over many tensors per call (pin_adamw_step): decoupled weight decay, moments of 32 or of 8 bits.
 
