@@ -1166,7 +1166,8 @@ int pin_vocab_nll(const pin_vocab_head* h, const int32_t* labels, float* nll_out
  * contiguous, of the head's type, WRITTEN (not added).  Rows without a label take no part, whatever they hold. */
 int pin_vocab_nll_grad(const pin_vocab_head* h, const int32_t* labels, const float* lse, const float* grad_nll, void* dx, void* dweight,
                        void* dbias, void* workspace, int64_t workspace_bytes, void* stream);
-/* The two in one call (the operands are laid out once); the same bits. */
+/* The two in one call: the operands are laid out once, and the probabilities are formed from the maximum and the sum of the
+ * forward pass rather than from the rounded lse. */
 int pin_vocab_nll_step(const pin_vocab_head* h, const int32_t* labels, const float* grad_nll, float* nll_out, float* lse_out, void* dx,
                        void* dweight, void* dbias, void* workspace, int64_t workspace_bytes, void* stream);
 /* label_out[i] = the lowest label of the largest logit, logprob_out[i] = its log-probability; a row without a finite sum of

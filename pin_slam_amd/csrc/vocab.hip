@@ -5,12 +5,14 @@
 // csrc/sem.h), without ever holding the n x V logits: the forward pass keeps a running maximum and sum a row, the gradient pass forms the
 // logits again in pieces of the vocabulary.
 //
-// Numerics.  Logits are kept in units of log 2 (one fused multiply-add, and exp2 is the instruction).  bf16 / fp16 inputs multiply
-// as they are, fp32 as two fp16 pieces of the value times a power of two per row (vocab_tile.h); sums, maxima and statistics are
-// fp32.  D is kept in fp16 times 2^14 / 2^floor(log2 max |g|): 11 bits down to 2^-28 of the largest (rounded to bf16 it would
-// cost as much error as the output's own rounding does), and the transposed x and W beside it in fp16 times a power of two of
-// the tensor, which holds bf16 exactly down to 2^-31 of its largest value; fp32 again as two pieces each.
-#include "vocab_tile.h"
+// Numerics.  bf16 / fp16 inputs multiply as they are, fp32 as two fp16 pieces of the value times a power of two per row
+// (vocab_tile.h); sums, maxima and statistics are fp32.  16-bit inputs keep their logits in units of log 2 (one fused multiply-add, and
+// exp2 is the instruction); fp32 keeps them as they are, where they are rounded half as coarsely.  p is formed from the
+// maximum and the sum (exp(s - m) / total), not from the rounded lse.  D is kept in fp16 times 2^14 / 2^ceil(log2 max |g|): 11 bits
+// down to 2^-28 of the largest (rounded to bf16 it would cost as much error as the output's own rounding does), and the transposed
+// x and W beside it in fp16 times a power of two of the tensor, which holds bf16 exactly down to 2^-31 of its largest value;
+// fp32 again as two pieces each.
+#include "vocab_stream.h"
 
 namespace pin {
 
@@ -24,7 +26,7 @@ struct VocabArgs {
     const void* bias;
     long ldx, ldw;
     int n, V, d;
-    int dk, nk, Vk;          // padded to 64; Vk to 128
+    int dk, nk, Vk;          // d padded to 64, n and V to 128
     const int* labels;
     const float* grad_nll;
     float* nll;
@@ -40,9 +42,13 @@ struct VocabArgs {
     float *amax;             // [3][V_AMAX] partial maxima of |x|, |W|, |g|
     float *part_m, *part_s;  // [splits][nk]
     int* part_i;
-    float *tlogit, *lse2, *gs;
-    float* dxp;              // [dx_splits][nk][d]
-    int splits, tiles_per_split, dx_splits, piece;
+    float* tlogit;
+    float *gm, *gc, *gn, *g; // of a row: reference of the exponent, its offset, the upstream gradient scaled below 1 and as it is
+    int* part;               // its label, -1 where it takes no part in the gradient
+    int* bad;                // 1: no label and not finite (its copy in xa is zero)
+    float *dxp, *dwp, *dbp;  // partial sums [splits][nk][dk], [splits][Vk][dk], [splits][Vk]
+    int splits, tiles_per_split, dx_splits, dw_splits, piece;
+    int order;               // 1: the transposed operands in the order of v_stream_row
     int* status;
 };
 
@@ -85,44 +91,65 @@ __device__ float v_block_max(const float* part, float* sh) {  // the maximum of 
 
 __device__ __forceinline__ bool v_takes_part(const VocabArgs& a, long row) { return a.labels[row] >= 0 && a.labels[row] < a.V; }
 
-// Staging, first launch: one wave a row.  The largest |x|, |W|, |g|; the padded bias in units of log 2 (-inf: excluded, and behind the
-// last label); COPY: the operand of the logit product (two scaled fp16 pieces of fp32; a padded copy of rows that are not aligned).
-template <int D, bool COPY>
-__global__ __launch_bounds__(256) void vocab_rows_kernel(VocabArgs a, int scan) {  // scan: the rows are needed at all (maxima or copies)
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    float mx = 0.f, mw = 0.f, mg = 0.f;
-    for (long r = scan ? (long)blockIdx.x * 4 + wave : (long)a.n + a.V; r < (long)a.n + a.V; r += (long)gridDim.x * 4) {
-        const bool is_x = r < a.n;
-        const long row = is_x ? r : r - a.n;
-        const void* src = is_x ? a.x : a.w;
-        const long at = row * (is_x ? a.ldx : a.ldw);
-        float m = 0.f;
-        for (int k = lane; k < a.d; k += 64) m = fmaxf(m, fabsf(v_get<D>(src, at + k)));
-        if constexpr (COPY) {
-            unsigned short* out = (is_x ? a.xa : a.wa) + row * a.dk;
-            const long plane = (long)(is_x ? a.n : a.V) * a.dk;
-            if constexpr (D == PIN_F32) {
-                const int e = v_scale_exp(wave_max_f32(m));
-                for (int k = lane; k < a.dk; k += 64) {
-                    const float v = k < a.d ? ldexpf(v_get<D>(src, at + k), e) : 0.f;
-                    const unsigned short h = v_half(v);
-                    out[k] = h;
-                    out[plane + k] = v_half(v - v_from_half(h));
-                }
-                if (lane == 0) (is_x ? a.xs : a.ws_)[row] = ldexpf(is_x ? 1.f : V_LOG2E, -e);
-            } else {
-                for (int k = lane; k < a.dk; k += 64) out[k] = k < a.d ? reinterpret_cast<const unsigned short*>(src)[at + k] : (unsigned short)0;
-            }
+// Staging, first launch: one wave a row.  The largest |x| (of the rows that take part), |W|, |g|; the padded bias (-inf: switched off, and
+// behind the last label); the operand of the logit product where it has to be made (COPY_W: two scaled fp16 pieces of fp32, or a
+// padded copy of rows that are not aligned; x is always copied for the gradient: a row without a label that is not finite is zero
+// there, so that no kernel behind has to look for it).
+template <int D>
+__device__ __forceinline__ float v_stage_row(const VocabArgs& a, bool is_x, long row, bool copy) {
+    const int lane = threadIdx.x & 63;
+    const void* src = is_x ? a.x : a.w;
+    const long at = row * (is_x ? a.ldx : a.ldw);
+    float m = 0.f;
+    bool odd = false;
+    for (int k = lane; k < a.d; k += 64) {
+        const float v = fabsf(v_get<D>(src, at + k));
+        m = fmaxf(m, v);
+        odd |= !(v < INFINITY);
+    }
+    if (!copy) return m;
+    const bool zero = is_x && a.part != nullptr && !v_takes_part(a, row) && __any(odd);
+    if (is_x && a.part != nullptr && lane == 0) a.bad[row] = zero;
+    unsigned short* out = (is_x ? a.xa : a.wa) + row * a.dk;
+    if constexpr (D == PIN_F32) {
+        const long plane = (long)(is_x ? a.n : a.V) * a.dk;
+        const int e = zero ? 0 : v_scale_exp(wave_max_f32(m));
+        for (int k = lane; k < a.dk; k += 64) {
+            const float v = k < a.d && !zero ? ldexpf(v_get<D>(src, at + k), e) : 0.f;
+            const unsigned short h = v_half(v);
+            out[k] = h;
+            out[plane + k] = v_half(v - v_from_half(h));
         }
-        if (!is_x) mw = fmaxf(mw, m);
-        else if (a.labels == nullptr || v_takes_part(a, row)) mx = fmaxf(mx, m);
+        if (lane == 0) (is_x ? a.xs : a.ws_)[row] = ldexpf(1.f, -e);
+    } else {
+        for (int k = lane; k < a.dk; k += 64) out[k] = k < a.d && !zero ? reinterpret_cast<const unsigned short*>(src)[at + k] : (unsigned short)0;
     }
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < a.Vk; i += (long)gridDim.x * 256) {
+    return m;
+}
+template <int D>
+__global__ __launch_bounds__(256) void vocab_rows_kernel(VocabArgs a, int scan_w) {  // scan_w: W's largest value is wanted
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const bool copy_x = a.xa != nullptr, copy_w = a.wa != nullptr;
+    float mx = 0.f, mw = 0.f, mg = 0.f;
+    const long rx = copy_x ? a.n : 0, rw = copy_w || scan_w ? a.V : 0;
+    for (long r = (long)blockIdx.x * 4 + wave; r < rx + rw; r += (long)gridDim.x * 4) {
+        if (r < rx) {
+            const float m = v_stage_row<D>(a, true, r, true);
+            if (a.labels == nullptr || v_takes_part(a, r)) mx = fmaxf(mx, m);
+        } else {
+            mw = fmaxf(mw, v_stage_row<D>(a, false, r - rx, copy_w));
+        }
+    }
+    const long first = (long)blockIdx.x * 256 + threadIdx.x, stride = (long)gridDim.x * 256;
+    for (long i = first; i < a.Vk + 64; i += stride) {
         const float b = i >= a.V ? -INFINITY : a.bias == nullptr ? 0.f : v_get<D>(a.bias, i);
-        a.b2[i] = b <= V_FLOOR ? -INFINITY : b * V_LOG2E;
+        a.b2[i] = b <= V_FLOOR ? -INFINITY : D == PIN_F32 ? b : b * V_LOG2E;
+        if (D == PIN_F32 && i >= a.V) a.ws_[i] = 1.f;
     }
+    if (D == PIN_F32)
+        for (long i = a.n + first; i < a.nk + 64; i += stride) a.xs[i] = 1.f;
     if (a.grad_nll != nullptr)
-        for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < a.n; i += (long)gridDim.x * 256)
+        for (long i = first; i < a.n; i += stride)
             if (v_takes_part(a, i)) mg = fmaxf(mg, fabsf(a.grad_nll[i]));
     __shared__ float sh[3][4];
     mx = wave_max_f32(mx); mw = wave_max_f32(mw); mg = wave_max_f32(mg);
@@ -158,7 +185,7 @@ __global__ __launch_bounds__(256) void vocab_transpose_kernel(VocabArgs a, int x
     for (int i = threadIdx.x; i < 4096; i += 256) {
         const int k = i >> 6, r = i & 63;
         if (k0 + k >= a.d) continue;
-        const float v = ldexpf(tile[r][k], e);
+        const float v = ldexpf(tile[a.order ? (r & 32) + v_stream_row(r & 31) : r][k], e);
         const unsigned short h = v_half(v);
         const long at = (long)(k0 + k) * padded + r0 + r;
         out[at] = h;
@@ -166,27 +193,38 @@ __global__ __launch_bounds__(256) void vocab_transpose_kernel(VocabArgs a, int x
     }
 }
 
-// one logit in units of log 2: acc = W_v . x_i (times the two rows' powers of two for fp32)
+// one logit from the product: in units of log 2 (16-bit inputs), or as it is, times the two rows' powers of two (fp32)
 template <int SEGS>
 __device__ __forceinline__ float v_logit(float acc, float xs, float ws, float b2) {
     if constexpr (SEGS == 1) return fmaf(acc, V_LOG2E, b2);
     else return fmaf(acc, xs * ws, b2);
 }
+// exp of a difference of two of them
+template <int SEGS>
+__device__ __forceinline__ float v_exp(float diff) {
+    return __builtin_amdgcn_exp2f(SEGS == 1 ? diff : diff * V_LOG2E);
+}
+// 2^14 p of a logit that is still a product: `m` and `c` are gm and gc of its row
+template <int SEGS>
+__device__ __forceinline__ float v_prob(float acc, float xs, float ws, float b2, float m, float c) {
+    if constexpr (SEGS == 1) return __builtin_amdgcn_exp2f(fmaf(acc, V_LOG2E, b2 + c));
+    else return __builtin_amdgcn_exp2f(fmaf(fmaf(acc, xs * ws, b2) - m, V_LOG2E, c));
+}
 
-// the wave's 64 labels x 64 rows of logits: acc -> units of log 2
+// the wave's 64 labels x 64 rows of logits from their products
 template <int SEGS>
 __device__ __forceinline__ void v_logits(const VocabArgs& a, vt_f4 (&acc)[4][4], int v0, int i0) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
     const int vb = v0 + (wave >> 1) * 64 + 4 * g, ib = i0 + (wave & 1) * 64 + c;
     float xs[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) xs[j] = SEGS == 1 ? 1.f : a.xs[min(ib + 16 * j, a.n - 1)];
+    for (int j = 0; j < 4; ++j) xs[j] = SEGS == 1 ? 1.f : a.xs[ib + 16 * j];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const vt_f4 b2 = *reinterpret_cast<const vt_f4*>(a.b2 + vb + 16 * i);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const float ws = SEGS == 1 ? 1.f : a.ws_[min(vb + 16 * i + r, a.V - 1)];
+            const float ws = SEGS == 1 ? 1.f : a.ws_[vb + 16 * i + r];
 #pragma unroll
             for (int j = 0; j < 4; ++j) acc[i][j][r] = v_logit<SEGS>(acc[i][j][r], xs[j], ws, b2[r]);
         }
@@ -198,6 +236,15 @@ __device__ __forceinline__ VocabOperand v_operand_w(const VocabArgs& a) {
 }
 __device__ __forceinline__ VocabOperand v_operand_x(const VocabArgs& a) {
     return a.xa != nullptr ? VocabOperand{a.xa, a.dk, (long)a.n * a.dk, a.n} : VocabOperand{reinterpret_cast<const unsigned short*>(a.x), a.ldx, 0, a.n};
+}
+
+// (maximum, sum, lowest label of the maximum) of two sets of labels
+template <int SEGS>
+__device__ __forceinline__ void v_join(float& m1, float& s1, int& a1, float m2, float s2, int a2) {
+    const float top = fmaxf(m1, m2);
+    s1 = s1 * v_exp<SEGS>(m1 - top) + s2 * v_exp<SEGS>(m2 - top);
+    a1 = m1 > m2 ? a1 : m2 > m1 ? a2 : min(a1, a2);
+    m1 = top;
 }
 
 // Forward: workgroup (row tile, split of the vocabulary).  A lane keeps (maximum, sum, lowest label of the maximum) of its 4 rows
@@ -249,11 +296,11 @@ __global__ __launch_bounds__(256, 2) void vocab_forward_kernel(VocabArgs a) {
                             if (lab[j] >= 0 && lab[j] == vb + 16 * i + r) a.tlogit[ib + 16 * j] = acc[i][j][r];
                 }
             }
-            float sum = s[j] * exp2f(m[j] - top);
+            float sum = s[j] * v_exp<SEGS>(m[j] - top);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f(acc[i][j][r] - top);
+                for (int r = 0; r < 4; ++r) sum += v_exp<SEGS>(acc[i][j][r] - top);
             m[j] = top;
             s[j] = sum;
         }
@@ -261,19 +308,13 @@ __global__ __launch_bounds__(256, 2) void vocab_forward_kernel(VocabArgs a) {
     // join: lanes g (labels 4 g ..), then the two waves of the same rows
     __syncthreads();
     float* sh = reinterpret_cast<float*>(vlds);
-    auto join = [](float& m1, float& s1, int& a1, float m2, float s2, int a2) {
-        const float top = fmaxf(m1, m2);
-        s1 = s1 * exp2f(m1 - top) + s2 * exp2f(m2 - top);
-        a1 = m1 > m2 ? a1 : m2 > m1 ? a2 : min(a1, a2);
-        m1 = top;
-    };
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
 #pragma unroll
         for (int o = 16; o <= 32; o <<= 1) {
             const float m2 = __shfl_xor(m[j], o, 64), s2 = __shfl_xor(s[j], o, 64);
             const int a2 = __shfl_xor(arg[j], o, 64);
-            join(m[j], s[j], arg[j], m2, s2, a2);
+            v_join<SEGS>(m[j], s[j], arg[j], m2, s2, a2);
         }
         if (wave >= 2 && g == 0) {
             const int at = (wave & 1) * 64 + 16 * j + c;
@@ -287,7 +328,7 @@ __global__ __launch_bounds__(256, 2) void vocab_forward_kernel(VocabArgs a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int at = wave * 64 + 16 * j + c;
-            join(m[j], s[j], arg[j], sh[at], sh[VT + at], reinterpret_cast<int*>(sh)[2 * VT + at]);
+            v_join<SEGS>(m[j], s[j], arg[j], sh[at], sh[VT + at], reinterpret_cast<int*>(sh)[2 * VT + at]);
             if (i0 + at < a.n) {
                 const long o = (long)blockIdx.y * a.nk + i0 + at;
                 a.part_m[o] = m[j];
@@ -298,65 +339,74 @@ __global__ __launch_bounds__(256, 2) void vocab_forward_kernel(VocabArgs a) {
     }
 }
 
-// what the gradient pass reads of a row: lse in units of log 2 and the scaled upstream gradient (0: the row takes no part)
-__device__ __forceinline__ void v_row_of_gradient(const VocabArgs& a, int i, int label, float lse, float gmax) {
-    const bool none = i >= a.n || label < 0 || label >= a.V || lse == -INFINITY;
-    a.lse2[i] = none ? 0.f : lse * V_LOG2E;
-    a.gs[i] = none ? 0.f : isnan(lse) ? NAN : ldexpf(a.grad_nll[i], v_scale_exp(gmax));
+// what the gradient pass reads of a row: 2^14 p = exp2(s + gc) (log 2 units; gc = 14 - log2 sum exp2 s), or exp2((s - gm) / log 2 + gc)
+// with gm the maximum and gc = 14 - log2 of the sum over it
+template <int SEGS>
+__device__ __forceinline__ void v_row_of_gradient(const VocabArgs& a, int i, int label, float m, float log2_total, float gmax) {
+    const bool none = i >= a.n || label < 0 || label >= a.V || log2_total == -INFINITY || a.bad[min(i, a.n - 1)] != 0;
+    a.part[i] = none ? -1 : label;
+    a.gm[i] = none || SEGS == 1 ? 0.f : m;
+    a.gc[i] = none ? -INFINITY : 14.f - (SEGS == 1 ? m + log2_total : log2_total);
+    const float g = none ? 0.f : isnan(log2_total) ? NAN : a.grad_nll[i];
+    a.g[i] = g;
+    a.gn[i] = ldexpf(g, v_scale_exp(gmax) - 15);
 }
 
-template <bool ARG, bool GRAD>
+// Joins the splits of the forward pass: 16 rows a workgroup, 16 threads a row (a call for one row has hundreds of splits).
+template <int SEGS, bool ARG, bool GRAD>
 __global__ __launch_bounds__(256) void vocab_finish_kernel(VocabArgs a) {
-    __shared__ float sh[4];
+    __shared__ float sh[4], sm[16][17], ss[16][17];
+    __shared__ int sa[16][17];
     float gmax = 0.f;
     if constexpr (GRAD) gmax = v_block_max(a.amax + 2 * V_AMAX, sh);
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i >= a.nk) return;
+    const int row = threadIdx.x & 15, part = threadIdx.x >> 4, i = blockIdx.x * 16 + row;
     float m = V_FLOOR, s = 0.f;
     int arg = 0x7FFFFFFF;
     if (i < a.n)
-        for (int p = 0; p < a.splits; ++p) {
-            const float m2 = a.part_m[(long)p * a.nk + i], s2 = a.part_s[(long)p * a.nk + i], top = fmaxf(m, m2);
-            s = s * exp2f(m - top) + s2 * exp2f(m2 - top);
-            if constexpr (ARG) {
-                const int a2 = a.part_i[(long)p * a.nk + i];
-                arg = m > m2 ? arg : m2 > m ? a2 : min(arg, a2);
-            }
-            m = top;
-        }
+        for (int p = part; p < a.splits; p += 16)
+            v_join<SEGS>(m, s, arg, a.part_m[(long)p * a.nk + i], a.part_s[(long)p * a.nk + i], ARG ? a.part_i[(long)p * a.nk + i] : 0);
+    sm[part][row] = m; ss[part][row] = s; sa[part][row] = arg;
+    __syncthreads();
+    if (part != 0) return;
+#pragma unroll
+    for (int p = 1; p < 16; ++p) v_join<SEGS>(m, s, arg, sm[p][row], ss[p][row], sa[p][row]);
+    const float log2_total = log2f(s), unit = SEGS == 1 ? V_LN2 : 1.f;
     if constexpr (ARG) {
         if (i < a.n) {
-            const float rest = -log2f(s) * V_LN2;  // s = 1 + the others
             const bool fine = s > 0.f && s < INFINITY;
             a.label_out[i] = fine ? arg : -1;
-            a.logprob[i] = s == 0.f ? -INFINITY : fine ? rest : NAN;
+            a.logprob[i] = s == 0.f ? -INFINITY : fine ? -log2_total * V_LN2 : NAN;  // (the sum holds the largest as 1)
         }
     } else {
-        const float lse = s == 0.f ? -INFINITY : (m + log2f(s)) * V_LN2;
         const int label = i < a.n ? a.labels[i] : -1;
         if (i < a.n) {
-            a.lse[i] = lse;
+            const bool bad = GRAD && a.bad[i] != 0;
+            a.lse[i] = bad ? NAN : s == 0.f ? -INFINITY : m * unit + log2_total * V_LN2;
             float nll = 0.f;
             if (label >= a.V) {
                 nll = NAN;
                 atomicOr(a.status, PIN_STATUS_LABEL_RANGE);
             } else if (label >= 0) {
-                nll = s == 0.f ? INFINITY : (m - a.tlogit[i] + log2f(s)) * V_LN2;
+                nll = s == 0.f ? INFINITY : (m - a.tlogit[i]) * unit + log2_total * V_LN2;
             }
             a.nll[i] = nll;
         }
-        if constexpr (GRAD) v_row_of_gradient(a, i, label, lse, gmax);
+        if constexpr (GRAD)
+            v_row_of_gradient<SEGS>(a, i, label, m, log2_total, gmax);
     }
 }
 
+template <int SEGS>
 __global__ __launch_bounds__(256) void vocab_prepare_kernel(VocabArgs a) {  // the gradient pass alone, with the lse of an earlier call
     __shared__ float sh[4];
     const float gmax = v_block_max(a.amax + 2 * V_AMAX, sh);
     const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i >= a.nk) return;
+    if (i >= a.nk + 64) return;
     const int label = i < a.n ? a.labels[i] : -1;
     if (label >= a.V) atomicOr(a.status, PIN_STATUS_LABEL_RANGE);
-    v_row_of_gradient(a, i, label, i < a.n ? a.lse[i] : 0.f, gmax);
+    const float lse = i < a.n ? a.lse[i] : 0.f;
+    const float log2_total = lse == -INFINITY ? -INFINITY : isnan(lse) ? NAN : 0.f;
+    v_row_of_gradient<SEGS>(a, i, label, SEGS == 1 ? lse * V_LOG2E : lse, log2_total, gmax);
 }
 
 // D of one piece of the vocabulary: the logits again, D [n][piece] and D^T [piece][n] in fp16 (two pieces of fp32)
@@ -371,33 +421,38 @@ __global__ __launch_bounds__(256, 2) void vocab_probs_kernel(VocabArgs a, int p0
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = vt_f4{0.f, 0.f, 0.f, 0.f};
     vt_product<BF, SEGS>(v_operand_w(a), v_operand_x(a), v0, i0, 0, a.dk / VT_K, vlds, acc);
-    v_logits<SEGS>(a, acc, v0, i0);
     const int vb = v0 + (wave >> 1) * 64 + 4 * g, ib = i0 + (wave & 1) * 64 + c;
     const long plane = (long)a.nk * a.piece;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int row = ib + 16 * j;
-        if (row >= a.nk) continue;
-        const float lse2 = a.lse2[row], gs = a.gs[row];
-        const int lab = gs == 0.f ? -1 : a.labels[row];
+        const float gm = a.gm[row], gc = a.gc[row], gn = a.gn[row], xs = SEGS == 1 ? 1.f : a.xs[row];
+        const int lab = a.part[row];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            unsigned short h[4], l[4];
+            const vt_f4 b2 = *reinterpret_cast<const vt_f4*>(a.b2 + vb + 16 * i);
+            float d[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                float p = __builtin_amdgcn_exp2f(acc[i][j][r] - lse2);
-                p = (lab == vb + 16 * i + r ? p - 1.f : p) * gs;
-                p = gs == 0.f ? 0.f : p;
-                h[r] = v_half(p);
-                l[r] = SEGS == 1 ? 0 : v_half(p - v_from_half(h[r]));
-                const long at = (long)(vb + 16 * i + r - p0) * a.nk + row;
-                a.pt[at] = h[r];
-                if constexpr (SEGS > 1) a.pt[plane + at] = l[r];
+                float p = v_prob<SEGS>(acc[i][j][r], xs, SEGS == 1 ? 1.f : a.ws_[vb + 16 * i + r], b2[r], gm, gc);
+                d[r] = (lab == vb + 16 * i + r ? p - 0x1p14f : p) * gn;
+            }
+            unsigned h[2], l[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                if constexpr (SEGS > 1) v_split(d[2 * r], d[2 * r + 1], h[r], l[r]);
+                else h[r] = v_pack(d[2 * r], d[2 * r + 1]);
+                const long at = (long)(vb + 16 * i + 2 * r - p0) * a.nk + row;
+                a.pt[at] = (unsigned short)h[r];
+                a.pt[at + a.nk] = (unsigned short)(h[r] >> 16);
+                if constexpr (SEGS > 1) {
+                    a.pt[plane + at] = (unsigned short)l[r];
+                    a.pt[plane + at + a.nk] = (unsigned short)(l[r] >> 16);
+                }
             }
             const long at = (long)row * a.piece + vb + 16 * i - p0;
-            *reinterpret_cast<uint2*>(a.p + at) = make_uint2(h[0] | (unsigned)h[1] << 16, h[2] | (unsigned)h[3] << 16);
-            if constexpr (SEGS > 1)
-                *reinterpret_cast<uint2*>(a.p + plane + at) = make_uint2(l[0] | (unsigned)l[1] << 16, l[2] | (unsigned)l[3] << 16);
+            *reinterpret_cast<uint2*>(a.p + at) = make_uint2(h[0], h[1]);
+            if constexpr (SEGS > 1) *reinterpret_cast<uint2*>(a.p + plane + at) = make_uint2(l[0], l[1]);
         }
     }
 }
@@ -411,7 +466,7 @@ __global__ __launch_bounds__(256, 2) void vocab_dx_kernel(VocabArgs a, int p0, i
     const int steps = width / VT_K, per = (steps + a.dx_splits - 1) / a.dx_splits, s0 = min((int)blockIdx.z * per, steps), s1 = min(s0 + per, steps);
     const VocabOperand P{a.p, a.piece, (long)a.nk * a.piece, a.nk}, WT{a.wt + p0, a.Vk, (long)a.d * a.Vk, a.d};
     vt_f4 acc[4][4];
-    float* out = a.dxp + (long)blockIdx.z * a.nk * a.d;
+    float* out = a.dxp + (long)blockIdx.z * a.nk * a.dk;
     const int ib = i0 + (wave >> 1) * 64 + 4 * g, kb = k0 + (wave & 1) * 64 + c;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -419,7 +474,7 @@ __global__ __launch_bounds__(256, 2) void vocab_dx_kernel(VocabArgs a, int p0, i
         for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                acc[i][j][r] = p0 > 0 && ib + 16 * i + r < a.n && kb + 16 * j < a.d ? out[(long)(ib + 16 * i + r) * a.d + kb + 16 * j] : 0.f;
+                acc[i][j][r] = p0 > 0 && ib + 16 * i + r < a.n && kb + 16 * j < a.d ? out[(long)(ib + 16 * i + r) * a.dk + kb + 16 * j] : 0.f;
     vt_product<false, SEGS>(P, WT, i0, k0, (long)s0 * VT_K, s1 - s0, vlds, acc);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -427,7 +482,7 @@ __global__ __launch_bounds__(256, 2) void vocab_dx_kernel(VocabArgs a, int p0, i
         for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                if (ib + 16 * i + r < a.n && kb + 16 * j < a.d) out[(long)(ib + 16 * i + r) * a.d + kb + 16 * j] = acc[i][j][r];
+                if (ib + 16 * i + r < a.n && kb + 16 * j < a.d) out[(long)(ib + 16 * i + r) * a.dk + kb + 16 * j] = acc[i][j][r];
 }
 
 // dW and db of one piece
@@ -448,7 +503,7 @@ __global__ __launch_bounds__(256, 2) void vocab_dw_kernel(VocabArgs a, int p0) {
     }
     const bool bias = a.db != nullptr && k0 == 0 && (wave & 1) == 0;
     vt_product<false, SEGS, true>(PT, XT, v0, k0, 0, a.nk / VT_K, vlds, acc, ones, bias);
-    const int eg = v_scale_exp(gmax), e = eg + (D == PIN_F16 ? 0 : v_scale_exp(xmax));
+    const int eg = v_scale_exp(gmax) - 1, e = eg + (D == PIN_F16 ? 0 : v_scale_exp(xmax));  // (D: 2^14 times g 2^(e - 15))
     const int vb = p0 + v0 + (wave >> 1) * 64 + 4 * g, kb = k0 + (wave & 1) * 64 + c;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -463,17 +518,290 @@ __global__ __launch_bounds__(256, 2) void vocab_dw_kernel(VocabArgs a, int p0) {
         }
 }
 
+// ---------------------------------------------------------------------------------------------------- streaming kernels
 template <int D>
-__global__ __launch_bounds__(256) void vocab_dx_finish_kernel(VocabArgs a) {
-    __shared__ float sh[4];
-    const float gmax = v_block_max(a.amax + 2 * V_AMAX, sh), wmax = v_block_max(a.amax + V_AMAX, sh);
-    const int e = v_scale_exp(gmax) + (D == PIN_F16 ? 0 : v_scale_exp(wmax));
-    const long all = (long)a.n * a.d;
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long)gridDim.x * 256) {
-        float s = 0.f;
-        for (int p = 0; p < a.dx_splits; ++p) s += a.dxp[(long)p * a.nk * a.d + i];
-        v_put<D>(a.dx, i, ldexpf(s, -e));
+__device__ __forceinline__ int v_down_x(const VocabArgs& a, float* sh) {  // exponent of x^T's scale
+    return D == PIN_F16 ? 0 : v_scale_exp(v_block_max(a.amax, sh));
+}
+template <int D>
+__device__ __forceinline__ int v_down_w(const VocabArgs& a, float* sh) {
+    return D == PIN_F16 ? 0 : v_scale_exp(v_block_max(a.amax + V_AMAX, sh));
+}
+
+template <int D, int KT, int MODE>
+__global__ __launch_bounds__(256, MODE >= VS_DX && KT == 8 && D != PIN_F32 ? 1 : 2) void vocab_stream_kernel(VocabArgs a) {
+    constexpr bool BF = D == PIN_BF16, GRAD = MODE >= VS_DX, OWN_X = MODE != VS_DW;
+    constexpr int PL = D == PIN_F32 ? 2 : 1, SEGS = D == PIN_F32 ? 3 : 1, NJ = vs_nj<PL, KT, MODE>();
+    typedef VsShape<PL, KT, MODE> S;
+    constexpr int TR = S::TR, TROW = S::DK * 2, TTROW = TR * 2, FT = S::DK / 16;
+    extern __shared__ __attribute__((aligned(16))) char vlds[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+    const int o0 = ((int)blockIdx.x * 4 + wave) * 16 * NJ;
+    const VocabOperand X = v_operand_x(a), W = v_operand_w(a);
+    const VocabOperand own = OWN_X ? X : W, str = OWN_X ? W : X;
+    const unsigned short* trans = OWN_X ? a.wt : a.xt;
+    const long trans_ld = OWN_X ? a.Vk : a.nk, trans_plane = (long)a.d * trans_ld;
+
+    // the owners' operand and their numbers
+    vt_u4 o[PL][NJ][KT];
+    float own_b[NJ], own_s[NJ], own_m[NJ];  // b2 or gc; power of two; gm
+    int own_l[NJ];                          // label of the row, or the label that the row of W is
+    float m[NJ], s[NJ];
+    int arg[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        const int row = o0 + 16 * j + c, in = min(row, own.rows - 1);
+#pragma unroll
+        for (int p = 0; p < PL; ++p)
+#pragma unroll
+            for (int k = 0; k < KT; ++k) o[p][j][k] = *reinterpret_cast<const vt_u4*>(own.p + p * own.plane + in * own.ld + k * 32 + g * 8);
+        own_s[j] = PL == 1 ? 1.f : OWN_X ? a.xs[in] : a.ws_[in];
+        own_b[j] = MODE == VS_DX ? a.gc[in] : MODE == VS_DW ? a.b2[in] : 0.f;
+        own_m[j] = PL == 2 && MODE == VS_DX ? a.gm[in] : 0.f;
+        own_l[j] = MODE == VS_DW ? row : MODE == VS_DX ? a.part[in] : MODE == VS_FORWARD && row < a.n ? a.labels[in] : -1;
+        m[j] = V_FLOOR; s[j] = 0.f; arg[j] = 0x7FFFFFFF;
     }
+    vt_f4 acc2[GRAD ? FT : 1][NJ], ones[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        ones[j] = vt_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int f = 0; f < (GRAD ? FT : 1); ++f) acc2[f][j] = vt_f4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    const int tiles = (OWN_X ? a.Vk : a.nk) / TR, per = (tiles + (int)gridDim.y - 1) / (int)gridDim.y;
+    const int t0 = min((int)blockIdx.y * per, tiles), t1 = min(t0 + per, tiles);
+    auto load = [&](int t) {
+        char* at = vlds + (t & 1) * S::BUF;
+        const int r0 = t * TR;
+        // the streamed rows' numbers: 64 floats each, one instruction of one wave
+        const float* src[5] = {a.b2, a.ws_, nullptr, nullptr, nullptr};
+        if constexpr (MODE == VS_DW) {
+            src[0] = a.gc; src[1] = a.gn; src[2] = reinterpret_cast<const float*>(a.part); src[3] = a.gm; src[4] = a.xs;
+        }
+#pragma unroll
+        for (int k = 0; k < S::NC; ++k)
+            if (wave == (k & 3))
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src[k] + r0 + lane),
+                                                 (__attribute__((address_space(3))) void*)(at + S::T_BYTES + S::TT_BYTES + k * 256), 4, 0, 0);
+        vs_load<TR, TROW, PL>(str.p, str.ld, str.plane, r0, str.rows - 1, 0, at);
+        if constexpr (GRAD) vs_load<S::DK, TTROW, PL>(trans, trans_ld, trans_plane, 0, a.d - 1, r0, at + S::T_BYTES);
+    };
+    if (t0 < t1) load(t0);
+    for (int t = t0; t < t1; ++t) {
+        // this step has arrived and the other buffer's reads are done, for every wave
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        if (t + 1 < t1) load(t + 1);
+        const char* T = vlds + (t & 1) * S::BUF;
+        const char* TT = T + S::T_BYTES;
+        const float* K = reinterpret_cast<const float*>(TT + S::TT_BYTES);
+        const int r0 = t * TR;
+        bool hot = false;  // (dW) a streamed row's label is one of the wave's
+        if constexpr (MODE == VS_DW) hot = __any(lane < TR && (unsigned)(reinterpret_cast<const int*>(K)[2 * 64 + lane] - o0) < 16u * NJ);
+#pragma unroll
+        for (int q = 0; q < TR / 32; ++q) {
+            vt_f4 acc[2][NJ];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) acc[i][j] = vt_f4{0.f, 0.f, 0.f, 0.f};
+                if constexpr (PL == 2) {
+#pragma unroll
+                    for (int k = 0; k < KT; ++k) {
+                        const vt_u4 lo = vs_read<TROW>(T + TR * TROW, 32 * q + 16 * i + c, 4 * k + g);
+#pragma unroll
+                        for (int j = 0; j < NJ; ++j) acc[i][j] = vt_mfma<false>(lo, o[0][j][k], acc[i][j]);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < KT; ++k) {
+                    const vt_u4 hi = vs_read<TROW>(T, 32 * q + 16 * i + c, 4 * k + g);
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) {
+                        if constexpr (PL == 2) acc[i][j] = vt_mfma<false>(hi, o[1][j][k], acc[i][j]);
+                        acc[i][j] = vt_mfma<BF>(hi, o[0][j][k], acc[i][j]);
+                    }
+                }
+            }
+            const int rq = r0 + 32 * q;
+            if constexpr (!GRAD) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const vt_f4 b2 = *reinterpret_cast<const vt_f4*>(K + 32 * q + 16 * i + 4 * g);
+                    vt_f4 ws = {1.f, 1.f, 1.f, 1.f};
+                    if constexpr (PL == 2) ws = *reinterpret_cast<const vt_f4*>(K + 64 + 32 * q + 16 * i + 4 * g);
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) acc[i][j][r] = v_logit<SEGS>(acc[i][j][r], own_s[j], ws[r], b2[r]);
+                }
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    float top = m[j];
+                    if constexpr (MODE == VS_ARGMAX) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                if (acc[i][j][r] > top) { top = acc[i][j][r]; arg[j] = rq + 16 * i + 4 * g + r; }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[i][j][r]);
+                        if (__any((unsigned)(own_l[j] - rq) < 32u)) {
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                                for (int r = 0; r < 4; ++r)
+                                    if (own_l[j] == rq + 16 * i + 4 * g + r) a.tlogit[o0 + 16 * j + c] = acc[i][j][r];
+                        }
+                    }
+                    float sum = s[j] * v_exp<SEGS>(m[j] - top);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) sum += v_exp<SEGS>(acc[i][j][r] - top);
+                    m[j] = top;
+                    s[j] = sum;
+                }
+            } else {
+                vt_u4 pb[PL][NJ];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int at = 32 * q + 16 * i + 4 * g;
+                    const vt_f4 k0 = *reinterpret_cast<const vt_f4*>(K + at);
+                    vt_f4 k1 = {1.f, 1.f, 1.f, 1.f}, km = {0.f, 0.f, 0.f, 0.f}, kx = {1.f, 1.f, 1.f, 1.f};
+                    if constexpr (MODE == VS_DW || PL == 2) k1 = *reinterpret_cast<const vt_f4*>(K + 64 + at);  // gn of the rows, or ws of the labels
+                    if constexpr (MODE == VS_DW && PL == 2) {
+                        km = *reinterpret_cast<const vt_f4*>(K + 3 * 64 + at);
+                        kx = *reinterpret_cast<const vt_f4*>(K + 4 * 64 + at);
+                    }
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            acc[i][j][r] = MODE == VS_DX ? v_prob<SEGS>(acc[i][j][r], own_s[j], k1[r], k0[r], own_m[j], own_b[j])
+                                                         : v_prob<SEGS>(acc[i][j][r], kx[r], own_s[j], own_b[j], km[r], k0[r]);
+                    if constexpr (MODE == VS_DX) {
+#pragma unroll
+                        for (int j = 0; j < NJ; ++j)
+                            if (__any((unsigned)(own_l[j] - rq - 16 * i) < 16u)) {
+#pragma unroll
+                                for (int r = 0; r < 4; ++r)
+                                    if (own_l[j] == rq + 16 * i + 4 * g + r) acc[i][j][r] -= 0x1p14f;
+                            }
+                    } else {
+                        if (hot) {
+                            const int* L = reinterpret_cast<const int*>(K) + 2 * 64 + at;
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const int l = L[r];
+#pragma unroll
+                                for (int j = 0; j < NJ; ++j)
+                                    if (l == own_l[j]) acc[i][j][r] -= 0x1p14f;
+                            }
+                        }
+#pragma unroll
+                        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) acc[i][j][r] *= k1[r];
+                    }
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; r += 2) {
+                            unsigned h, l = 0;
+                            if constexpr (PL == 2) v_split(acc[i][j][r], acc[i][j][r + 1], h, l);
+                            else h = v_pack(acc[i][j][r], acc[i][j][r + 1]);
+                            pb[0][j][2 * i + r / 2] = h;
+                            if constexpr (PL == 2) pb[PL - 1][j][2 * i + r / 2] = l;
+                        }
+                }
+#pragma unroll
+                for (int f = 0; f < FT; ++f) {
+                    if constexpr (PL == 2) {
+                        const vt_u4 lo = vs_read<TTROW>(TT + S::DK * TTROW, 16 * f + c, 4 * q + g);
+#pragma unroll
+                        for (int j = 0; j < NJ; ++j) acc2[f][j] = vt_mfma<false>(lo, pb[0][j], acc2[f][j]);
+                    }
+                    const vt_u4 hi = vs_read<TTROW>(TT, 16 * f + c, 4 * q + g);
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) {
+                        if constexpr (PL == 2) acc2[f][j] = vt_mfma<false>(hi, pb[PL - 1][j], acc2[f][j]);
+                        acc2[f][j] = vt_mfma<false>(hi, pb[0][j], acc2[f][j]);
+                    }
+                }
+                if constexpr (MODE == VS_DW) {
+                    const vt_u4 one = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) {
+                        if constexpr (PL == 2) ones[j] = vt_mfma<false>(one, pb[PL - 1][j], ones[j]);
+                        ones[j] = vt_mfma<false>(one, pb[0][j], ones[j]);
+                    }
+                }
+            }
+        }
+    }
+    if constexpr (!GRAD) {  // join the lanes g of a row
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+#pragma unroll
+            for (int d = 16; d <= 32; d <<= 1) {
+                const float m2 = __shfl_xor(m[j], d, 64), s2 = __shfl_xor(s[j], d, 64);
+                const int a2 = __shfl_xor(arg[j], d, 64);
+                v_join<SEGS>(m[j], s[j], arg[j], m2, s2, a2);
+            }
+            const int row = o0 + 16 * j + c;
+            if (g == 0 && row < a.n) {
+                const long at = (long)blockIdx.y * a.nk + row;
+                a.part_m[at] = m[j];
+                a.part_s[at] = s[j];
+                if constexpr (MODE == VS_ARGMAX) a.part_i[at] = arg[j];
+            }
+        }
+    } else {
+        const int rows = OWN_X ? a.n : a.V;
+        float* out = OWN_X ? a.dxp + (long)blockIdx.y * a.nk * a.dk : a.dwp + (long)blockIdx.y * a.Vk * a.dk;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int row = o0 + 16 * j + c;
+            if (row >= rows) continue;
+#pragma unroll
+            for (int f = 0; f < FT; ++f) *reinterpret_cast<vt_f4*>(out + (long)row * a.dk + 16 * f + 4 * g) = acc2[f][j];
+            if (MODE == VS_DW && g == 0) a.dbp[(long)blockIdx.y * a.Vk + row] = ones[j][0];
+        }
+    }
+}
+
+// sums of the partial gradients, scaled back and rounded to the tensors' type.  row_g: dx of the streaming kernel, whose D does not hold g
+template <int D>
+__global__ __launch_bounds__(256) void vocab_join_kernel(VocabArgs a, int x_blocks, int row_g, int with_dw) {
+    __shared__ float sh[4];
+    const int eg = v_scale_exp(v_block_max(a.amax + 2 * V_AMAX, sh)) - 1, ex = v_down_x<D>(a, sh), ew = v_down_w<D>(a, sh);
+    const bool is_x = (int)blockIdx.x < x_blocks;
+    const long first = ((long)blockIdx.x - (is_x ? 0 : x_blocks)) * 256 + threadIdx.x;
+    const long stride = (long)(is_x ? x_blocks : (int)gridDim.x - x_blocks) * 256;
+    const int rows = is_x ? a.n : a.V, splits = is_x ? a.dx_splits : a.dw_splits;
+    const float* part = is_x ? a.dxp : a.dwp;
+    const long plane = (long)(is_x ? a.nk : a.Vk) * a.dk, all = (long)rows * a.d;
+    const int e = is_x ? ew + (row_g ? 14 : eg) : ex + eg;
+    if (is_x || with_dw)
+        for (long i = first; i < all; i += stride) {
+            const long row = i / a.d, at = row * a.dk + (i - row * a.d);
+            float s = 0.f;
+            for (int p = 0; p < splits; ++p) s += part[p * plane + at];
+            s = ldexpf(s, -e);
+            if (is_x && row_g) s *= a.g[row];
+            v_put<D>(is_x ? a.dx : a.dw, i, s);
+        }
+    if (!is_x && with_dw && a.db != nullptr)
+        for (long v = first; v < a.V; v += stride) {
+            float s = 0.f;
+            for (int p = 0; p < a.dw_splits; ++p) s += a.dbp[(long)p * a.Vk + v];
+            v_put<D>(a.db, v, ldexpf(s, -eg));
+        }
 }
 
 template <int D>
@@ -486,20 +814,30 @@ __global__ __launch_bounds__(256) void vocab_no_rows_kernel(VocabArgs a) {  // n
 
 int pin_warm_vocab() {
     hipFuncAttributes at;
-    return hipFuncGetAttributes(&at, reinterpret_cast<const void*>(&vocab_prepare_kernel)) == hipSuccess ? 0 : -1;
+    return hipFuncGetAttributes(&at, reinterpret_cast<const void*>(&vocab_prepare_kernel<1>)) == hipSuccess ? 0 : -1;
 }
 
 // ---------------------------------------------------------------------------------------------------- host
 enum { V_PREDICT = 0, V_NLL = 1, V_GRAD = 2, V_STEP = 3 };
+constexpr int V_STREAM_DIM = 256;  // features of the streaming kernels at most
+constexpr int V_FILL = 1024;       // workgroups a launch is split for
 
 struct VocabPlan {
     VocabArgs a;
-    int dtype, segs;
-    bool copy;
+    int dtype, kt;  // kt: 32s of features of the streaming kernels, 0: the tiles of vocab_tile.h
     long bytes;
 };
 
 static long v_up(long v, long m) { return (v + m - 1) / m * m; }
+static int v_splits(int workgroups, int tiles) {
+    const int s = workgroups >= V_FILL ? 1 : (V_FILL + workgroups - 1) / workgroups;
+    return s < tiles ? s : tiles;
+}
+// owners of a workgroup of the streaming kernels (vs_nj)
+static int vs_owners(int dtype, int kt, bool grad) {
+    const int pl = dtype == PIN_F32 ? 2 : 1;
+    return 64 * (!grad ? (pl * kt <= 8 ? 4 : 2) : kt == 2 ? (pl == 1 ? 4 : 2) : pl * kt <= 8 ? 2 : 1);
+}
 
 static VocabPlan v_plan(const pin_vocab_head* h, int mode, char* base) {
     VocabPlan p;
@@ -509,39 +847,47 @@ static VocabPlan v_plan(const pin_vocab_head* h, int mode, char* base) {
     a.x = h->x; a.w = h->weight; a.bias = h->bias; a.ldx = h->x_stride; a.ldw = h->weight_stride;
     a.dk = (int)v_up(a.d, VT_K); a.nk = (int)v_up(a.n > 0 ? a.n : 1, VT); a.Vk = (int)v_up(a.V, VT);
     p.dtype = h->dtype;
-    p.segs = h->dtype == PIN_F32 ? 3 : 1;
-    const int planes = p.segs == 1 ? 1 : 2;
+    p.kt = a.dk <= V_STREAM_DIM ? a.dk / 32 : 0;
+    a.order = p.kt > 0;
+    const bool two = h->dtype == PIN_F32, grads = mode == V_GRAD || mode == V_STEP;
+    const int planes = two ? 2 : 1;
     // 16-bit rows that begin and end on 16-byte borders are read where they are
-    p.copy = p.segs > 1 || a.d % VT_K != 0 || a.ldx % 8 != 0 || a.ldw % 8 != 0 || ((uintptr_t)a.x | (uintptr_t)a.w) % 16 != 0;
+    const bool copy_w = two || a.d % VT_K != 0 || a.ldw % 8 != 0 || (uintptr_t)a.w % 16 != 0;
+    const bool copy_x = grads || two || a.d % VT_K != 0 || a.ldx % 8 != 0 || (uintptr_t)a.x % 16 != 0;
     const int rows = a.nk / VT, tiles = a.Vk / VT;
-    // forward: enough workgroups to fill the card twice over
-    a.splits = rows >= 1024 ? 1 : (1024 + rows - 1) / rows;
-    if (a.splits > tiles) a.splits = tiles;
-    a.tiles_per_split = (tiles + a.splits - 1) / a.splits;
-    a.splits = (tiles + a.tiles_per_split - 1) / a.tiles_per_split;
-    // gradient: pieces whose D and D^T take about 256 MB together
+    if (p.kt > 0) {
+        const int own = vs_owners(p.dtype, p.kt, false), grad = vs_owners(p.dtype, p.kt, true), tr = planes * p.kt <= 4 ? 64 : 32;
+        a.splits = v_splits((a.nk + own - 1) / own, a.Vk / tr);
+        a.dx_splits = v_splits((a.nk + grad - 1) / grad, a.Vk / tr);
+        a.dw_splits = v_splits((a.Vk + grad - 1) / grad, a.nk / tr);
+    } else {
+        a.splits = v_splits(rows, tiles);
+        a.tiles_per_split = (tiles + a.splits - 1) / a.splits;
+        a.splits = (tiles + a.tiles_per_split - 1) / a.tiles_per_split;
+        const int dx_tiles = rows * (int)((a.d + VT - 1) / VT);
+        a.dx_splits = dx_tiles >= 512 ? 1 : (512 + dx_tiles - 1) / dx_tiles;
+        if (a.dx_splits > 16) a.dx_splits = 16;
+        a.dw_splits = 0;
+    }
+    // pieces whose D and D^T take about 256 MB together
     long piece = (128l << 20) / (2l * planes * a.nk) / VT * VT;
     if (piece < VT) piece = VT;
     if (piece > a.Vk) piece = a.Vk;
     a.piece = (int)piece;
-    const int dx_tiles = rows * (int)((a.d + VT - 1) / VT);
-    a.dx_splits = dx_tiles >= 512 ? 1 : (512 + dx_tiles - 1) / dx_tiles;
-    if (a.dx_splits > 16) a.dx_splits = 16;
     long at = 0;
     auto take = [&](long bytes) {
         char* q = base + at;
         at += v_up(bytes, 256);
         return q;
     };
+    auto rows_of = [&](long count) { return (float*)take((count + 64) * 4); };  // (64 more: the streaming kernels read whole 64s)
     a.amax = (float*)take(3 * V_AMAX * 4);
-    a.b2 = (float*)take((long)a.Vk * 4);
-    if (p.copy) {
-        a.xa = (unsigned short*)take((long)planes * a.n * a.dk * 2);
-        a.wa = (unsigned short*)take((long)planes * a.V * a.dk * 2);
-        if (p.segs > 1) {
-            a.xs = (float*)take((long)a.n * 4);
-            a.ws_ = (float*)take((long)a.V * 4);
-        }
+    a.b2 = rows_of(a.Vk);
+    if (copy_x) a.xa = (unsigned short*)take((long)planes * a.n * a.dk * 2);
+    if (copy_w) a.wa = (unsigned short*)take((long)planes * a.V * a.dk * 2);
+    if (two) {
+        a.xs = rows_of(a.nk);
+        a.ws_ = rows_of(a.Vk);
     }
     if (mode != V_GRAD) {
         a.part_m = (float*)take((long)a.splits * a.nk * 4);
@@ -549,14 +895,20 @@ static VocabPlan v_plan(const pin_vocab_head* h, int mode, char* base) {
         if (mode == V_PREDICT) a.part_i = (int*)take((long)a.splits * a.nk * 4);
         else a.tlogit = (float*)take((long)a.nk * 4);
     }
-    if (mode == V_GRAD || mode == V_STEP) {
+    if (grads) {
         a.xt = (unsigned short*)take((long)planes * a.d * a.nk * 2);
         a.wt = (unsigned short*)take((long)planes * a.d * a.Vk * 2);
-        a.lse2 = (float*)take((long)a.nk * 4);
-        a.gs = (float*)take((long)a.nk * 4);
-        a.p = (unsigned short*)take((long)planes * a.nk * a.piece * 2);
-        a.pt = (unsigned short*)take((long)planes * a.nk * a.piece * 2);
-        a.dxp = (float*)take((long)a.dx_splits * a.nk * a.d * 4);
+        a.gm = rows_of(a.nk); a.gc = rows_of(a.nk); a.gn = rows_of(a.nk); a.g = rows_of(a.nk);
+        a.part = (int*)rows_of(a.nk);
+        a.bad = (int*)rows_of(a.nk);
+        a.dxp = (float*)take((long)a.dx_splits * a.nk * a.dk * 4);
+        if (p.kt > 0) {
+            a.dwp = (float*)take((long)a.dw_splits * a.Vk * a.dk * 4);
+            a.dbp = (float*)take((long)a.dw_splits * a.Vk * 4);
+        } else {
+            a.p = (unsigned short*)take((long)planes * a.nk * a.piece * 2);
+            a.pt = (unsigned short*)take((long)planes * a.nk * a.piece * 2);
+        }
     }
     p.bytes = at;
     return p;
@@ -578,51 +930,73 @@ static int v_reserve(F* kernel, int bytes) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     return e == hipSuccess ? 0 : fail(-2, "label head: cannot reserve %d bytes of LDS: %s", bytes, hipGetErrorString(e));
 }
-#define V_RESERVE(kernel)                                      \
-    do {                                                       \
-        static const int reserved = v_reserve(kernel, VT_LDS); \
-        if (reserved != 0) return reserved;                    \
+#define V_RESERVE(kernel, bytes)                              \
+    do {                                                      \
+        static const int reserved = v_reserve(kernel, bytes); \
+        if (reserved != 0) return reserved;                   \
     } while (0)
 #define V_LAUNCH(kernel, grid, lds, ...) hipLaunchKernelGGL(kernel, grid, dim3(256), lds, s, __VA_ARGS__)
 
-template <int D>
-static void v_stage(const VocabPlan& p, bool transposed, hipStream_t s) {
+template <int D, int KT, int MODE>
+static int v_stream(const VocabPlan& p, hipStream_t s) {
     const VocabArgs& a = p.a;
-    if (p.copy) V_LAUNCH((vocab_rows_kernel<D, true>), dim3(V_AMAX), 0, a, 1);
-    else if constexpr (D != PIN_F32) V_LAUNCH((vocab_rows_kernel<D, false>), dim3(V_AMAX), 0, a, transposed && D == PIN_BF16 ? 1 : 0);
-    if (transposed) V_LAUNCH((vocab_transpose_kernel<D>), dim3(a.nk / 64 + a.Vk / 64, a.dk / 64), 0, a, a.nk / 64);
-}
-
-template <bool BF, int SEGS>
-static int v_forward(const VocabPlan& p, int mode, hipStream_t s) {
-    const VocabArgs& a = p.a;
-    const dim3 grid(a.nk / VT, a.splits);
-    V_RESERVE((&vocab_forward_kernel<BF, SEGS, true>));
-    V_RESERVE((&vocab_forward_kernel<BF, SEGS, false>));
-    if (mode == V_PREDICT) V_LAUNCH((vocab_forward_kernel<BF, SEGS, true>), grid, VT_LDS, a);
-    else V_LAUNCH((vocab_forward_kernel<BF, SEGS, false>), grid, VT_LDS, a);
-    const dim3 fin(cdiv(a.nk, 256));
-    if (mode == V_PREDICT) V_LAUNCH((vocab_finish_kernel<true, false>), fin, 0, a);
-    else if (mode == V_NLL) V_LAUNCH((vocab_finish_kernel<false, false>), fin, 0, a);
-    else V_LAUNCH((vocab_finish_kernel<false, true>), fin, 0, a);
+    constexpr int lds = VsShape<D == PIN_F32 ? 2 : 1, KT, MODE>::LDS;
+    V_RESERVE((&vocab_stream_kernel<D, KT, MODE>), lds);
+    const int own = vs_owners(D, KT, MODE >= VS_DX), splits = MODE == VS_DW ? a.dw_splits : MODE == VS_DX ? a.dx_splits : a.splits;
+    V_LAUNCH((vocab_stream_kernel<D, KT, MODE>), dim3(((MODE == VS_DW ? a.V : a.n) + own - 1) / own, splits), lds, a);
     return 0;
 }
+template <int D, int MODE>
+static int v_stream_kt(const VocabPlan& p, hipStream_t s) {
+    return p.kt == 2 ? v_stream<D, 2, MODE>(p, s) : p.kt == 4 ? v_stream<D, 4, MODE>(p, s) : p.kt == 6 ? v_stream<D, 6, MODE>(p, s) : v_stream<D, 8, MODE>(p, s);
+}
 
-template <int D, bool BF, int SEGS>
-static int v_gradient(const VocabPlan& p, hipStream_t s) {
+template <int D>
+static int v_run_typed(const VocabPlan& p, int mode, hipStream_t s) {
+    constexpr int SEGS = D == PIN_F32 ? 3 : 1;
+    constexpr bool BF = D == PIN_BF16;
     const VocabArgs& a = p.a;
-    const int kt = cdiv(a.d, VT);
-    V_RESERVE((&vocab_probs_kernel<BF, SEGS>));
-    V_RESERVE((&vocab_dx_kernel<SEGS>));
-    V_RESERVE((&vocab_dw_kernel<D, SEGS>));
-    for (int p0 = 0; p0 < a.Vk; p0 += a.piece) {
-        const int width = p0 + a.piece < a.Vk ? a.piece : a.Vk - p0;
-        V_LAUNCH((vocab_probs_kernel<BF, SEGS>), dim3(a.nk / VT, width / VT), VT_LDS, a, p0);
-        V_LAUNCH((vocab_dx_kernel<SEGS>), dim3(a.nk / VT, kt, a.dx_splits), VT_LDS, a, p0, width);
-        V_LAUNCH((vocab_dw_kernel<D, SEGS>), dim3(width / VT, kt), VT_LDS, a, p0);
+    const bool grads = mode == V_GRAD || mode == V_STEP;
+    V_LAUNCH((vocab_rows_kernel<D>), dim3(V_AMAX), 0, a, grads && D == PIN_BF16 ? 1 : 0);
+    if (grads) V_LAUNCH((vocab_transpose_kernel<D>), dim3(a.nk / 64 + a.Vk / 64, a.dk / 64), 0, a, a.nk / 64);
+    PIN_CHECK_LAUNCH();
+    if (mode != V_GRAD) {
+        if (p.kt > 0) {
+            if (int e = mode == V_PREDICT ? v_stream_kt<D, VS_ARGMAX>(p, s) : v_stream_kt<D, VS_FORWARD>(p, s)) return e;
+        } else {
+            V_RESERVE((&vocab_forward_kernel<BF, SEGS, true>), VT_LDS);
+            V_RESERVE((&vocab_forward_kernel<BF, SEGS, false>), VT_LDS);
+            const dim3 grid(a.nk / VT, a.splits);
+            if (mode == V_PREDICT) V_LAUNCH((vocab_forward_kernel<BF, SEGS, true>), grid, VT_LDS, a);
+            else V_LAUNCH((vocab_forward_kernel<BF, SEGS, false>), grid, VT_LDS, a);
+        }
+        if (mode == V_PREDICT) V_LAUNCH((vocab_finish_kernel<SEGS, true, false>), dim3(cdiv(a.n, 16)), 0, a);
+        else if (mode == V_NLL) V_LAUNCH((vocab_finish_kernel<SEGS, false, false>), dim3(cdiv(a.n, 16)), 0, a);
+        else V_LAUNCH((vocab_finish_kernel<SEGS, false, true>), dim3((a.nk + 64) / 16), 0, a);
+    } else {
+        V_LAUNCH((vocab_prepare_kernel<SEGS>), dim3(cdiv(a.nk + 64, 256)), 0, a);
     }
-    const long all = (long)a.n * a.d;
-    V_LAUNCH((vocab_dx_finish_kernel<D>), dim3(all < 1024 * 256 ? cdiv(all, 256) : 1024), 0, a);
+    PIN_CHECK_LAUNCH();
+    if (!grads) return 0;
+    if (p.kt > 0) {
+        if (int e = v_stream_kt<D, VS_DX>(p, s)) return e;
+        if (int e = v_stream_kt<D, VS_DW>(p, s)) return e;
+    } else {
+        const int kt = cdiv(a.d, VT);
+        V_RESERVE((&vocab_probs_kernel<BF, SEGS>), VT_LDS);
+        V_RESERVE((&vocab_dx_kernel<SEGS>), VT_LDS);
+        V_RESERVE((&vocab_dw_kernel<D, SEGS>), VT_LDS);
+        for (int p0 = 0; p0 < a.Vk; p0 += a.piece) {
+            const int width = p0 + a.piece < a.Vk ? a.piece : a.Vk - p0;
+            V_LAUNCH((vocab_probs_kernel<BF, SEGS>), dim3(a.nk / VT, width / VT), VT_LDS, a, p0);
+            V_LAUNCH((vocab_dx_kernel<SEGS>), dim3(a.nk / VT, kt, a.dx_splits), VT_LDS, a, p0, width);
+            V_LAUNCH((vocab_dw_kernel<D, SEGS>), dim3(width / VT, kt), VT_LDS, a, p0);
+        }
+    }
+    const int xb = (int)(((long)a.n * a.d + 1023) / 1024 < 1024 ? ((long)a.n * a.d + 1023) / 1024 : 1024);
+    const int wb = p.kt == 0 ? 0 : (int)(((long)a.V * a.d + 1023) / 1024 < 2048 ? ((long)a.V * a.d + 1023) / 1024 : 2048);
+    V_LAUNCH((vocab_join_kernel<D>), dim3(xb + wb), 0, a, xb, p.kt > 0 ? 1 : 0, p.kt > 0 ? 1 : 0);
+    PIN_CHECK_LAUNCH();
     return 0;
 }
 
@@ -647,24 +1021,7 @@ static int v_run(const pin_vocab_head* h, int mode, const int32_t* labels, const
     PIN_CHECK_ARG(workspace_bytes >= p.bytes, "workspace too small (pin_vocab_workspace_bytes)");
     a.status = status_word();
     if (a.status == nullptr) return fail(-2, "%s: no status word on this device", __func__);
-    if (p.dtype == PIN_F32) v_stage<PIN_F32>(p, grads, s);
-    else if (p.dtype == PIN_BF16) v_stage<PIN_BF16>(p, grads, s);
-    else v_stage<PIN_F16>(p, grads, s);
-    PIN_CHECK_LAUNCH();
-    if (mode != V_GRAD) {
-        const int e = p.dtype == PIN_F32 ? v_forward<false, 3>(p, mode, s) : p.dtype == PIN_BF16 ? v_forward<true, 1>(p, mode, s) : v_forward<false, 1>(p, mode, s);
-        if (e != 0) return e;
-    } else {
-        V_LAUNCH(vocab_prepare_kernel, dim3(cdiv(a.nk, 256)), 0, a);
-    }
-    PIN_CHECK_LAUNCH();
-    if (grads) {
-        const int e = p.dtype == PIN_F32 ? v_gradient<PIN_F32, false, 3>(p, s)
-                      : p.dtype == PIN_BF16 ? v_gradient<PIN_BF16, true, 1>(p, s) : v_gradient<PIN_F16, false, 1>(p, s);
-        if (e != 0) return e;
-        PIN_CHECK_LAUNCH();
-    }
-    return 0;
+    return p.dtype == PIN_F32 ? v_run_typed<PIN_F32>(p, mode, s) : p.dtype == PIN_BF16 ? v_run_typed<PIN_BF16>(p, mode, s) : v_run_typed<PIN_F16>(p, mode, s);
 }
 }  // namespace pin
 

@@ -1,0 +1,91 @@
+// The label head for features of up to 256 dimensions: the rows of one side ("owners") stay in registers, the other side streams through
+// LDS, and nothing of the n x V products leaves the compute unit.
+//
+//   forward    owners x,  streamed W:   s = T O^T, running maximum and sum of a row in the lane
+//   dx         owners x,  streamed W:   s again, D from it, acc += T^T D
+//   dW, db     owners W,  streamed x:   s again, D from it, acc += T^T D
+//
+// A wave owns 16 NJ rows.  s comes out of the matrix cores with the owner in the lane and four consecutive streamed rows in its
+// registers (lane (c, g), tile i: streamed rows 16 i + 4 g ..), which is also how the second product wants D, as its operand over the
+// streamed rows, if those are counted in the order (g, i, r) within each 32: D goes from accumulator to operand without leaving the lane,
+// and T^T is laid out in that order by the staging launch (v_stream_row).
+//
+// What bounds it: at 64 dimensions the exponential and the arithmetic around it (one v_exp_f32 of 16 cycles and 3 to 4 instructions of 4
+// cycles an element and wave, against 2 products of 64), at 256 the matrix cores and, as much, the LDS reads that feed them: each
+// operand read serves the wave's NJ tiles of owners.
+#pragma once
+#include "vocab_tile.h"
+
+namespace pin {
+
+enum { VS_FORWARD = 0, VS_ARGMAX = 1, VS_DX = 2, VS_DW = 3 };
+
+// streamed row at position p of its group of 32 in the transposed operand
+__host__ __device__ constexpr int v_stream_row(int p) { return 4 * ((p >> 3) & 3) + (p & 3) + 16 * ((p >> 2) & 1); }
+
+template <int PL, int KT, int MODE>
+struct VsShape {
+    static constexpr int DK = KT * 32;
+    static constexpr int TR = PL * KT <= 4 ? 64 : 32;               // streamed rows a step
+    static constexpr int T_BYTES = TR * DK * 2 * PL;                 // [plane][row][k]
+    static constexpr int TT_BYTES = MODE >= VS_DX ? T_BYTES : 0;     // [plane][feature][row]
+    static constexpr int NC = MODE == VS_DW ? (PL == 2 ? 5 : 3) : PL; // per-row numbers of the streamed side, 64 floats each
+    static constexpr int BUF = T_BYTES + TT_BYTES + NC * 256;
+    static constexpr int LDS = 2 * BUF;
+};
+// owners a wave holds, in tiles of 16: as many as leave the accumulators and the owners' operands in the 256 registers of two waves a SIMD
+template <int PL, int KT, int MODE>
+constexpr int vs_nj() {
+    return MODE < VS_DX ? (PL * KT <= 8 ? 4 : 2) : KT == 2 ? (PL == 1 ? 4 : 2) : PL * KT <= 8 ? 2 : 1;
+}
+
+// position of chunk c (8 k) of row r: the 16 lanes that read one chunk of 16 rows touch every bank once
+template <int ROW_BYTES>
+__device__ __forceinline__ int vs_place(int r, int c) {
+    if constexpr (ROW_BYTES % 256 == 0) return c ^ (r & 15);
+    else if constexpr (ROW_BYTES % 128 == 0) return c ^ ((r >> 1) & 7);
+    else return c ^ ((r >> 2) & 3);
+}
+
+// `rows` rows of ROW_BYTES of every plane -> LDS, from row `first` on (row `last` again behind it)
+template <int ROWS, int ROW_BYTES, int PL>
+__device__ __forceinline__ void vs_load(const unsigned short* base, long ld, long plane, int first, int last, long k0, char* lds) {
+    constexpr int CH = ROW_BYTES / 16, PER = ROWS * CH / 256;
+    static_assert(ROWS * CH % 256 == 0, "whole instructions of four waves");
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int p = 0; p < PL; ++p)
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int slot = (i * 4 + wave) * 64 + lane, r = slot / CH, c = vs_place<ROW_BYTES>(r, slot % CH);
+            const unsigned short* src = base + p * plane + (long)min(first + r, last) * ld + k0 + c * 8;
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                             (__attribute__((address_space(3))) void*)(lds + p * ROWS * ROW_BYTES + (i * 4 + wave) * 1024), 16, 0, 0);
+        }
+}
+template <int ROW_BYTES>
+__device__ __forceinline__ vt_u4 vs_read(const char* lds, int r, int c) {
+    return *reinterpret_cast<const vt_u4*>(lds + r * ROW_BYTES + (vs_place<ROW_BYTES>(r, c) << 4));
+}
+
+struct VsSide {
+    VocabOperand op;              // [plane][row][k]
+    const unsigned short* trans;  // [plane][feature][row], in the order of v_stream_row
+    long trans_ld, trans_plane;
+};
+
+// two fp32 -> two fp16, the first in the low half
+__device__ __forceinline__ unsigned v_pack(float x, float y) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const h2 h = {(_Float16)x, (_Float16)y};
+    return __builtin_bit_cast(unsigned, h);
+}
+// ... and what is left of them.  The empty asm keeps `h` the bits that are stored: left to itself the compiler rounds x to fp16 once for
+// h and once more for the difference, from a product before and after its own rounding, and where the two differ l is a step off.
+__device__ __forceinline__ void v_split(float x, float y, unsigned& h, unsigned& l) {
+    h = v_pack(x, y);
+    asm volatile("" : "+v"(h));
+    l = v_pack(x - (float)__builtin_bit_cast(_Float16, (unsigned short)h), y - (float)__builtin_bit_cast(_Float16, (unsigned short)(h >> 16)));
+}
+
+}  // namespace pin

@@ -975,7 +975,8 @@ def vocab_nll_grad(x, weight, bias, labels, lse, grad_nll, ws=None):
 
 
 def vocab_nll_step(x, weight, bias, labels, grad_nll, ws=None):
-    """vocab_nll and vocab_nll_grad in one call (the operands are laid out once; the same bits): (nll, lse, dx, dweight, dbias)."""
+    """vocab_nll and vocab_nll_grad in one call (the operands are laid out once, the probabilities formed before lse is rounded):
+    (nll, lse, dx, dweight, dbias)."""
     h = _vocab_head(x, weight, bias)
     lab, g = _vocab_rows("labels", labels, x, torch.int32), _vocab_rows("grad_nll", grad_nll, x, torch.float32)
     nll, lse = (torch.empty((h.n,), dtype=torch.float32, device=x.device) for _ in range(2))

@@ -118,7 +118,8 @@ def _check(x, w, b, labels, g, got):
     rp = 2.0 ** -20 if two else 2.0 ** -11
     # (D below 2^-14 of its scale, which is at most 2^-14 of the largest |g|, in fp16's subnormals; two pieces: their sum)
     sub = g.abs().double().max() * 2.0 ** (-39 if not two else -50)
-    err = d.abs() * (2 * stat[:, None] + rp) + sub * (d != 0)
+    # (the label's entry is g (p - 1): off by 2 delta of p, however near p is to 1)
+    err = torch.exp(s - lse[:, None]).nan_to_num() * g.abs()[:, None] * (2 * stat[:, None]) * (d != 0) + d.abs() * rp + sub * (d != 0)
     eps = torch.finfo(x.dtype).eps / 2
     tiny = {torch.float16: 2.0 ** -25}.get(x.dtype, 2.0 ** -140)
     for name, out, full, mag, lost, terms, top in (
@@ -135,7 +136,7 @@ def _check(x, w, b, labels, g, got):
 
 
 SHAPES = [(1, 1, 1), (1, 33, 16), (3, 5, 7), (2, 1000, 3), (64, 128, 64), (129, 257, 65), (127, 1000, 50), (256, 150, 64), (130, 5000, 200), (1000, 40, 300),
-          (513, 1025, 128), (40, 20011, 96), (300, 3000, 520), (2049, 8191, 72)]
+          (513, 1025, 128), (40, 20011, 96), (300, 3000, 520), (2049, 8191, 72), (260, 777, 180), (900, 1500, 256)]
 
 
 @gpu
@@ -149,8 +150,9 @@ def test_nll_and_gradients(shape, dtype, masked):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
-def test_several_pieces_of_the_vocabulary(dtype):
-    x, w, b, labels, g = _inputs(1500, 70001, 40, dtype, 3, True)
+@pytest.mark.parametrize("dim", [40, 260])
+def test_several_pieces_of_the_vocabulary(dtype, dim):
+    x, w, b, labels, g = _inputs(1500, 70001, dim, dtype, 3, True)
     _check(x, w, b, labels, g, ops.vocab_nll_step(x, w, b, labels, g))
 
 
@@ -174,15 +176,24 @@ def test_no_bias_and_strided_rows(dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
-def test_step_is_the_two_calls_and_repeats_bit_for_bit(dtype):
-    x, w, b, labels, g = _inputs(700, 3001, 130, dtype, 5, True)
+@pytest.mark.parametrize("dim", [130, 400])
+def test_the_two_calls_and_repeats(dtype, dim):
+    """The step's loss is vocab_nll's bit for bit; the gradient of a given lse keeps the same bounds; every call repeats its bits, whatever
+    an earlier one left in the workspace."""
+    x, w, b, labels, g = _inputs(700, 3001, dim, dtype, 5, True)
     nll, lse, *grads = ops.vocab_nll_step(x, w, b, labels, g)
-    ws = ops.vocab_workspace(700, 3001, 130, dtype)
+    ws = ops.vocab_workspace(700, 3001, dim, dtype)
+    first = None
     for _ in range(2):
-        ws.fill_(0xFF)  # (whatever an earlier call left)
+        ws.fill_(0xFF)
         a, l = ops.vocab_nll(x, w, b, labels, ws=ws)
         assert torch.equal(a, nll) and torch.equal(l, lse)
-        for p, q in zip(ops.vocab_nll_grad(x, w, b, labels, l, g, ws=ws), grads):
+        ws.fill_(0xFF)
+        alone = ops.vocab_nll_grad(x, w, b, labels, l, g, ws=ws)
+        _check(x, w, b, labels, g, (a, l, *alone))
+        first = first or alone
+        ws.fill_(0xFF)
+        for p, q in zip((*alone, *ops.vocab_nll_step(x, w, b, labels, g, ws=ws)), (*first, nll, lse, *grads)):
             assert torch.equal(p, q)
 
 
@@ -205,9 +216,10 @@ def test_magnitudes(dtype, scale):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
-def test_rows_without_a_label_take_no_part(dtype):
+@pytest.mark.parametrize("dim", [40, 64, 320])
+def test_rows_without_a_label_take_no_part(dtype, dim):
     """NaN and infinities in rows without a label reach no gradient; without any label all gradients are zero."""
-    x, w, b, labels, g = _inputs(300, 500, 64, dtype, 7)
+    x, w, b, labels, g = _inputs(300, 500, dim, dtype, 7)
     none = torch.zeros(300, dtype=torch.bool, device="cuda")
     none[::3] = True
     labels[none] = -1
@@ -218,14 +230,17 @@ def test_rows_without_a_label_take_no_part(dtype):
     assert (got[0][none] == 0).all() and (got[2][none] == 0).all()
     assert torch.equal(got[0], clean[0]) and torch.equal(got[2], clean[2]) and torch.equal(got[4], clean[4])
     assert torch.equal(got[3], clean[3])
+    plain = ops.vocab_nll(x, w, b, labels)
+    assert torch.equal(plain[0], clean[0]) and torch.equal(plain[1].nan_to_num(posinf=0, neginf=0)[~none], clean[1][~none])
     for t in ops.vocab_nll_step(x, w, b, torch.full_like(labels, -7), g)[2:]:
         assert (t == 0).all()
 
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
-def test_a_labelled_row_that_is_not_finite_is_seen(dtype):
-    x, w, b, labels, g = _inputs(200, 300, 40, dtype, 8)
+@pytest.mark.parametrize("dim", [40, 64, 320])
+def test_a_labelled_row_that_is_not_finite_is_seen(dtype, dim):
+    x, w, b, labels, g = _inputs(200, 300, dim, dtype, 8)
     x[10, 3] = math.nan
     nll, lse, dx, dw, db = ops.vocab_nll_step(x, w, b, labels, g)
     assert nll.isnan().nonzero().flatten().tolist() == [10] and dx[10].isnan().all() and not dx[11].isnan().any()
