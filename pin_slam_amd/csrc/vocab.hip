@@ -18,7 +18,7 @@ namespace pin {
 
 constexpr float V_LOG2E = 1.44269504088896340736f, V_LN2 = 0.69314718055994530942f;
 constexpr float V_FLOOR = -1e30f;  // a maximum below every logit of a label that is not excluded (in units of log 2)
-constexpr int V_AMAX = 512;        // workgroups (and partial maxima) of the first staging launch
+constexpr int V_AMAX = 1024;       // workgroups (and partial maxima) of the first staging launch
 
 struct VocabArgs {
     const void* x;
@@ -48,6 +48,7 @@ struct VocabArgs {
     int* bad;                // 1: no label and not finite (its copy in xa is zero)
     float *dxp, *dwp, *dbp;  // partial sums [splits][nk][dk], [splits][Vk][dk], [splits][Vk]
     int splits, tiles_per_split, dx_splits, dw_splits, piece;
+    int* exps;               // exponents: of the scaled g (below 1), of x^T's and of W^T's power of two
     int order;               // 1: the transposed operands in the order of v_stream_row
     int* status;
 };
@@ -64,8 +65,6 @@ __device__ __forceinline__ void v_put(void* p, long i, float x) {
     else if constexpr (D == PIN_BF16) reinterpret_cast<__bf16*>(p)[i] = (__bf16)x;
     else reinterpret_cast<_Float16*>(p)[i] = (_Float16)x;
 }
-__device__ __forceinline__ unsigned short v_half(float x) { return __builtin_bit_cast(unsigned short, (_Float16)x); }
-__device__ __forceinline__ float v_from_half(unsigned short h) { return (float)__builtin_bit_cast(_Float16, h); }
 // e with |x| 2^e in [2^14, 2^15); 0 where there is nothing to scale or nothing finite
 __device__ __forceinline__ int v_scale_exp(float amax) {
     const unsigned b = __float_as_uint(amax) & 0x7FFFFFFFu;
@@ -80,7 +79,9 @@ __device__ __forceinline__ float wave_max_f32(float v) {
     return v;
 }
 __device__ float v_block_max(const float* part, float* sh) {  // the maximum of V_AMAX partial maxima, in every thread of 256
-    float m = fmaxf(part[threadIdx.x], part[threadIdx.x + 256]);
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < V_AMAX; i += 256) m = fmaxf(m, part[threadIdx.x + i]);
     m = wave_max_f32(m);
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = m;
     __syncthreads();
@@ -91,53 +92,102 @@ __device__ float v_block_max(const float* part, float* sh) {  // the maximum of 
 
 __device__ __forceinline__ bool v_takes_part(const VocabArgs& a, long row) { return a.labels[row] >= 0 && a.labels[row] < a.V; }
 
-// Staging, first launch: one wave a row.  The largest |x| (of the rows that take part), |W|, |g|; the padded bias (-inf: switched off, and
-// behind the last label); the operand of the logit product where it has to be made (COPY_W: two scaled fp16 pieces of fp32, or a
-// padded copy of rows that are not aligned; x is always copied for the gradient: a row without a label that is not finite is zero
-// there, so that no kernel behind has to look for it).
+// eight consecutive elements of a row from k on, zero behind its end; VEC: they begin on a 16-byte border
 template <int D>
-__device__ __forceinline__ float v_stage_row(const VocabArgs& a, bool is_x, long row, bool copy) {
-    const int lane = threadIdx.x & 63;
-    const void* src = is_x ? a.x : a.w;
-    const long at = row * (is_x ? a.ldx : a.ldw);
-    float m = 0.f;
-    bool odd = false;
-    for (int k = lane; k < a.d; k += 64) {
-        const float v = fabsf(v_get<D>(src, at + k));
-        m = fmaxf(m, v);
-        odd |= !(v < INFINITY);
-    }
-    if (!copy) return m;
-    const bool zero = is_x && a.part != nullptr && !v_takes_part(a, row) && __any(odd);
-    if (is_x && a.part != nullptr && lane == 0) a.bad[row] = zero;
-    unsigned short* out = (is_x ? a.xa : a.wa) + row * a.dk;
-    if constexpr (D == PIN_F32) {
-        const long plane = (long)(is_x ? a.n : a.V) * a.dk;
-        const int e = zero ? 0 : v_scale_exp(wave_max_f32(m));
-        for (int k = lane; k < a.dk; k += 64) {
-            const float v = k < a.d && !zero ? ldexpf(v_get<D>(src, at + k), e) : 0.f;
-            const unsigned short h = v_half(v);
-            out[k] = h;
-            out[plane + k] = v_half(v - v_from_half(h));
+__device__ __forceinline__ void v_chunk(const void* row, int k, int d, bool vec, float (&x)[8]) {
+    if (vec && k + 8 <= d) {
+        if constexpr (D == PIN_F32) {
+            const vt_f4 p = *reinterpret_cast<const vt_f4*>(reinterpret_cast<const float*>(row) + k);
+            const vt_f4 q = *reinterpret_cast<const vt_f4*>(reinterpret_cast<const float*>(row) + k + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { x[i] = p[i]; x[4 + i] = q[i]; }
+        } else {
+            const vt_u4 u = *reinterpret_cast<const vt_u4*>(reinterpret_cast<const unsigned short*>(row) + k);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (D == PIN_BF16) {
+                    x[2 * i] = __uint_as_float(u[i] << 16);
+                    x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+                } else {
+                    x[2 * i] = (float)__builtin_bit_cast(_Float16, (unsigned short)u[i]);
+                    x[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (unsigned short)(u[i] >> 16));
+                }
+            }
         }
-        if (lane == 0) (is_x ? a.xs : a.ws_)[row] = ldexpf(1.f, -e);
     } else {
-        for (int k = lane; k < a.dk; k += 64) out[k] = k < a.d && !zero ? reinterpret_cast<const unsigned short*>(src)[at + k] : (unsigned short)0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = k + i < d ? v_get<D>(row, k + i) : 0.f;
     }
-    return m;
 }
 template <int D>
-__global__ __launch_bounds__(256) void vocab_rows_kernel(VocabArgs a, int scan_w) {  // scan_w: W's largest value is wanted
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const bool copy_x = a.xa != nullptr, copy_w = a.wa != nullptr;
+__device__ __forceinline__ const void* v_row(const void* p, long row, long ld) {
+    return reinterpret_cast<const char*>(p) + row * ld * (D == PIN_F32 ? 4 : 2);
+}
+template <int D>
+__device__ __forceinline__ bool v_aligned(const void* p, long ld) {
+    return ((uintptr_t)p | (uintptr_t)(ld * (D == PIN_F32 ? 4 : 2))) % 16 == 0;
+}
+
+// Staging, first launch.  The largest |x| (of the rows that take part), |W|, |g|; the padded bias (-inf: switched off, and behind the
+// last label); the operands of the logit product where they have to be made: two fp16 pieces of fp32 times the row's power of two, or a padded
+// copy of rows that are not aligned.  x is always copied for the gradient: a row without a label that is not finite is zero there, so that
+// no kernel behind has to look for it.  `lanes` lanes take a row, 8 elements each at a time: 16-byte reads and writes, whole waves
+// busy from 64 elements a row on.
+template <int D>
+__global__ __launch_bounds__(256) void vocab_rows_kernel(VocabArgs a, int lanes, int scan_w) {  // scan_w: W's largest value is wanted
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, per = 64 / lanes, mine = lane & (lanes - 1);
+    const bool copy_x = a.xa != nullptr, copy_w = a.wa != nullptr, vx = v_aligned<D>(a.x, a.ldx), vw = v_aligned<D>(a.w, a.ldw);
     float mx = 0.f, mw = 0.f, mg = 0.f;
-    const long rx = copy_x ? a.n : 0, rw = copy_w || scan_w ? a.V : 0;
-    for (long r = (long)blockIdx.x * 4 + wave; r < rx + rw; r += (long)gridDim.x * 4) {
-        if (r < rx) {
-            const float m = v_stage_row<D>(a, true, r, true);
-            if (a.labels == nullptr || v_takes_part(a, r)) mx = fmaxf(mx, m);
-        } else {
-            mw = fmaxf(mw, v_stage_row<D>(a, false, r - rx, copy_w));
+    const long rx = copy_x ? a.n : 0, rw = copy_w || scan_w ? a.V : 0, waves = (long)gridDim.x * 4;
+    for (long base = ((long)blockIdx.x * 4 + wave) * per; base < rx + rw; base += waves * per) {
+        const long r = base + lane / lanes;
+        if (r >= rx + rw) continue;  // (the lanes of a row leave together)
+        const bool is_x = r < rx, copy = is_x || copy_w;
+        const long row = is_x ? r : r - rx;
+        const void* src = v_row<D>(is_x ? a.x : a.w, row, is_x ? a.ldx : a.ldw);
+        const bool vec = is_x ? vx : vw;
+        float x[8], m = 0.f;
+        bool odd = false;
+        for (int k = mine * 8; k < a.dk; k += lanes * 8) {
+            v_chunk<D>(src, k, a.d, vec, x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                m = fmaxf(m, fabsf(x[i]));
+                odd |= !(fabsf(x[i]) < INFINITY);
+            }
+        }
+        const bool part = !is_x || a.labels == nullptr || v_takes_part(a, row);
+        if (is_x) mx = part ? fmaxf(mx, m) : mx;
+        else mw = fmaxf(mw, m);
+        if (!copy) continue;
+        const unsigned long long group = (lanes == 64 ? ~0ull : (1ull << lanes) - 1) << (lane & ~(lanes - 1));
+        const bool zero = is_x && a.part != nullptr && !part && (__ballot(odd) & group) != 0;
+        if (is_x && a.part != nullptr && mine == 0) a.bad[row] = zero;
+        unsigned short* out = (is_x ? a.xa : a.wa) + row * a.dk;
+        int e = 0;
+        if constexpr (D == PIN_F32) {
+            for (int o = lanes >> 1; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+            e = zero ? 0 : v_scale_exp(m);
+            if (mine == 0) (is_x ? a.xs : a.ws_)[row] = ldexpf(1.f, -e);
+        }
+        for (int k = mine * 8; k < a.dk; k += lanes * 8) {
+            if (a.dk > lanes * 8) v_chunk<D>(src, k, a.d, vec, x);  // (else they are still in registers)
+            vt_u4 h, l;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (D == PIN_F32) {
+                    unsigned hh, ll;
+                    v_split(zero ? 0.f : ldexpf(x[2 * i], e), zero ? 0.f : ldexpf(x[2 * i + 1], e), hh, ll);
+                    h[i] = hh;
+                    l[i] = ll;
+                } else if constexpr (D == PIN_BF16) {
+                    h[i] = zero ? 0u : (__float_as_uint(x[2 * i]) >> 16) | (__float_as_uint(x[2 * i + 1]) & 0xFFFF0000u);
+                } else {
+                    h[i] = zero ? 0u : v_pack(x[2 * i], x[2 * i + 1]);
+                }
+            }
+            *reinterpret_cast<vt_u4*>(out + k) = h;
+            if constexpr (D == PIN_F32) *reinterpret_cast<vt_u4*>(out + (long)(is_x ? a.n : a.V) * a.dk + k) = l;
         }
     }
     const long first = (long)blockIdx.x * 256 + threadIdx.x, stride = (long)gridDim.x * 256;
@@ -148,9 +198,9 @@ __global__ __launch_bounds__(256) void vocab_rows_kernel(VocabArgs a, int scan_w
     }
     if (D == PIN_F32)
         for (long i = a.n + first; i < a.nk + 64; i += stride) a.xs[i] = 1.f;
-    if (a.grad_nll != nullptr)
-        for (long i = first; i < a.n; i += stride)
-            if (v_takes_part(a, i)) mg = fmaxf(mg, fabsf(a.grad_nll[i]));
+    if (a.grad_nll == nullptr) return;
+    for (long i = first; i < a.n; i += stride)
+        if (v_takes_part(a, i)) mg = fmaxf(mg, fabsf(a.grad_nll[i]));
     __shared__ float sh[3][4];
     mx = wave_max_f32(mx); mw = wave_max_f32(mw); mg = wave_max_f32(mg);
     if (lane == 0) { sh[0][wave] = mx; sh[1][wave] = mw; sh[2][wave] = mg; }
@@ -162,34 +212,55 @@ __global__ __launch_bounds__(256) void vocab_rows_kernel(VocabArgs a, int scan_w
 }
 
 // Staging, second launch: x^T [d][nk] and W^T [d][Vk] in fp16 (two pieces of fp32), times the tensor's power of two (fp16 as it is).
-// 64 x 64 tiles through LDS; columns behind the last row are zero, and so are rows of x without a label (what they hold must not
-// meet the zeros of D).
+// 64 x 64 tiles through LDS, 16 elements a thread on both sides; columns behind the last row are zero, and so are rows of x without a
+// label (what they hold must not meet the zeros of D).
 template <int D>
 __global__ __launch_bounds__(256) void vocab_transpose_kernel(VocabArgs a, int x_tiles) {
     __shared__ float sh[4];
     __shared__ float tile[64][65];
     const bool is_x = (int)blockIdx.x < x_tiles;
-    const float amax = v_block_max(a.amax + (is_x ? 0 : V_AMAX), sh);
-    const int e = D == PIN_F16 ? 0 : v_scale_exp(amax);
+    const int e = D == PIN_F16 ? 0 : v_scale_exp(v_block_max(a.amax + (is_x ? 0 : V_AMAX), sh));
     const int r0 = ((int)blockIdx.x - (is_x ? 0 : x_tiles)) * 64, k0 = blockIdx.y * 64;
     const int rows = is_x ? a.n : a.V, padded = is_x ? a.nk : a.Vk;
-    const void* src = is_x ? a.x : a.w;
+    const void* base = is_x ? a.x : a.w;
     const long ld = is_x ? a.ldx : a.ldw;
-    for (int i = threadIdx.x; i < 4096; i += 256) {
-        const int r = i >> 6, k = i & 63;
-        tile[r][k] = r0 + r < rows && k0 + k < a.d && (!is_x || v_takes_part(a, r0 + r)) ? v_get<D>(src, (r0 + r) * ld + k0 + k) : 0.f;
+    const bool vec = v_aligned<D>(base, ld);
+    {
+        const int r = threadIdx.x >> 2, k = (threadIdx.x & 3) * 16;
+        const bool in = r0 + r < rows && (!is_x || v_takes_part(a, r0 + r));
+#pragma unroll
+        for (int half = 0; half < 16; half += 8) {
+            float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (in && k0 + k + half < a.d) v_chunk<D>(v_row<D>(base, r0 + r, ld), k0 + k + half, a.d, vec, x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) tile[r][k + half + i] = x[i];
+        }
     }
     __syncthreads();
-    unsigned short* out = is_x ? a.xt : a.wt;
+    const int k = threadIdx.x >> 2;
+    if (k0 + k >= a.d) return;
+    unsigned short* out = (is_x ? a.xt : a.wt) + (long)(k0 + k) * padded + r0;
     const long plane = (long)a.d * padded;
-    for (int i = threadIdx.x; i < 4096; i += 256) {
-        const int k = i >> 6, r = i & 63;
-        if (k0 + k >= a.d) continue;
-        const float v = ldexpf(tile[a.order ? (r & 32) + v_stream_row(r & 31) : r][k], e);
-        const unsigned short h = v_half(v);
-        const long at = (long)(k0 + k) * padded + r0 + r;
-        out[at] = h;
-        if constexpr (D == PIN_F32) out[plane + at] = v_half(v - v_from_half(h));
+#pragma unroll
+    for (int half = 0; half < 16; half += 8) {
+        const int at = (threadIdx.x & 3) * 16 + half;
+        vt_u4 h, l;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float v[2];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int p = at + 2 * i + q;
+                v[q] = ldexpf(tile[a.order ? (p & 32) + v_stream_row(p & 31) : p][k], e);
+            }
+            unsigned hh, ll = 0;
+            if constexpr (D == PIN_F32) v_split(v[0], v[1], hh, ll);
+            else hh = v_pack(v[0], v[1]);
+            h[i] = hh;
+            l[i] = ll;
+        }
+        *reinterpret_cast<vt_u4*>(out + at) = h;
+        if constexpr (D == PIN_F32) *reinterpret_cast<vt_u4*>(out + plane + at) = l;
     }
 }
 
@@ -342,34 +413,56 @@ __global__ __launch_bounds__(256, 2) void vocab_forward_kernel(VocabArgs a) {
 // what the gradient pass reads of a row: 2^14 p = exp2(s + gc) (log 2 units; gc = 14 - log2 sum exp2 s), or exp2((s - gm) / log 2 + gc)
 // with gm the maximum and gc = 14 - log2 of the sum over it
 template <int SEGS>
-__device__ __forceinline__ void v_row_of_gradient(const VocabArgs& a, int i, int label, float m, float log2_total, float gmax) {
+__device__ __forceinline__ void v_row_of_gradient(const VocabArgs& a, int i, int label, float m, float log2_total, int eg) {
     const bool none = i >= a.n || label < 0 || label >= a.V || log2_total == -INFINITY || a.bad[min(i, a.n - 1)] != 0;
     a.part[i] = none ? -1 : label;
     a.gm[i] = none || SEGS == 1 ? 0.f : m;
     a.gc[i] = none ? -INFINITY : 14.f - (SEGS == 1 ? m + log2_total : log2_total);
     const float g = none ? 0.f : isnan(log2_total) ? NAN : a.grad_nll[i];
     a.g[i] = g;
-    a.gn[i] = ldexpf(g, v_scale_exp(gmax) - 15);
+    a.gn[i] = ldexpf(g, eg);
 }
 
-// Joins the splits of the forward pass: 16 rows a workgroup, 16 threads a row (a call for one row has hundreds of splits).
-template <int SEGS, bool ARG, bool GRAD>
+// the exponents of the gradient pass, once for the launches behind (every workgroup of this one needs g's); returns g's
+template <int D>
+__device__ __forceinline__ int v_exponents(const VocabArgs& a, float* sh) {
+    const int eg = v_scale_exp(v_block_max(a.amax + 2 * V_AMAX, sh)) - 15;
+    if (blockIdx.x == 0) {
+        const float mx = v_block_max(a.amax, sh), mw = v_block_max(a.amax + V_AMAX, sh);
+        if (threadIdx.x == 0) {
+            a.exps[0] = eg;
+            a.exps[1] = D == PIN_F16 ? 0 : v_scale_exp(mx);
+            a.exps[2] = D == PIN_F16 ? 0 : v_scale_exp(mw);
+        }
+    }
+    return eg;
+}
+
+// Joins the splits of the forward pass, PER threads a row (a call for one row has a thousand splits).
+template <int D, bool ARG, bool GRAD, int PER>
 __global__ __launch_bounds__(256) void vocab_finish_kernel(VocabArgs a) {
-    __shared__ float sh[4], sm[16][17], ss[16][17];
-    __shared__ int sa[16][17];
-    float gmax = 0.f;
-    if constexpr (GRAD) gmax = v_block_max(a.amax + 2 * V_AMAX, sh);
-    const int row = threadIdx.x & 15, part = threadIdx.x >> 4, i = blockIdx.x * 16 + row;
+    constexpr int ROWS = 256 / PER, SEGS = D == PIN_F32 ? 3 : 1;
+    __shared__ float sh[4], sm[PER][ROWS + 1], ss[PER][ROWS + 1];
+    __shared__ int sa[PER][ROWS + 1];
+    int eg = 0;
+    if constexpr (GRAD) eg = v_exponents<D>(a, sh);
+    const int row = threadIdx.x % ROWS, part = threadIdx.x / ROWS, i = blockIdx.x * ROWS + row;
     float m = V_FLOOR, s = 0.f;
     int arg = 0x7FFFFFFF;
     if (i < a.n)
-        for (int p = part; p < a.splits; p += 16)
+#pragma unroll 4
+        for (int p = part; p < a.splits; p += PER)
             v_join<SEGS>(m, s, arg, a.part_m[(long)p * a.nk + i], a.part_s[(long)p * a.nk + i], ARG ? a.part_i[(long)p * a.nk + i] : 0);
     sm[part][row] = m; ss[part][row] = s; sa[part][row] = arg;
-    __syncthreads();
-    if (part != 0) return;
 #pragma unroll
-    for (int p = 1; p < 16; ++p) v_join<SEGS>(m, s, arg, sm[p][row], ss[p][row], sa[p][row]);
+    for (int o = PER / 2; o > 0; o >>= 1) {
+        __syncthreads();
+        if (part < o) {
+            v_join<SEGS>(m, s, arg, sm[part + o][row], ss[part + o][row], sa[part + o][row]);
+            sm[part][row] = m; ss[part][row] = s; sa[part][row] = arg;
+        }
+    }
+    if (part != 0) return;
     const float log2_total = log2f(s), unit = SEGS == 1 ? V_LN2 : 1.f;
     if constexpr (ARG) {
         if (i < a.n) {
@@ -392,21 +485,22 @@ __global__ __launch_bounds__(256) void vocab_finish_kernel(VocabArgs a) {
             a.nll[i] = nll;
         }
         if constexpr (GRAD)
-            v_row_of_gradient<SEGS>(a, i, label, m, log2_total, gmax);
+            v_row_of_gradient<SEGS>(a, i, label, m, log2_total, eg);
     }
 }
 
-template <int SEGS>
+template <int D>
 __global__ __launch_bounds__(256) void vocab_prepare_kernel(VocabArgs a) {  // the gradient pass alone, with the lse of an earlier call
+    constexpr int SEGS = D == PIN_F32 ? 3 : 1;
     __shared__ float sh[4];
-    const float gmax = v_block_max(a.amax + 2 * V_AMAX, sh);
+    const int eg = v_exponents<D>(a, sh);
     const int i = blockIdx.x * 256 + threadIdx.x;
     if (i >= a.nk + 64) return;
     const int label = i < a.n ? a.labels[i] : -1;
     if (label >= a.V) atomicOr(a.status, PIN_STATUS_LABEL_RANGE);
     const float lse = i < a.n ? a.lse[i] : 0.f;
     const float log2_total = lse == -INFINITY ? -INFINITY : isnan(lse) ? NAN : 0.f;
-    v_row_of_gradient<SEGS>(a, i, label, SEGS == 1 ? lse * V_LOG2E : lse, log2_total, gmax);
+    v_row_of_gradient<SEGS>(a, i, label, SEGS == 1 ? lse * V_LOG2E : lse, log2_total, eg);
 }
 
 // D of one piece of the vocabulary: the logits again, D [n][piece] and D^T [piece][n] in fp16 (two pieces of fp32)
@@ -489,8 +583,6 @@ __global__ __launch_bounds__(256, 2) void vocab_dx_kernel(VocabArgs a, int p0, i
 template <int D, int SEGS>
 __global__ __launch_bounds__(256, 2) void vocab_dw_kernel(VocabArgs a, int p0) {
     extern __shared__ __attribute__((aligned(16))) char vlds[];
-    __shared__ float sh[4];
-    const float gmax = v_block_max(a.amax + 2 * V_AMAX, sh), xmax = v_block_max(a.amax, sh);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
     const int v0 = blockIdx.x * VT, k0 = blockIdx.y * VT;
     const VocabOperand PT{a.pt, a.nk, (long)a.nk * a.piece, a.piece}, XT{a.xt, a.nk, (long)a.d * a.nk, a.d};
@@ -503,7 +595,7 @@ __global__ __launch_bounds__(256, 2) void vocab_dw_kernel(VocabArgs a, int p0) {
     }
     const bool bias = a.db != nullptr && k0 == 0 && (wave & 1) == 0;
     vt_product<false, SEGS, true>(PT, XT, v0, k0, 0, a.nk / VT_K, vlds, acc, ones, bias);
-    const int eg = v_scale_exp(gmax) - 1, e = eg + (D == PIN_F16 ? 0 : v_scale_exp(xmax));  // (D: 2^14 times g 2^(e - 15))
+    const int eg = a.exps[0] + 14, e = eg + a.exps[1];  // (D holds 2^14 p and the scaled g)
     const int vb = p0 + v0 + (wave >> 1) * 64 + 4 * g, kb = k0 + (wave & 1) * 64 + c;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -519,15 +611,6 @@ __global__ __launch_bounds__(256, 2) void vocab_dw_kernel(VocabArgs a, int p0) {
 }
 
 // ---------------------------------------------------------------------------------------------------- streaming kernels
-template <int D>
-__device__ __forceinline__ int v_down_x(const VocabArgs& a, float* sh) {  // exponent of x^T's scale
-    return D == PIN_F16 ? 0 : v_scale_exp(v_block_max(a.amax, sh));
-}
-template <int D>
-__device__ __forceinline__ int v_down_w(const VocabArgs& a, float* sh) {
-    return D == PIN_F16 ? 0 : v_scale_exp(v_block_max(a.amax + V_AMAX, sh));
-}
-
 template <int D, int KT, int MODE>
 __global__ __launch_bounds__(256, MODE >= VS_DX && KT == 8 && D != PIN_F32 ? 1 : 2) void vocab_stream_kernel(VocabArgs a) {
     constexpr bool BF = D == PIN_BF16, GRAD = MODE >= VS_DX, OWN_X = MODE != VS_DW;
@@ -775,33 +858,57 @@ __global__ __launch_bounds__(256, MODE >= VS_DX && KT == 8 && D != PIN_F32 ? 1 :
     }
 }
 
-// sums of the partial gradients, scaled back and rounded to the tensors' type.  row_g: dx of the streaming kernel, whose D does not hold g
-template <int D>
-__global__ __launch_bounds__(256) void vocab_join_kernel(VocabArgs a, int x_blocks, int row_g, int with_dw) {
-    __shared__ float sh[4];
-    const int eg = v_scale_exp(v_block_max(a.amax + 2 * V_AMAX, sh)) - 1, ex = v_down_x<D>(a, sh), ew = v_down_w<D>(a, sh);
-    const bool is_x = (int)blockIdx.x < x_blocks;
-    const long first = ((long)blockIdx.x - (is_x ? 0 : x_blocks)) * 256 + threadIdx.x;
-    const long stride = (long)(is_x ? x_blocks : (int)gridDim.x - x_blocks) * 256;
-    const int rows = is_x ? a.n : a.V, splits = is_x ? a.dx_splits : a.dw_splits;
-    const float* part = is_x ? a.dxp : a.dwp;
-    const long plane = (long)(is_x ? a.nk : a.Vk) * a.dk, all = (long)rows * a.d;
-    const int e = is_x ? ew + (row_g ? 14 : eg) : ex + eg;
-    if (is_x || with_dw)
-        for (long i = first; i < all; i += stride) {
-            const long row = i / a.d, at = row * a.dk + (i - row * a.d);
-            float s = 0.f;
-            for (int p = 0; p < splits; ++p) s += part[p * plane + at];
-            s = ldexpf(s, -e);
-            if (is_x && row_g) s *= a.g[row];
-            v_put<D>(is_x ? a.dx : a.dw, i, s);
+// Sums of the partial gradients, scaled back and rounded to the tensors' type.  A thread adds four neighbours over every GROUPS-th split, and
+// GROUPS threads are joined through LDS: few outputs with many splits still fill the card.  Workgroups: dx, then dW, then db.
+template <int D, int GROUPS>
+__global__ __launch_bounds__(256) void vocab_join_kernel(VocabArgs a, int x_blocks, int w_blocks, int streamed) {
+    constexpr int COLS = 256 / GROUPS;
+    __shared__ vt_f4 sum[GROUPS][COLS];
+    const int eg = a.exps[0] + 14, ex = a.exps[1], ew = a.exps[2];
+    const int b = blockIdx.x, kind = b < x_blocks ? 0 : b < x_blocks + w_blocks ? 1 : 2;
+    const int col = threadIdx.x % COLS, group = threadIdx.x / COLS;
+    const long at = ((long)(b - (kind == 0 ? 0 : kind == 1 ? x_blocks : x_blocks + w_blocks)) * COLS + col) * 4;
+    const long all = kind == 0 ? (long)a.n * a.dk : kind == 1 ? (long)a.V * a.dk : a.V;
+    const long plane = kind == 0 ? (long)a.nk * a.dk : kind == 1 ? (long)a.Vk * a.dk : a.Vk;
+    const float* part = kind == 0 ? a.dxp : kind == 1 ? a.dwp : a.dbp;
+    const int splits = kind == 0 ? a.dx_splits : a.dw_splits;
+    vt_f4 s = {0.f, 0.f, 0.f, 0.f};
+    if (at < all) {
+#pragma unroll 8
+        for (int p = group; p < splits; p += GROUPS) s += *reinterpret_cast<const vt_f4*>(part + p * plane + at);
+    }
+    if constexpr (GROUPS > 1) {
+        sum[group][col] = s;
+        __syncthreads();
+        if (group != 0) return;
+#pragma unroll
+        for (int p = 1; p < GROUPS; ++p) s += sum[p][col];
+    }
+    if (at >= all) return;
+    if (kind == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (at + i < a.V) v_put<D>(a.db, at + i, ldexpf(s[i], -eg));
+        return;
+    }
+    const int row = (int)(at / a.dk), k = (int)(at - (long)row * a.dk), e = kind == 0 ? ew + (streamed ? 14 : eg) : ex + eg;
+    const float g = kind == 0 && streamed ? a.g[row] : 1.f;
+    void* out = kind == 0 ? a.dx : a.dw;
+    const long to = (long)row * a.d + k;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = ldexpf(s[i], -e) * g;
+    if (k + 4 <= a.d && (a.d & 3) == 0 && ((uintptr_t)out & 15) == 0) {
+        if constexpr (D == PIN_F32) *reinterpret_cast<vt_f4*>(reinterpret_cast<float*>(out) + to) = s;
+        else if constexpr (D == PIN_F16) *reinterpret_cast<uint2*>(reinterpret_cast<unsigned short*>(out) + to) = make_uint2(v_pack(s[0], s[1]), v_pack(s[2], s[3]));
+        else {
+            typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+            *reinterpret_cast<b4*>(reinterpret_cast<__bf16*>(out) + to) = b4{(__bf16)s[0], (__bf16)s[1], (__bf16)s[2], (__bf16)s[3]};
         }
-    if (!is_x && with_dw && a.db != nullptr)
-        for (long v = first; v < a.V; v += stride) {
-            float s = 0.f;
-            for (int p = 0; p < a.dw_splits; ++p) s += a.dbp[(long)p * a.Vk + v];
-            v_put<D>(a.db, v, ldexpf(s, -eg));
-        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (k + i < a.d) v_put<D>(out, to + i, s[i]);
+    }
 }
 
 template <int D>
@@ -814,7 +921,7 @@ __global__ __launch_bounds__(256) void vocab_no_rows_kernel(VocabArgs a) {  // n
 
 int pin_warm_vocab() {
     hipFuncAttributes at;
-    return hipFuncGetAttributes(&at, reinterpret_cast<const void*>(&vocab_prepare_kernel<1>)) == hipSuccess ? 0 : -1;
+    return hipFuncGetAttributes(&at, reinterpret_cast<const void*>(&vocab_prepare_kernel<PIN_F32>)) == hipSuccess ? 0 : -1;
 }
 
 // ---------------------------------------------------------------------------------------------------- host
@@ -901,6 +1008,7 @@ static VocabPlan v_plan(const pin_vocab_head* h, int mode, char* base) {
         a.gm = rows_of(a.nk); a.gc = rows_of(a.nk); a.gn = rows_of(a.nk); a.g = rows_of(a.nk);
         a.part = (int*)rows_of(a.nk);
         a.bad = (int*)rows_of(a.nk);
+        a.exps = (int*)take(256);
         a.dxp = (float*)take((long)a.dx_splits * a.nk * a.dk * 4);
         if (p.kt > 0) {
             a.dwp = (float*)take((long)a.dw_splits * a.Vk * a.dk * 4);
@@ -951,13 +1059,32 @@ static int v_stream_kt(const VocabPlan& p, hipStream_t s) {
     return p.kt == 2 ? v_stream<D, 2, MODE>(p, s) : p.kt == 4 ? v_stream<D, 4, MODE>(p, s) : p.kt == 6 ? v_stream<D, 6, MODE>(p, s) : v_stream<D, 8, MODE>(p, s);
 }
 
+template <int D, int PER>
+static void v_finish(const VocabArgs& a, int mode, int rows, hipStream_t s) {
+    const dim3 grid(cdiv(rows, 256 / PER));
+    if (mode == V_PREDICT) V_LAUNCH((vocab_finish_kernel<D, true, false, PER>), grid, 0, a);
+    else if (mode == V_NLL) V_LAUNCH((vocab_finish_kernel<D, false, false, PER>), grid, 0, a);
+    else V_LAUNCH((vocab_finish_kernel<D, false, true, PER>), grid, 0, a);
+}
+
+template <int D, int GROUPS>
+static void v_join_partial(const VocabPlan& p, hipStream_t s) {
+    const VocabArgs& a = p.a;
+    const long cols = 256 / GROUPS * 4;
+    const int xb = (int)(((long)a.n * a.dk + cols - 1) / cols), wb = p.kt == 0 ? 0 : (int)(((long)a.V * a.dk + cols - 1) / cols);
+    const int bb = p.kt == 0 || a.db == nullptr ? 0 : (int)((a.V + cols - 1) / cols);
+    V_LAUNCH((vocab_join_kernel<D, GROUPS>), dim3(xb + wb + bb), 0, a, xb, wb, p.kt > 0 ? 1 : 0);
+}
+
 template <int D>
 static int v_run_typed(const VocabPlan& p, int mode, hipStream_t s) {
     constexpr int SEGS = D == PIN_F32 ? 3 : 1;
     constexpr bool BF = D == PIN_BF16;
     const VocabArgs& a = p.a;
     const bool grads = mode == V_GRAD || mode == V_STEP;
-    V_LAUNCH((vocab_rows_kernel<D>), dim3(V_AMAX), 0, a, grads && D == PIN_BF16 ? 1 : 0);
+    int lanes = 8;
+    while (lanes < 64 && lanes * 8 < a.dk) lanes *= 2;
+    V_LAUNCH((vocab_rows_kernel<D>), dim3(V_AMAX), 0, a, lanes, grads && D == PIN_BF16 ? 1 : 0);
     if (grads) V_LAUNCH((vocab_transpose_kernel<D>), dim3(a.nk / 64 + a.Vk / 64, a.dk / 64), 0, a, a.nk / 64);
     PIN_CHECK_LAUNCH();
     if (mode != V_GRAD) {
@@ -970,11 +1097,11 @@ static int v_run_typed(const VocabPlan& p, int mode, hipStream_t s) {
             if (mode == V_PREDICT) V_LAUNCH((vocab_forward_kernel<BF, SEGS, true>), grid, VT_LDS, a);
             else V_LAUNCH((vocab_forward_kernel<BF, SEGS, false>), grid, VT_LDS, a);
         }
-        if (mode == V_PREDICT) V_LAUNCH((vocab_finish_kernel<SEGS, true, false>), dim3(cdiv(a.n, 16)), 0, a);
-        else if (mode == V_NLL) V_LAUNCH((vocab_finish_kernel<SEGS, false, false>), dim3(cdiv(a.n, 16)), 0, a);
-        else V_LAUNCH((vocab_finish_kernel<SEGS, false, true>), dim3((a.nk + 64) / 16), 0, a);
+        const int rows = mode == V_STEP ? a.nk + 64 : a.n;
+        if (a.splits > 64) v_finish<D, 64>(a, mode, rows, s);
+        else v_finish<D, 16>(a, mode, rows, s);
     } else {
-        V_LAUNCH((vocab_prepare_kernel<SEGS>), dim3(cdiv(a.nk + 64, 256)), 0, a);
+        V_LAUNCH((vocab_prepare_kernel<D>), dim3(cdiv(a.nk + 64, 256)), 0, a);
     }
     PIN_CHECK_LAUNCH();
     if (!grads) return 0;
@@ -993,9 +1120,10 @@ static int v_run_typed(const VocabPlan& p, int mode, hipStream_t s) {
             V_LAUNCH((vocab_dw_kernel<D, SEGS>), dim3(width / VT, kt), VT_LDS, a, p0);
         }
     }
-    const int xb = (int)(((long)a.n * a.d + 1023) / 1024 < 1024 ? ((long)a.n * a.d + 1023) / 1024 : 1024);
-    const int wb = p.kt == 0 ? 0 : (int)(((long)a.V * a.d + 1023) / 1024 < 2048 ? ((long)a.V * a.d + 1023) / 1024 : 2048);
-    V_LAUNCH((vocab_join_kernel<D>), dim3(xb + wb), 0, a, xb, p.kt > 0 ? 1 : 0, p.kt > 0 ? 1 : 0);
+    const int most = a.dx_splits > a.dw_splits ? a.dx_splits : a.dw_splits;
+    if (most > 16) v_join_partial<D, 16>(p, s);
+    else if (most > 2) v_join_partial<D, 4>(p, s);
+    else v_join_partial<D, 1>(p, s);
     PIN_CHECK_LAUNCH();
     return 0;
 }
