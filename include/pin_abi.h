@@ -1114,7 +1114,7 @@ int pin_dp_sync_side_effects(void* comm, float* certainty, const float* certaint
 #define PIN_BF16 1
 #define PIN_F16 2
 #define PIN_ADAMW_BLOCK 256
-#define PIN_ADAMW_CLOCK_DOUBLES 8  /* t, beta1^t, beta2^t, lr, and at PIN_ADAMW_CLOCK_TICKET a 64-bit counter (0 between calls) */
+#define PIN_ADAMW_CLOCK_DOUBLES 8  /* t, beta1^t, beta2^t, lr, at PIN_ADAMW_CLOCK_TICKET a 64-bit counter (0 between calls); the rest: scratch of a call */
 #define PIN_ADAMW_CLOCK_TICKET 4
 typedef struct pin_adamw_tensor {
     void* param;             /* [n] updated in place */

@@ -11,22 +11,22 @@
 // that is small in its block stays bounded.  A moving average moves by (1 - b2) of itself a step, far less than half of a code's
 // spacing: rounded to nearest it would never move.  Codes are therefore rounded up with the probability of the remainder, the
 // dither being a hash of (seed, step, element): a step's result depends on nothing else, and a rerun gives the same bits.
-// v > 0 never rounds to the code 0 (its root would divide m alone).
+// v > 0 never rounds to the code 0 (its root would divide m alone).  The conversion is the hardware's dithered one (v_cvt_sr_fp8_f32 /
+// v_cvt_sr_bf8_f32): floor(x / spacing + dither) in exact arithmetic, subnormal codes included, checked over 2^24 values.
 //
 // Memory-bound: 28 bytes an element with fp32 p, g and moments, 16.06 with 8-bit moments, 10.06 with p and g in 16 bits.  One
 // wave takes 256 elements (4 a lane: 16-byte loads of fp32, and the wave is the block of a scale, whose maximum is a reduction in
 // registers), a workgroup CHUNK of them per round; one launch serves up to 64 tensors, whose addresses travel as
-// kernel arguments -- no table to upload, nothing to keep alive, and the call can be captured.  The step count lives on the device
-// (the clock, written by the last workgroup of the last launch): a captured step counts on when it is replayed.
+// kernel arguments -- no table to upload, nothing to keep alive, and the call can be captured.  The step count lives on the device (the
+// clock): a captured step counts on when it is replayed.
 #include "pin_common.h"
 
 namespace pin {
 
 constexpr int AW_BLOCK = PIN_ADAMW_BLOCK;   // elements that share a scale = elements of a wave
-constexpr int AW_TENSORS = 64;              // tensors per launch: 64 x 40 bytes of arguments
-constexpr int AW_UNROLL = 2;                // 256-element blocks of a wave in flight
-constexpr int AW_CHUNK = 4 * AW_UNROLL * AW_BLOCK;
-constexpr int AW_GRID = 2048;               // eight workgroups a compute unit, each walking its share
+constexpr int AW_TENSORS = 96;              // tensors per launch: 96 x 40 bytes of arguments, of the 4 KB there are
+constexpr int AW_CHUNK = 4 * AW_BLOCK;      // elements of a workgroup at a time (two or four blocks a wave in flight: no faster)
+constexpr int AW_GRID = 1 << 20;
 
 struct AwTensor {
     void* param;
@@ -48,6 +48,20 @@ struct AwArgs {
     unsigned seed;
     int advance, zero_grad;
 };
+// Who counts the step: the workgroups of the only launch, by tickets (one launch less: what a few small tensors cost is launches), or a
+// launch of its own in front, which every later one finds done.  A ticket is an atomic on one address, about 55 ns each whatever the card
+// does beside it (measured: 1024 workgroups more cost 56 us), so tickets serve up to AW_MAX_TICKETS workgroups.
+enum { AW_TICKED = 0, AW_TICKETS = 1 };
+constexpr int AW_MAX_TICKETS = 32;
+constexpr int AW_LR = 5, AW_ROOT = 6;  // of the clock: lr / (1 - beta1^t) and 1 / sqrt(1 - beta2^t) of the step that adamw_tick_kernel counted
+__global__ void adamw_tick_kernel(double* clock, float beta1, float beta2) {
+    const double p1 = clock[1] * (double)beta1, p2 = clock[2] * (double)beta2;
+    clock[0] += 1.0;
+    clock[1] = p1;
+    clock[2] = p2;
+    clock[AW_LR] = (double)(float)clock[3] / (1.0 - p1);
+    clock[AW_ROOT] = 1.0 / sqrt(1.0 - p2);
+}
 static_assert(sizeof(AwArgs) <= 4096, "kernel arguments");
 
 // dtype codes of the ABI: 0 fp32, 1 bf16, 2 fp16
@@ -131,69 +145,89 @@ __device__ __forceinline__ int aw_scale_exponent(unsigned largest) {
 }
 __device__ __forceinline__ float aw_pow2(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
 
-// Code of |x| / 2^scale_exponent in a format of BITS fraction bits whose smallest normal is 2^LOW: n = floor(x / spacing + dither)
-// spacings, and the code is the binade's first code plus n (n = 2^(BITS + 1) carries into the next binade by itself).
-template <int BITS, int LOW>
-__device__ __forceinline__ unsigned aw_encode(float size, float dither, unsigned largest_code) {
-    const int e = max((int)(__float_as_uint(size) >> 23) - 127, LOW);
-    const float n = floorf(size * aw_pow2(BITS - e) + dither);
-    return min((unsigned)((e - LOW) << BITS) + (unsigned)n, largest_code);
+// what a lane holds of a block of 256: its four elements
+template <bool EIGHT>
+struct AwRegs {
+    float p[4], g[4], m[EIGHT ? 1 : 4], v[EIGHT ? 1 : 4], ms, vs;
+    unsigned mc, vc;
+};
+
+template <int PD, int GD, bool EIGHT, bool FULL>
+__device__ __forceinline__ void aw_fetch(const AwArgs& a, const AwTensor& t, long block, AwRegs<EIGHT>& x) {
+    const long i = block * AW_BLOCK + 4 * (threadIdx.x & 63), s = t.offset + i;
+    aw_load<PD, FULL>(t.param, i, t.n, x.p);
+    aw_load<GD, FULL>(t.grad, i, t.n, x.g);
+    if constexpr (EIGHT) {
+        x.mc = reinterpret_cast<const unsigned*>(a.m)[s >> 2];
+        x.vc = reinterpret_cast<const unsigned*>(a.v)[s >> 2];
+        x.ms = a.m_scale[s / AW_BLOCK];
+        x.vs = a.v_scale[s / AW_BLOCK];
+    } else {
+        aw_load<PIN_F32, true>(a.m, s, 0, x.m);  // (the layout is padded to whole blocks: always 16 bytes)
+        aw_load<PIN_F32, true>(a.v, s, 0, x.v);
+    }
 }
 
 template <int PD, int GD, bool EIGHT, bool FULL>
-__device__ __forceinline__ void aw_block(const AwArgs& a, const AwTensor& t, long block, float lr, float lr_over_bc1, float inv_sqrt_bc2,
-                                         unsigned key) {
+__device__ __forceinline__ void aw_block(const AwArgs& a, const AwTensor& t, long block, AwRegs<EIGHT>& x, float lr, float lr_over_bc1,
+                                         float inv_sqrt_bc2, unsigned key) {
     const int lane = threadIdx.x & 63;
     const long i = block * AW_BLOCK + 4 * lane, s = t.offset + i;
-    float p[4], g[4], m[4], v[4];
-    aw_load<PD, FULL>(t.param, i, t.n, p);
-    aw_load<GD, FULL>(t.grad, i, t.n, g);
+    float m[4], v[4];
     if constexpr (EIGHT) {
-        const unsigned mc = reinterpret_cast<const unsigned*>(a.m)[s >> 2], vc = reinterpret_cast<const unsigned*>(a.v)[s >> 2];
-        const float ms = a.m_scale[s / AW_BLOCK], vs = a.v_scale[s / AW_BLOCK];
-        const auto m01 = __builtin_amdgcn_cvt_pk_f32_fp8(mc, false), m23 = __builtin_amdgcn_cvt_pk_f32_fp8(mc, true);
-        const auto v01 = __builtin_amdgcn_cvt_pk_f32_bf8(vc, false), v23 = __builtin_amdgcn_cvt_pk_f32_bf8(vc, true);
-        m[0] = m01[0] * ms; m[1] = m01[1] * ms; m[2] = m23[0] * ms; m[3] = m23[1] * ms;
-        v[0] = v01[0] * vs; v[1] = v01[1] * vs; v[2] = v23[0] * vs; v[3] = v23[1] * vs;
+        const auto m01 = __builtin_amdgcn_cvt_pk_f32_fp8(x.mc, false), m23 = __builtin_amdgcn_cvt_pk_f32_fp8(x.mc, true);
+        const auto v01 = __builtin_amdgcn_cvt_pk_f32_bf8(x.vc, false), v23 = __builtin_amdgcn_cvt_pk_f32_bf8(x.vc, true);
+        m[0] = m01[0] * x.ms; m[1] = m01[1] * x.ms; m[2] = m23[0] * x.ms; m[3] = m23[1] * x.ms;
+        v[0] = v01[0] * x.vs; v[1] = v01[1] * x.vs; v[2] = v23[0] * x.vs; v[3] = v23[1] * x.vs;
     } else {
-        aw_load<PIN_F32, true>(a.m, s, 0, m);  // (the layout is padded to whole blocks: always 16 bytes)
-        aw_load<PIN_F32, true>(a.v, s, 0, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { m[j] = x.m[j]; v[j] = x.v[j]; }
     }
     const float keep = 1.f - lr * t.decay;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        p[j] *= keep;
-        adam_elem(p[j], m[j], v[j], g[j], lr_over_bc1, inv_sqrt_bc2, a.beta1, a.beta2, a.eps);
+        x.p[j] *= keep;
+        if constexpr (EIGHT) {
+            float q = 0.f;  // (adam_elem's moments, which the codes hang on bit for bit; the step with the 1-ulp root and reciprocal)
+            adam_elem(q, m[j], v[j], x.g[j], 0.f, 0.f, a.beta1, a.beta2, 1.f);
+            x.p[j] -= lr_over_bc1 * (m[j] * __builtin_amdgcn_rcpf(fmaf(__builtin_amdgcn_sqrtf(v[j]), inv_sqrt_bc2, a.eps)));
+        } else {
+            adam_elem(x.p[j], m[j], v[j], x.g[j], lr_over_bc1, inv_sqrt_bc2, a.beta1, a.beta2, a.eps);
+        }
     }
-    aw_store<PD, FULL>(t.param, i, t.n, p);
+    aw_store<PD, FULL>(t.param, i, t.n, x.p);
     if (a.zero_grad) {
         const float zero[4] = {0.f, 0.f, 0.f, 0.f};
         aw_store<GD, FULL>(t.grad, i, t.n, zero);
     }
     if constexpr (EIGHT) {
-        unsigned mb[4], mm = 0, vm = 0;
+        unsigned mm = 0, vm = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            mb[j] = __float_as_uint(m[j]) & 0x7FFFFFFFu;
-            mm = max(mm, mb[j]);
+            mm = max(mm, __float_as_uint(m[j]) & 0x7FFFFFFFu);
             vm = max(vm, __float_as_uint(v[j]) & 0x7FFFFFFFu);
         }
         mm = wave_max_u32(mm);
         vm = wave_max_u32(vm);
         const int me = aw_scale_exponent<8>(mm), ve = aw_scale_exponent<15>(vm);
         const float down = aw_pow2(-me), vdown = aw_pow2(-ve);
-        unsigned mc = 0, vc = 0;
+        unsigned h[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const unsigned h = aw_mixed((unsigned)(s + j) ^ key);
-            const unsigned cm = aw_encode<3, -6>(__uint_as_float(mb[j]) * down, (float)(h & 0xFFFFu) * 0x1p-16f, 0x7Eu);
-            unsigned cv = aw_encode<2, -14>(v[j] * vdown, (float)(h >> 16) * 0x1p-16f, 0x7Bu);
-            cv = v[j] > 0.f && cv == 0 ? 1u : cv;
-            mc |= (cm | (m[j] < 0.f ? 0x80u : 0u)) << (8 * j);
-            vc |= cv << (8 * j);
+            h[j] = aw_mixed((unsigned)(s + j) ^ key);
+            m[j] *= down;
+            v[j] = v[j] > 0.f ? fmaxf(v[j] * vdown, 0x1p-16f) : 0.f;
         }
-        reinterpret_cast<unsigned*>(a.m)[s >> 2] = mc;
-        reinterpret_cast<unsigned*>(a.v)[s >> 2] = vc;
+        int mc = __builtin_amdgcn_cvt_sr_fp8_f32(m[0], (int)(h[0] << 16), 0, 0);
+        mc = __builtin_amdgcn_cvt_sr_fp8_f32(m[1], (int)(h[1] << 16), mc, 1);
+        mc = __builtin_amdgcn_cvt_sr_fp8_f32(m[2], (int)(h[2] << 16), mc, 2);
+        mc = __builtin_amdgcn_cvt_sr_fp8_f32(m[3], (int)(h[3] << 16), mc, 3);
+        int vc = __builtin_amdgcn_cvt_sr_bf8_f32(v[0], (int)(h[0] & 0xFFFF0000u), 0, 0);
+        vc = __builtin_amdgcn_cvt_sr_bf8_f32(v[1], (int)(h[1] & 0xFFFF0000u), vc, 1);
+        vc = __builtin_amdgcn_cvt_sr_bf8_f32(v[2], (int)(h[2] & 0xFFFF0000u), vc, 2);
+        vc = __builtin_amdgcn_cvt_sr_bf8_f32(v[3], (int)(h[3] & 0xFFFF0000u), vc, 3);
+        reinterpret_cast<int*>(a.m)[s >> 2] = mc;
+        reinterpret_cast<int*>(a.v)[s >> 2] = vc;
         if (lane == 0) {  // a moment that is not finite makes its block's scale NaN: seen by every later step, not silently coded away
             a.m_scale[s / AW_BLOCK] = mm >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : aw_pow2(me);
             a.v_scale[s / AW_BLOCK] = vm >= 0x7F800000u ? __uint_as_float(0x7FC00000u) : aw_pow2(ve);
@@ -206,15 +240,35 @@ __device__ __forceinline__ void aw_block(const AwArgs& a, const AwTensor& t, lon
 
 template <int PD, int GD, bool EIGHT>
 __global__ __launch_bounds__(256) void adamw_kernel(AwArgs a) {
-    __shared__ double sh[3];
+    __shared__ float sh[2];
     __shared__ unsigned sh_key;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, first = lane < a.n_tensors ? a.t[lane].first_chunk : 0x7FFFFFFF;
+    const int second = lane + 64 < a.n_tensors ? a.t[lane + 64].first_chunk : 0x7FFFFFFF;
+    constexpr int ALIGN_P = PD == PIN_F32 ? 15 : 7, ALIGN_G = GD == PIN_F32 ? 15 : 7;
+    int c = blockIdx.x, j = 0;
+    long base = 0;
+    bool full = false;
+    AwRegs<EIGHT> x;
+    // chunk c: its tensor (a lane holds two tensors' first chunks: no search), and what it holds, if it is whole and on 16-byte borders
+    auto fetch = [&]() {
+        j = __popcll(__ballot(first <= c)) + __popcll(__ballot(second <= c)) - 1;
+        const AwTensor& t = a.t[j];
+        base = (long)(c - t.first_chunk) * (AW_CHUNK / AW_BLOCK);
+        full = ((reinterpret_cast<uintptr_t>(t.param) & ALIGN_P) | (reinterpret_cast<uintptr_t>(t.grad) & ALIGN_G)) == 0 &&
+               (base + AW_CHUNK / AW_BLOCK) * AW_BLOCK <= t.n;
+        if (full) aw_fetch<PD, GD, EIGHT, true>(a, t, base + wave, x);
+    };
+    fetch();  // on the way while the step is worked out
     if (threadIdx.x == 0) {
-        const double t = a.clock[0] + 1.0, p1 = a.clock[1] * (double)a.beta1, p2 = a.clock[2] * (double)a.beta2, lr = a.clock[3];
-        sh[0] = lr;
-        sh[1] = (double)(float)lr / (1.0 - p1);
-        sh[2] = 1.0 / sqrt(1.0 - p2);
-        sh_key = aw_mixed(aw_mixed(a.seed) ^ (unsigned)(unsigned long long)t);
-        if (a.advance) {
+        double t = a.clock[0];
+        if (a.advance == AW_TICKED) {
+            sh[0] = (float)a.clock[AW_LR];
+            sh[1] = (float)a.clock[AW_ROOT];
+        } else {
+            t += 1.0;
+            const double p1 = a.clock[1] * (double)a.beta1, p2 = a.clock[2] * (double)a.beta2;
+            sh[0] = (float)((double)(float)a.clock[3] / (1.0 - p1));
+            sh[1] = (float)(1.0 / sqrt(1.0 - p2));
             // every workgroup takes a ticket once it has read the clock; the one with the last ticket sets it and clears the counter
             unsigned long long* ticket = reinterpret_cast<unsigned long long*>(a.clock + PIN_ADAMW_CLOCK_TICKET);
             __threadfence();
@@ -225,28 +279,24 @@ __global__ __launch_bounds__(256) void adamw_kernel(AwArgs a) {
                 *ticket = 0;
             }
         }
+        sh_key = aw_mixed(aw_mixed(a.seed) ^ (unsigned)(unsigned long long)t);
     }
+    const float lr = (float)a.clock[3];
     __syncthreads();
-    const float lr = (float)sh[0], lr_over_bc1 = (float)sh[1], inv_sqrt_bc2 = (float)sh[2];
+    const float lr_over_bc1 = sh[0], inv_sqrt_bc2 = sh[1];
     const unsigned key = sh_key;
-    const int wave = threadIdx.x >> 6;
-    int j = 0;
-    for (int c = blockIdx.x; c < a.n_chunks; c += gridDim.x) {
-        while (j + 1 < a.n_tensors && c >= a.t[j + 1].first_chunk) ++j;
+    while (true) {
         const AwTensor& t = a.t[j];
-        const long base = (long)(c - t.first_chunk) * (AW_CHUNK / AW_BLOCK);
-        const long blocks = (t.n + AW_BLOCK - 1) / AW_BLOCK;
-        constexpr int ALIGN_P = PD == PIN_F32 ? 15 : 7, ALIGN_G = GD == PIN_F32 ? 15 : 7;
-        const bool aligned = ((reinterpret_cast<uintptr_t>(t.param) & ALIGN_P) | (reinterpret_cast<uintptr_t>(t.grad) & ALIGN_G)) == 0;
-        if (aligned && (base + AW_CHUNK / AW_BLOCK) * AW_BLOCK <= t.n) {
-#pragma unroll
-            for (int u = 0; u < AW_UNROLL; ++u)
-                aw_block<PD, GD, EIGHT, true>(a, t, base + 4 * u + wave, lr, lr_over_bc1, inv_sqrt_bc2, key);
-        } else {  // the tensor's last chunk, or a view that begins between 16-byte borders
-            for (int u = 0; u < AW_UNROLL; ++u)
-                if (base + 4 * u + wave < blocks)
-                    aw_block<PD, GD, EIGHT, false>(a, t, base + 4 * u + wave, lr, lr_over_bc1, inv_sqrt_bc2, key);
+        if (full) {
+            aw_block<PD, GD, EIGHT, true>(a, t, base + wave, x, lr, lr_over_bc1, inv_sqrt_bc2, key);
+        } else if (base + wave < (t.n + AW_BLOCK - 1) / AW_BLOCK) {  // the tensor's last chunk, or a view that begins between 16-byte borders
+            AwRegs<EIGHT> y;
+            aw_fetch<PD, GD, EIGHT, false>(a, t, base + wave, y);
+            aw_block<PD, GD, EIGHT, false>(a, t, base + wave, y, lr, lr_over_bc1, inv_sqrt_bc2, key);
         }
+        c += gridDim.x;
+        if (c >= a.n_chunks) break;
+        fetch();
     }
 }
 
@@ -293,11 +343,25 @@ extern "C" int pin_adamw_step(const pin_adamw_tensor* tensors_host, int32_t n_te
     a.m = st->exp_avg; a.v = st->exp_avg_sq; a.m_scale = st->exp_avg_scale; a.v_scale = st->exp_avg_sq_scale; a.clock = st->clock;
     a.zero_grad = st->zero_grad;
     a.beta1 = beta1; a.beta2 = beta2; a.eps = eps; a.seed = seed;
-    // launches of up to AW_TENSORS tensors of one (parameter, gradient) type pair; the last one of the call sets the clock
-    long left = 0;
-    for (int j = 0; j < n_tensors; ++j) left += tensors_host[j].n > 0;
+    // launches of up to AW_TENSORS tensors of one (parameter, gradient) type pair
+    long count = 0, all_chunks = 0;
+    bool one = true;
+    const pin_adamw_tensor* first = nullptr;
+    for (int j = 0; j < n_tensors; ++j) {
+        const pin_adamw_tensor& t = tensors_host[j];
+        if (t.n == 0) continue;
+        first = first == nullptr ? &t : first;
+        one = one && t.param_dtype == first->param_dtype && t.grad_dtype == first->grad_dtype;
+        ++count;
+        all_chunks += (t.n + AW_CHUNK - 1) / AW_CHUNK;
+    }
     hipStream_t s = as_stream(stream);
-    if (left == 0) return fail(-1, "%s: no element to update", __func__);
+    if (count == 0) return fail(-1, "%s: no element to update", __func__);
+    a.advance = one && count <= AW_TENSORS && all_chunks <= AW_MAX_TICKETS ? AW_TICKETS : AW_TICKED;
+    if (a.advance == AW_TICKED) {
+        hipLaunchKernelGGL(adamw_tick_kernel, dim3(1), dim3(1), 0, s, a.clock, beta1, beta2);
+        PIN_CHECK_LAUNCH();
+    }
     for (int pd = PIN_F32; pd <= PIN_F16; ++pd)
         for (int gd = PIN_F32; gd <= PIN_F16; ++gd) {
             long chunks = 0;
@@ -309,11 +373,9 @@ extern "C" int pin_adamw_step(const pin_adamw_tensor* tensors_host, int32_t n_te
                     PIN_CHECK_ARG(chunks + more < (1l << 31), "too many elements");
                     a.t[a.n_tensors++] = AwTensor{t.param, t.grad, (long)t.n, (long)t.offset, t.weight_decay, (int)chunks};
                     chunks += more;
-                    --left;
                 }
                 if (a.n_tensors == AW_TENSORS || (j == n_tensors && a.n_tensors > 0)) {
                     a.n_chunks = (int)chunks;
-                    a.advance = left == 0;
                     const int grid = chunks < AW_GRID ? (int)chunks : AW_GRID;
                     if (pd == PIN_F32) aw_launch_p<PIN_F32>(gd, eight, grid, s, a);
                     else if (pd == PIN_BF16) aw_launch_p<PIN_BF16>(gd, eight, grid, s, a);

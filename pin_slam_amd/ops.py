@@ -1102,7 +1102,7 @@ class AdamW:
             self._bind(list(grads))
         elif self.grads is None:
             raise RuntimeError("no gradients: pass them to AdamW() or to step()")
-        elif [t.data_ptr() for t in self._bound] != self._addresses:  # (a buffer was replaced behind its tensor, e.g. by .data = ...)
+        elif list(map(torch.Tensor.data_ptr, self._bound)) != self._addresses:  # (a buffer was replaced behind its tensor, e.g. by .data = ...)
             self._bind(self.grads)
         if not self._any:
             return
