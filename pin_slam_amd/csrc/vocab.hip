@@ -410,6 +410,119 @@ __global__ __launch_bounds__(256, 2) void vocab_forward_kernel(VocabArgs a) {
     }
 }
 
+// Forward for a few rows (n <= 16 NT): W is read once, straight into the matrix cores' operand, and that is all there is -- no staging, no
+// LDS tiles.  A wave takes 16 RT labels; lane (c, g) reads 16 bytes of label c's row a step (16-bit types: k = 32 s + 8 g ..; fp32, whose
+// products are the fp32 matrix instruction's: k = 16 s + 4 g ..), four consecutive lanes g a contiguous 64 bytes.  Rows that do not
+// begin and end on 16-byte borders (VEC false) are read element by element.
+template <int N>
+struct VInt { static constexpr int value = N; };
+template <int D, int RT, int NT, bool VEC, bool ARG>
+__global__ __launch_bounds__(256) void vocab_few_kernel(VocabArgs a) {
+    constexpr int SEGS = D == PIN_F32 ? 3 : 1, EL = D == PIN_F32 ? 4 : 8, KS = 4 * EL, U = RT == 1 ? 8 : RT == 2 ? 4 : 2;
+    __shared__ float sm[4][16 * NT], ss[4][16 * NT];
+    __shared__ int sa[4][16 * NT];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+    const int v0 = ((int)blockIdx.x * 4 + wave) * 16 * RT;
+    const char* w[RT];
+    const char* x[NT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) w[i] = reinterpret_cast<const char*>(v_row<D>(a.w, min(v0 + 16 * i + c, a.V - 1), a.ldw));
+#pragma unroll
+    for (int j = 0; j < NT; ++j) x[j] = reinterpret_cast<const char*>(v_row<D>(a.x, min(16 * j + c, a.n - 1), a.ldx));
+    vt_f4 acc[RT][NT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = vt_f4{0.f, 0.f, 0.f, 0.f};
+    auto get = [&](const char* row, int k, bool tail) {  // EL elements from k on as they are, zero behind the end of the row
+        vt_u4 u = {0u, 0u, 0u, 0u};
+        if constexpr (VEC) {  // (d is a multiple of EL)
+            if (!tail || k < a.d) u = *reinterpret_cast<const vt_u4*>(row + k * (D == PIN_F32 ? 4 : 2));
+        } else if constexpr (D == PIN_F32) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) u[e] = !tail || k + e < a.d ? reinterpret_cast<const unsigned*>(row)[k + e] : 0u;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                u[e >> 1] |= (!tail || k + e < a.d ? (unsigned)reinterpret_cast<const unsigned short*>(row)[k + e] : 0u) << (16 * (e & 1));
+        }
+        return u;
+    };
+    auto step = [&](int s, auto count, bool tail) {  // `count` steps from s on: all their reads, then their products
+        constexpr int N = decltype(count)::value;
+        vt_u4 wu[N][RT], xu[N][NT];
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const int k = (s + u) * KS + g * EL;
+#pragma unroll
+            for (int i = 0; i < RT; ++i) wu[u][i] = get(w[i], k, tail);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) xu[u][j] = get(x[j], k, tail);
+        }
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    if constexpr (D == PIN_F32) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(wu[u][i][e]), __uint_as_float(xu[u][j][e]), acc[i][j], 0, 0, 0);
+                    } else {
+                        acc[i][j] = vt_mfma<D == PIN_BF16>(wu[u][i], xu[u][j], acc[i][j]);
+                    }
+                }
+    };
+    const int full = a.d / KS;
+    int s0 = 0;
+    for (; s0 + U <= full; s0 += U) step(s0, VInt<U>{}, false);
+    for (; s0 < full; ++s0) step(s0, VInt<1>{}, false);
+    if (a.d % KS != 0) step(full, VInt<1>{}, true);
+    float m[NT], s[NT];
+    int arg[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        m[j] = V_FLOOR; s[j] = 0.f; arg[j] = 0x7FFFFFFF;
+        const int row = 16 * j + c, label = !ARG && row < a.n ? a.labels[row] : -1;
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int v = v0 + 16 * i + 4 * g + r;
+                float b = v >= a.V ? -INFINITY : a.bias == nullptr ? 0.f : v_get<D>(a.bias, v);
+                b = b <= V_FLOOR ? -INFINITY : SEGS == 1 ? b * V_LOG2E : b;
+                const float z = v_logit<SEGS>(acc[i][j][r], 1.f, 1.f, b);
+                acc[i][j][r] = z;
+                if (z > m[j]) { m[j] = z; arg[j] = v; }
+                if (!ARG && v == label) a.tlogit[row] = z;
+            }
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[j] += v_exp<SEGS>(acc[i][j][r] - m[j]);
+#pragma unroll
+        for (int o = 16; o <= 32; o <<= 1) {
+            const float m2 = __shfl_xor(m[j], o, 64), s2 = __shfl_xor(s[j], o, 64);
+            const int a2 = __shfl_xor(arg[j], o, 64);
+            v_join<SEGS>(m[j], s[j], arg[j], m2, s2, a2);
+        }
+        if (g == 0) { sm[wave][row] = m[j]; ss[wave][row] = s[j]; sa[wave][row] = arg[j]; }
+    }
+    __syncthreads();
+    const int row = threadIdx.x;
+    if (row < 16 * NT && row < a.n) {
+        float m1 = sm[0][row], s1 = ss[0][row];
+        int a1 = sa[0][row];
+#pragma unroll
+        for (int q = 1; q < 4; ++q) v_join<SEGS>(m1, s1, a1, sm[q][row], ss[q][row], sa[q][row]);
+        const long at = (long)blockIdx.x * a.nk + row;
+        a.part_m[at] = m1;
+        a.part_s[at] = s1;
+        if constexpr (ARG) a.part_i[at] = a1;
+    }
+}
+
 // what the gradient pass reads of a row: 2^14 p = exp2(s + gc) (log 2 units; gc = 14 - log2 sum exp2 s), or exp2((s - gm) / log 2 + gc)
 // with gm the maximum and gc = 14 - log2 of the sum over it
 template <int SEGS>
@@ -927,11 +1040,14 @@ int pin_warm_vocab() {
 // ---------------------------------------------------------------------------------------------------- host
 enum { V_PREDICT = 0, V_NLL = 1, V_GRAD = 2, V_STEP = 3 };
 constexpr int V_STREAM_DIM = 256;  // features of the streaming kernels at most
+// Rows that vocab_few_kernel takes at most: its matrix instructions keep up with the reads of W to 64 rows (fp32: 32)
+static int v_few_rows(int dtype) { return dtype == PIN_F32 ? 32 : 64; }
 constexpr int V_FILL = 1024;       // workgroups a launch is split for
 
 struct VocabPlan {
     VocabArgs a;
     int dtype, kt;  // kt: 32s of features of the streaming kernels, 0: the tiles of vocab_tile.h
+    int few;        // 16s of labels a wave of vocab_few_kernel, 0: another forward kernel
     long bytes;
 };
 
@@ -957,10 +1073,12 @@ static VocabPlan v_plan(const pin_vocab_head* h, int mode, char* base) {
     p.kt = a.dk <= V_STREAM_DIM ? a.dk / 32 : 0;
     a.order = p.kt > 0;
     const bool two = h->dtype == PIN_F32, grads = mode == V_GRAD || mode == V_STEP;
+    // (a wave per 16 labels until there are eight waves a compute unit, then up to 64: the rows of x are read once for them)
+    p.few = grads || a.n > v_few_rows(h->dtype) ? 0 : a.V >= 131072 ? 4 : a.V >= 65536 ? 2 : 1;
     const int planes = two ? 2 : 1;
     // 16-bit rows that begin and end on 16-byte borders are read where they are
-    const bool copy_w = two || a.d % VT_K != 0 || a.ldw % 8 != 0 || (uintptr_t)a.w % 16 != 0;
-    const bool copy_x = grads || two || a.d % VT_K != 0 || a.ldx % 8 != 0 || (uintptr_t)a.x % 16 != 0;
+    const bool copy_w = !p.few && (two || a.d % VT_K != 0 || a.ldw % 8 != 0 || (uintptr_t)a.w % 16 != 0);
+    const bool copy_x = !p.few && (grads || two || a.d % VT_K != 0 || a.ldx % 8 != 0 || (uintptr_t)a.x % 16 != 0);
     const int rows = a.nk / VT, tiles = a.Vk / VT;
     if (p.kt > 0) {
         const int own = vs_owners(p.dtype, p.kt, false), grad = vs_owners(p.dtype, p.kt, true), tr = planes * p.kt <= 4 ? 64 : 32;
@@ -976,6 +1094,7 @@ static VocabPlan v_plan(const pin_vocab_head* h, int mode, char* base) {
         if (a.dx_splits > 16) a.dx_splits = 16;
         a.dw_splits = 0;
     }
+    if (p.few) a.splits = (a.V + 64 * p.few - 1) / (64 * p.few);
     // pieces whose D and D^T take about 256 MB together
     long piece = (128l << 20) / (2l * planes * a.nk) / VT * VT;
     if (piece < VT) piece = VT;
@@ -992,7 +1111,7 @@ static VocabPlan v_plan(const pin_vocab_head* h, int mode, char* base) {
     a.b2 = rows_of(a.Vk);
     if (copy_x) a.xa = (unsigned short*)take((long)planes * a.n * a.dk * 2);
     if (copy_w) a.wa = (unsigned short*)take((long)planes * a.V * a.dk * 2);
-    if (two) {
+    if (two && !p.few) {
         a.xs = rows_of(a.nk);
         a.ws_ = rows_of(a.Vk);
     }
@@ -1067,6 +1186,25 @@ static void v_finish(const VocabArgs& a, int mode, int rows, hipStream_t s) {
     else V_LAUNCH((vocab_finish_kernel<D, false, true, PER>), grid, 0, a);
 }
 
+template <int D, int RT, int NT, bool VEC>
+static void v_few_go(const VocabArgs& a, int mode, hipStream_t s) {
+    if (mode == V_PREDICT) V_LAUNCH((vocab_few_kernel<D, RT, NT, VEC, true>), dim3(a.splits), 0, a);
+    else V_LAUNCH((vocab_few_kernel<D, RT, NT, VEC, false>), dim3(a.splits), 0, a);
+}
+template <int D, int RT, int NT>
+static void v_few_rt(const VocabArgs& a, int mode, hipStream_t s) {
+    const int size = D == PIN_F32 ? 4 : 2;
+    if (((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)(a.ldx * size) | (uintptr_t)(a.ldw * size) | (uintptr_t)((long)a.d * size)) % 16 == 0) v_few_go<D, RT, NT, true>(a, mode, s);
+    else v_few_go<D, RT, NT, false>(a, mode, s);
+}
+template <int D>
+static void v_few(const VocabPlan& p, int mode, hipStream_t s) {
+    const VocabArgs& a = p.a;
+    if (a.n <= 16) p.few == 4 ? v_few_rt<D, 4, 1>(a, mode, s) : p.few == 2 ? v_few_rt<D, 2, 1>(a, mode, s) : v_few_rt<D, 1, 1>(a, mode, s);
+    else if (a.n <= 32) p.few == 4 ? v_few_rt<D, 4, 2>(a, mode, s) : p.few == 2 ? v_few_rt<D, 2, 2>(a, mode, s) : v_few_rt<D, 1, 2>(a, mode, s);
+    else if constexpr (D != PIN_F32) p.few == 4 ? v_few_rt<D, 4, 4>(a, mode, s) : p.few == 2 ? v_few_rt<D, 2, 4>(a, mode, s) : v_few_rt<D, 1, 4>(a, mode, s);
+}
+
 template <int D, int GROUPS>
 static void v_join_partial(const VocabPlan& p, hipStream_t s) {
     const VocabArgs& a = p.a;
@@ -1082,6 +1220,13 @@ static int v_run_typed(const VocabPlan& p, int mode, hipStream_t s) {
     constexpr bool BF = D == PIN_BF16;
     const VocabArgs& a = p.a;
     const bool grads = mode == V_GRAD || mode == V_STEP;
+    if (p.few) {
+        v_few<D>(p, mode, s);
+        if (a.splits > 64) v_finish<D, 64>(a, mode, a.n, s);
+        else v_finish<D, 16>(a, mode, a.n, s);
+        PIN_CHECK_LAUNCH();
+        return 0;
+    }
     int lanes = 8;
     while (lanes < 64 && lanes * 8 < a.dk) lanes *= 2;
     V_LAUNCH((vocab_rows_kernel<D>), dim3(V_AMAX), 0, a, lanes, grads && D == PIN_BF16 ? 1 : 0);

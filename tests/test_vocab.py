@@ -298,7 +298,7 @@ def test_no_rows(dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("shape", [(1, 1, 1), (1, 131, 64), (1, 70001, 512), (2, 33, 5), (5, 20011, 300), (16, 4096, 256), (17, 4097, 260), (64, 3001, 768), (33, 515, 1030),
+@pytest.mark.parametrize("shape", [(1, 1, 1), (1, 131, 64), (1, 70001, 512), (2, 33, 5), (5, 20011, 300), (16, 4096, 256), (17, 4097, 260), (64, 3001, 768), (33, 515, 1030), (20, 131072, 40), (3, 65600, 24), (65, 700, 515),
                                    (300, 1203, 64), (5000, 150, 50)])
 @pytest.mark.parametrize("masked", [False, True])
 def test_predict(shape, dtype, masked):
@@ -322,6 +322,17 @@ def test_predict(shape, dtype, masked):
     assert torch.equal(label[sure].long(), at[sure])
     if shape[1] > 40:
         assert label[0] == 3
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1, 131, 64), (7, 20001, 300), (16, 70001, 33), (31, 131073, 72), (33, 66000, 130), (64, 1000, 515), (65, 1000, 515)])
+def test_nll_of_a_few_rows(shape, dtype):
+    x, w, b, labels, g = _inputs(*shape, dtype, 40 + sum(shape), True)
+    _check(x, w, b, labels, g, ops.vocab_nll(x, w, b, labels))
+    wide = torch.full((shape[1], shape[2] + 1), math.nan, dtype=dtype, device="cuda")
+    wide[:, 1:] = w
+    _check(x, w, None, labels, g, ops.vocab_nll(x, wide[:, 1:], None, labels))
 
 
 @gpu
