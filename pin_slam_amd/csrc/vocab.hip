@@ -40,8 +40,8 @@ struct VocabArgs {
     unsigned short *xa, *wa, *xt, *wt, *p, *pt;
     float *xs, *ws_, *b2;
     float *amax;             // [3][V_AMAX] partial maxima of |x|, |W|, |g|
-    float *part_m, *part_s;  // [splits][nk]
-    int* part_i;
+    float2* part_ms;         // (maximum, sum) of a row and split [n][splits]
+    int* part_i;             // label of the maximum
     float* tlogit;
     float *gm, *gc, *gn, *g; // of a row: reference of the exponent, its offset, the upstream gradient scaled below 1 and as it is
     int* part;               // its label, -1 where it takes no part in the gradient
@@ -401,9 +401,8 @@ __global__ __launch_bounds__(256, 2) void vocab_forward_kernel(VocabArgs a) {
             const int at = wave * 64 + 16 * j + c;
             v_join<SEGS>(m[j], s[j], arg[j], sh[at], sh[VT + at], reinterpret_cast<int*>(sh)[2 * VT + at]);
             if (i0 + at < a.n) {
-                const long o = (long)blockIdx.y * a.nk + i0 + at;
-                a.part_m[o] = m[j];
-                a.part_s[o] = s[j];
+                const long o = (long)(i0 + at) * a.splits + blockIdx.y;
+                a.part_ms[o] = make_float2(m[j], s[j]);
                 if constexpr (ARG) a.part_i[o] = arg[j];
             }
         }
@@ -516,9 +515,8 @@ __global__ __launch_bounds__(256) void vocab_few_kernel(VocabArgs a) {
         int a1 = sa[0][row];
 #pragma unroll
         for (int q = 1; q < 4; ++q) v_join<SEGS>(m1, s1, a1, sm[q][row], ss[q][row], sa[q][row]);
-        const long at = (long)blockIdx.x * a.nk + row;
-        a.part_m[at] = m1;
-        a.part_s[at] = s1;
+        const long at = (long)row * a.splits + blockIdx.x;
+        a.part_ms[at] = make_float2(m1, s1);
         if constexpr (ARG) a.part_i[at] = a1;
     }
 }
@@ -551,31 +549,29 @@ __device__ __forceinline__ int v_exponents(const VocabArgs& a, float* sh) {
     return eg;
 }
 
-// Joins the splits of the forward pass, PER threads a row (a call for one row has a thousand splits).
+// Joins the splits of the forward pass, PER lanes a row (a call for one row has hundreds of splits).
 template <int D, bool ARG, bool GRAD, int PER>
 __global__ __launch_bounds__(256) void vocab_finish_kernel(VocabArgs a) {
-    constexpr int ROWS = 256 / PER, SEGS = D == PIN_F32 ? 3 : 1;
-    __shared__ float sh[4], sm[PER][ROWS + 1], ss[PER][ROWS + 1];
-    __shared__ int sa[PER][ROWS + 1];
+    constexpr int SEGS = D == PIN_F32 ? 3 : 1;
+    __shared__ float sh[4];
     int eg = 0;
     if constexpr (GRAD) eg = v_exponents<D>(a, sh);
-    const int row = threadIdx.x % ROWS, part = threadIdx.x / ROWS, i = blockIdx.x * ROWS + row;
+    const int part = threadIdx.x % PER, i = blockIdx.x * (256 / PER) + threadIdx.x / PER;
     float m = V_FLOOR, s = 0.f;
     int arg = 0x7FFFFFFF;
     if (i < a.n)
 #pragma unroll 4
-        for (int p = part; p < a.splits; p += PER)
-            v_join<SEGS>(m, s, arg, a.part_m[(long)p * a.nk + i], a.part_s[(long)p * a.nk + i], ARG ? a.part_i[(long)p * a.nk + i] : 0);
-    sm[part][row] = m; ss[part][row] = s; sa[part][row] = arg;
+        for (int p = part; p < a.splits; p += PER) {
+            const float2 ms = a.part_ms[(long)i * a.splits + p];
+            v_join<SEGS>(m, s, arg, ms.x, ms.y, ARG ? a.part_i[(long)i * a.splits + p] : 0);
+        }
 #pragma unroll
     for (int o = PER / 2; o > 0; o >>= 1) {
-        __syncthreads();
-        if (part < o) {
-            v_join<SEGS>(m, s, arg, sm[part + o][row], ss[part + o][row], sa[part + o][row]);
-            sm[part][row] = m; ss[part][row] = s; sa[part][row] = arg;
-        }
+        const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64);
+        const int a2 = ARG ? __shfl_xor(arg, o, 64) : 0;
+        v_join<SEGS>(m, s, arg, m2, s2, a2);
     }
-    if (part != 0) return;
+    if (part != 0 || i >= (GRAD ? a.nk + 64 : a.n)) return;
     const float log2_total = log2f(s), unit = SEGS == 1 ? V_LN2 : 1.f;
     if constexpr (ARG) {
         if (i < a.n) {
@@ -951,9 +947,8 @@ __global__ __launch_bounds__(256, MODE >= VS_DX && KT == 8 && D != PIN_F32 ? 1 :
             }
             const int row = o0 + 16 * j + c;
             if (g == 0 && row < a.n) {
-                const long at = (long)blockIdx.y * a.nk + row;
-                a.part_m[at] = m[j];
-                a.part_s[at] = s[j];
+                const long at = (long)row * a.splits + blockIdx.y;
+                a.part_ms[at] = make_float2(m[j], s[j]);
                 if constexpr (MODE == VS_ARGMAX) a.part_i[at] = arg[j];
             }
         }
@@ -1116,9 +1111,8 @@ static VocabPlan v_plan(const pin_vocab_head* h, int mode, char* base) {
         a.ws_ = rows_of(a.Vk);
     }
     if (mode != V_GRAD) {
-        a.part_m = (float*)take((long)a.splits * a.nk * 4);
-        a.part_s = (float*)take((long)a.splits * a.nk * 4);
-        if (mode == V_PREDICT) a.part_i = (int*)take((long)a.splits * a.nk * 4);
+        a.part_ms = (float2*)take((long)a.splits * a.n * 8);
+        if (mode == V_PREDICT) a.part_i = (int*)take((long)a.splits * a.n * 4);
         else a.tlogit = (float*)take((long)a.nk * 4);
     }
     if (grads) {
@@ -1179,11 +1173,17 @@ static int v_stream_kt(const VocabPlan& p, hipStream_t s) {
 }
 
 template <int D, int PER>
-static void v_finish(const VocabArgs& a, int mode, int rows, hipStream_t s) {
+static void v_finish_per(const VocabArgs& a, int mode, int rows, hipStream_t s) {
     const dim3 grid(cdiv(rows, 256 / PER));
     if (mode == V_PREDICT) V_LAUNCH((vocab_finish_kernel<D, true, false, PER>), grid, 0, a);
     else if (mode == V_NLL) V_LAUNCH((vocab_finish_kernel<D, false, false, PER>), grid, 0, a);
     else V_LAUNCH((vocab_finish_kernel<D, false, true, PER>), grid, 0, a);
+}
+template <int D>
+static void v_finish(const VocabArgs& a, int mode, int rows, hipStream_t s) {
+    if (a.splits > 16) v_finish_per<D, 64>(a, mode, rows, s);
+    else if (a.splits > 1) v_finish_per<D, 8>(a, mode, rows, s);
+    else v_finish_per<D, 1>(a, mode, rows, s);
 }
 
 template <int D, int RT, int NT, bool VEC>
@@ -1222,8 +1222,7 @@ static int v_run_typed(const VocabPlan& p, int mode, hipStream_t s) {
     const bool grads = mode == V_GRAD || mode == V_STEP;
     if (p.few) {
         v_few<D>(p, mode, s);
-        if (a.splits > 64) v_finish<D, 64>(a, mode, a.n, s);
-        else v_finish<D, 16>(a, mode, a.n, s);
+        v_finish<D>(a, mode, a.n, s);
         PIN_CHECK_LAUNCH();
         return 0;
     }
@@ -1242,9 +1241,7 @@ static int v_run_typed(const VocabPlan& p, int mode, hipStream_t s) {
             if (mode == V_PREDICT) V_LAUNCH((vocab_forward_kernel<BF, SEGS, true>), grid, VT_LDS, a);
             else V_LAUNCH((vocab_forward_kernel<BF, SEGS, false>), grid, VT_LDS, a);
         }
-        const int rows = mode == V_STEP ? a.nk + 64 : a.n;
-        if (a.splits > 64) v_finish<D, 64>(a, mode, rows, s);
-        else v_finish<D, 16>(a, mode, rows, s);
+        v_finish<D>(a, mode, mode == V_STEP ? a.nk + 64 : a.n, s);
     } else {
         V_LAUNCH((vocab_prepare_kernel<D>), dim3(cdiv(a.nk + 64, 256)), 0, a);
     }
