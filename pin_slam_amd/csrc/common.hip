@@ -34,7 +34,7 @@ int* status_word() {
 namespace pin {
 int pin_warm_knn(); int pin_warm_pool(); int pin_warm_prep(); int pin_warm_comm(); int pin_warm_train(); int pin_warm_maint();
 int pin_warm_dp(); int pin_warm_sdf(); int pin_warm_brick(); int pin_warm_adamw();
-int pin_warm_vocab();
+int pin_warm_vocab_f32(); int pin_warm_vocab_bf16(); int pin_warm_vocab_f16();
 }  // namespace pin
 
 extern "C" int pin_warmup(void) {
@@ -42,7 +42,8 @@ extern "C" int pin_warmup(void) {
     // inside a SLAM loop that is a frame of 100 ms the first time a stage runs.  One attribute query per translation unit
     // loads them all up front.
     int (*const warm[])() = {pin::pin_warm_knn, pin::pin_warm_pool, pin::pin_warm_prep, pin::pin_warm_comm, pin::pin_warm_train,
-                             pin::pin_warm_maint, pin::pin_warm_dp, pin::pin_warm_sdf, pin::pin_warm_brick, pin::pin_warm_adamw, pin::pin_warm_vocab};
+                             pin::pin_warm_maint, pin::pin_warm_dp, pin::pin_warm_sdf, pin::pin_warm_brick, pin::pin_warm_adamw, pin::pin_warm_vocab_f32,
+                             pin::pin_warm_vocab_bf16, pin::pin_warm_vocab_f16};
     for (auto f : warm)
         if (f() != 0) return pin::fail(-2, "pin_warmup: a code object could not be loaded: %s", hipGetErrorString(hipGetLastError()));
     return 0;

@@ -1,0 +1,1290 @@
+// The label head over a large label set: x [n][d] rows, W [V][d] weights, b [V] biases.
+//   s_iv = x_i . W_v + b_v        lse_i = log sum_v exp s_iv        nll_i = lse_i - s_i,label(i)
+//   D_iv = g_i (exp(s_iv - lse_i) - [v = label(i)])     dx = D W     dW = D^T x     db = sum_i D
+// (what Decoder.sem_label_prob, model/decoder.py:100-103, and the NLL term of Mapper.mapping, utils/mapper.py:782-800, do for a few labels:
+// csrc/sem.h), without ever holding the n x V logits: the forward pass keeps a running maximum and sum a row, the gradient pass forms the
+// logits again in pieces of the vocabulary.
+//
+// Numerics.  bf16 / fp16 inputs multiply as they are, fp32 as two fp16 pieces of the value times a power of two per row
+// (vocab_tile.h); sums, maxima and statistics are fp32.  16-bit inputs keep their logits in units of log 2 (one fused multiply-add, and
+// exp2 is the instruction); fp32 keeps them as they are, where they are rounded half as coarsely.  p is formed from the
+// maximum and the sum (exp(s - m) / total), not from the rounded lse.  D is kept in fp16 times 2^14 / 2^ceil(log2 max |g|): 11 bits
+// down to 2^-28 of the largest (rounded to bf16 it would cost as much error as the output's own rounding does), and the transposed
+// x and W beside it in fp16 times a power of two of the tensor, which holds bf16 exactly down to 2^-31 of its largest value;
+// fp32 again as two pieces each.
+#pragma once
+#include "vocab_stream.h"
+
+namespace pin {
+
+constexpr float V_LOG2E = 1.44269504088896340736f, V_LN2 = 0.69314718055994530942f;
+constexpr float V_FLOOR = -1e30f;  // a maximum below every logit of a label that is not excluded (in units of log 2)
+constexpr int V_AMAX = 1024;       // workgroups (and partial maxima) of the first staging launch
+
+struct VocabArgs {
+    const void* x;
+    const void* w;
+    const void* bias;
+    long ldx, ldw;
+    int n, V, d;
+    int dk, nk, Vk;          // d padded to 64, n and V to 128
+    const int* labels;
+    const float* grad_nll;
+    float* nll;
+    float* lse;
+    int* label_out;
+    float* logprob;
+    void* dx;
+    void* dw;
+    void* db;
+    // workspace
+    unsigned short *xa, *wa, *xt, *wt, *p, *pt;
+    float *xs, *ws_, *b2;
+    float *amax;             // [3][V_AMAX] partial maxima of |x|, |W|, |g|
+    float2* part_ms;         // (maximum, sum) of a row and split [n][splits]
+    int* part_i;             // label of the maximum
+    float* tlogit;
+    float *gm, *gc, *gn, *g; // of a row: reference of the exponent, its offset, the upstream gradient scaled below 1 and as it is
+    int* part;               // its label, -1 where it takes no part in the gradient
+    int* bad;                // 1: no label and not finite (its copy in xa is zero)
+    float *dxp, *dwp, *dbp;  // partial sums [splits][nk][dk], [splits][Vk][dk], [splits][Vk]
+    int splits, tiles_per_split, dx_splits, dw_splits, piece;
+    int* exps;               // exponents: of the scaled g (below 1), of x^T's and of W^T's power of two
+    int order;               // 1: the transposed operands in the order of v_stream_row
+    int* status;
+};
+
+template <int D>
+__device__ __forceinline__ float v_get(const void* p, long i) {
+    if constexpr (D == PIN_F32) return reinterpret_cast<const float*>(p)[i];
+    else if constexpr (D == PIN_BF16) return __uint_as_float((unsigned)reinterpret_cast<const unsigned short*>(p)[i] << 16);
+    else return (float)reinterpret_cast<const _Float16*>(p)[i];
+}
+template <int D>
+__device__ __forceinline__ void v_put(void* p, long i, float x) {
+    if constexpr (D == PIN_F32) reinterpret_cast<float*>(p)[i] = x;
+    else if constexpr (D == PIN_BF16) reinterpret_cast<__bf16*>(p)[i] = (__bf16)x;
+    else reinterpret_cast<_Float16*>(p)[i] = (_Float16)x;
+}
+// e with |x| 2^e in [2^14, 2^15); 0 where there is nothing to scale or nothing finite
+__device__ __forceinline__ int v_scale_exp(float amax) {
+    const unsigned b = __float_as_uint(amax) & 0x7FFFFFFFu;
+    if (b == 0 || b >= 0x7F800000u) return 0;
+    int e;
+    frexpf(amax, &e);
+    return 15 - e;
+}
+__device__ __forceinline__ float wave_max_f32(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
+__device__ float v_block_max(const float* part, float* sh) {  // the maximum of V_AMAX partial maxima, in every thread of 256
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < V_AMAX; i += 256) m = fmaxf(m, part[threadIdx.x + i]);
+    m = wave_max_f32(m);
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
+    __syncthreads();
+    return m;
+}
+
+__device__ __forceinline__ bool v_takes_part(const VocabArgs& a, long row) { return a.labels[row] >= 0 && a.labels[row] < a.V; }
+
+// eight consecutive elements of a row from k on, zero behind its end; VEC: they begin on a 16-byte border
+template <int D>
+__device__ __forceinline__ void v_chunk(const void* row, int k, int d, bool vec, float (&x)[8]) {
+    if (vec && k + 8 <= d) {
+        if constexpr (D == PIN_F32) {
+            const vt_f4 p = *reinterpret_cast<const vt_f4*>(reinterpret_cast<const float*>(row) + k);
+            const vt_f4 q = *reinterpret_cast<const vt_f4*>(reinterpret_cast<const float*>(row) + k + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { x[i] = p[i]; x[4 + i] = q[i]; }
+        } else {
+            const vt_u4 u = *reinterpret_cast<const vt_u4*>(reinterpret_cast<const unsigned short*>(row) + k);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (D == PIN_BF16) {
+                    x[2 * i] = __uint_as_float(u[i] << 16);
+                    x[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+                } else {
+                    x[2 * i] = (float)__builtin_bit_cast(_Float16, (unsigned short)u[i]);
+                    x[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (unsigned short)(u[i] >> 16));
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = k + i < d ? v_get<D>(row, k + i) : 0.f;
+    }
+}
+template <int D>
+__device__ __forceinline__ const void* v_row(const void* p, long row, long ld) {
+    return reinterpret_cast<const char*>(p) + row * ld * (D == PIN_F32 ? 4 : 2);
+}
+template <int D>
+__device__ __forceinline__ bool v_aligned(const void* p, long ld) {
+    return ((uintptr_t)p | (uintptr_t)(ld * (D == PIN_F32 ? 4 : 2))) % 16 == 0;
+}
+
+// Staging, first launch.  The largest |x| (of the rows that take part), |W|, |g|; the padded bias (-inf: switched off, and behind the
+// last label); the operands of the logit product where they have to be made: two fp16 pieces of fp32 times the row's power of two, or a padded
+// copy of rows that are not aligned.  x is always copied for the gradient: a row without a label that is not finite is zero there, so that
+// no kernel behind has to look for it.  `lanes` lanes take a row, 8 elements each at a time: 16-byte reads and writes, whole waves
+// busy from 64 elements a row on.
+template <int D>
+__global__ __launch_bounds__(256) void vocab_rows_kernel(VocabArgs a, int lanes, int scan_w) {  // scan_w: W's largest value is wanted
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, per = 64 / lanes, mine = lane & (lanes - 1);
+    const bool copy_x = a.xa != nullptr, copy_w = a.wa != nullptr, vx = v_aligned<D>(a.x, a.ldx), vw = v_aligned<D>(a.w, a.ldw);
+    float mx = 0.f, mw = 0.f, mg = 0.f;
+    const long rx = copy_x ? a.n : 0, rw = copy_w || scan_w ? a.V : 0, waves = (long)gridDim.x * 4;
+    for (long base = ((long)blockIdx.x * 4 + wave) * per; base < rx + rw; base += waves * per) {
+        const long r = base + lane / lanes;
+        if (r >= rx + rw) continue;  // (the lanes of a row leave together)
+        const bool is_x = r < rx, copy = is_x || copy_w;
+        const long row = is_x ? r : r - rx;
+        const void* src = v_row<D>(is_x ? a.x : a.w, row, is_x ? a.ldx : a.ldw);
+        const bool vec = is_x ? vx : vw;
+        float x[8], m = 0.f;
+        bool odd = false;
+        for (int k = mine * 8; k < a.dk; k += lanes * 8) {
+            v_chunk<D>(src, k, a.d, vec, x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                m = fmaxf(m, fabsf(x[i]));
+                odd |= !(fabsf(x[i]) < INFINITY);
+            }
+        }
+        const bool part = !is_x || a.labels == nullptr || v_takes_part(a, row);
+        if (is_x) mx = part ? fmaxf(mx, m) : mx;
+        else mw = fmaxf(mw, m);
+        if (!copy) continue;
+        const unsigned long long group = (lanes == 64 ? ~0ull : (1ull << lanes) - 1) << (lane & ~(lanes - 1));
+        const bool zero = is_x && a.part != nullptr && !part && (__ballot(odd) & group) != 0;
+        if (is_x && a.part != nullptr && mine == 0) a.bad[row] = zero;
+        unsigned short* out = (is_x ? a.xa : a.wa) + row * a.dk;
+        int e = 0;
+        if constexpr (D == PIN_F32) {
+            for (int o = lanes >> 1; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+            e = zero ? 0 : v_scale_exp(m);
+            if (mine == 0) (is_x ? a.xs : a.ws_)[row] = ldexpf(1.f, -e);
+        }
+        for (int k = mine * 8; k < a.dk; k += lanes * 8) {
+            if (a.dk > lanes * 8) v_chunk<D>(src, k, a.d, vec, x);  // (else they are still in registers)
+            vt_u4 h, l;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (D == PIN_F32) {
+                    unsigned hh, ll;
+                    v_split(zero ? 0.f : ldexpf(x[2 * i], e), zero ? 0.f : ldexpf(x[2 * i + 1], e), hh, ll);
+                    h[i] = hh;
+                    l[i] = ll;
+                } else if constexpr (D == PIN_BF16) {
+                    h[i] = zero ? 0u : (__float_as_uint(x[2 * i]) >> 16) | (__float_as_uint(x[2 * i + 1]) & 0xFFFF0000u);
+                } else {
+                    h[i] = zero ? 0u : v_pack(x[2 * i], x[2 * i + 1]);
+                }
+            }
+            *reinterpret_cast<vt_u4*>(out + k) = h;
+            if constexpr (D == PIN_F32) *reinterpret_cast<vt_u4*>(out + (long)(is_x ? a.n : a.V) * a.dk + k) = l;
+        }
+    }
+    const long first = (long)blockIdx.x * 256 + threadIdx.x, stride = (long)gridDim.x * 256;
+    for (long i = first; i < a.Vk + 64; i += stride) {
+        const float b = i >= a.V ? -INFINITY : a.bias == nullptr ? 0.f : v_get<D>(a.bias, i);
+        a.b2[i] = b <= V_FLOOR ? -INFINITY : D == PIN_F32 ? b : b * V_LOG2E;
+        if (D == PIN_F32 && i >= a.V) a.ws_[i] = 1.f;
+    }
+    if (D == PIN_F32)
+        for (long i = a.n + first; i < a.nk + 64; i += stride) a.xs[i] = 1.f;
+    if (a.grad_nll == nullptr) return;
+    for (long i = first; i < a.n; i += stride)
+        if (v_takes_part(a, i)) mg = fmaxf(mg, fabsf(a.grad_nll[i]));
+    __shared__ float sh[3][4];
+    mx = wave_max_f32(mx); mw = wave_max_f32(mw); mg = wave_max_f32(mg);
+    if (lane == 0) { sh[0][wave] = mx; sh[1][wave] = mw; sh[2][wave] = mg; }
+    __syncthreads();
+    if (threadIdx.x < 3) {
+        const float* s = sh[threadIdx.x];
+        a.amax[threadIdx.x * V_AMAX + blockIdx.x] = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+    }
+}
+
+// Staging, second launch: x^T [d][nk] and W^T [d][Vk] in fp16 (two pieces of fp32), times the tensor's power of two (fp16 as it is).
+// 64 x 64 tiles through LDS, 16 elements a thread on both sides; columns behind the last row are zero, and so are rows of x without a
+// label (what they hold must not meet the zeros of D).
+template <int D>
+__global__ __launch_bounds__(256) void vocab_transpose_kernel(VocabArgs a, int x_tiles) {
+    __shared__ float sh[4];
+    __shared__ float tile[64][65];
+    const bool is_x = (int)blockIdx.x < x_tiles;
+    const int e = D == PIN_F16 ? 0 : v_scale_exp(v_block_max(a.amax + (is_x ? 0 : V_AMAX), sh));
+    const int r0 = ((int)blockIdx.x - (is_x ? 0 : x_tiles)) * 64, k0 = blockIdx.y * 64;
+    const int rows = is_x ? a.n : a.V, padded = is_x ? a.nk : a.Vk;
+    const void* base = is_x ? a.x : a.w;
+    const long ld = is_x ? a.ldx : a.ldw;
+    const bool vec = v_aligned<D>(base, ld);
+    {
+        const int r = threadIdx.x >> 2, k = (threadIdx.x & 3) * 16;
+        const bool in = r0 + r < rows && (!is_x || v_takes_part(a, r0 + r));
+#pragma unroll
+        for (int half = 0; half < 16; half += 8) {
+            float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            if (in && k0 + k + half < a.d) v_chunk<D>(v_row<D>(base, r0 + r, ld), k0 + k + half, a.d, vec, x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) tile[r][k + half + i] = x[i];
+        }
+    }
+    __syncthreads();
+    const int k = threadIdx.x >> 2;
+    if (k0 + k >= a.d) return;
+    unsigned short* out = (is_x ? a.xt : a.wt) + (long)(k0 + k) * padded + r0;
+    const long plane = (long)a.d * padded;
+#pragma unroll
+    for (int half = 0; half < 16; half += 8) {
+        const int at = (threadIdx.x & 3) * 16 + half;
+        vt_u4 h, l;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float v[2];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int p = at + 2 * i + q;
+                v[q] = ldexpf(tile[a.order ? (p & 32) + v_stream_row(p & 31) : p][k], e);
+            }
+            unsigned hh, ll = 0;
+            if constexpr (D == PIN_F32) v_split(v[0], v[1], hh, ll);
+            else hh = v_pack(v[0], v[1]);
+            h[i] = hh;
+            l[i] = ll;
+        }
+        *reinterpret_cast<vt_u4*>(out + at) = h;
+        if constexpr (D == PIN_F32) *reinterpret_cast<vt_u4*>(out + plane + at) = l;
+    }
+}
+
+// one logit from the product: in units of log 2 (16-bit inputs), or as it is, times the two rows' powers of two (fp32)
+template <int SEGS>
+__device__ __forceinline__ float v_logit(float acc, float xs, float ws, float b2) {
+    if constexpr (SEGS == 1) return fmaf(acc, V_LOG2E, b2);
+    else return fmaf(acc, xs * ws, b2);
+}
+// exp of a difference of two of them
+template <int SEGS>
+__device__ __forceinline__ float v_exp(float diff) {
+    return __builtin_amdgcn_exp2f(SEGS == 1 ? diff : diff * V_LOG2E);
+}
+// 2^14 p of a logit that is still a product: `m` and `c` are gm and gc of its row
+template <int SEGS>
+__device__ __forceinline__ float v_prob(float acc, float xs, float ws, float b2, float m, float c) {
+    if constexpr (SEGS == 1) return __builtin_amdgcn_exp2f(fmaf(acc, V_LOG2E, b2 + c));
+    else return __builtin_amdgcn_exp2f(fmaf(fmaf(acc, xs * ws, b2) - m, V_LOG2E, c));
+}
+
+// the wave's 64 labels x 64 rows of logits from their products
+template <int SEGS>
+__device__ __forceinline__ void v_logits(const VocabArgs& a, vt_f4 (&acc)[4][4], int v0, int i0) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+    const int vb = v0 + (wave >> 1) * 64 + 4 * g, ib = i0 + (wave & 1) * 64 + c;
+    float xs[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) xs[j] = SEGS == 1 ? 1.f : a.xs[ib + 16 * j];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const vt_f4 b2 = *reinterpret_cast<const vt_f4*>(a.b2 + vb + 16 * i);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float ws = SEGS == 1 ? 1.f : a.ws_[vb + 16 * i + r];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j][r] = v_logit<SEGS>(acc[i][j][r], xs[j], ws, b2[r]);
+        }
+    }
+}
+
+__device__ __forceinline__ VocabOperand v_operand_w(const VocabArgs& a) {
+    return a.wa != nullptr ? VocabOperand{a.wa, a.dk, (long)a.V * a.dk, a.V} : VocabOperand{reinterpret_cast<const unsigned short*>(a.w), a.ldw, 0, a.V};
+}
+__device__ __forceinline__ VocabOperand v_operand_x(const VocabArgs& a) {
+    return a.xa != nullptr ? VocabOperand{a.xa, a.dk, (long)a.n * a.dk, a.n} : VocabOperand{reinterpret_cast<const unsigned short*>(a.x), a.ldx, 0, a.n};
+}
+
+// (maximum, sum, lowest label of the maximum) of two sets of labels
+template <int SEGS>
+__device__ __forceinline__ void v_join(float& m1, float& s1, int& a1, float m2, float s2, int a2) {
+    const float top = fmaxf(m1, m2);
+    s1 = s1 * v_exp<SEGS>(m1 - top) + s2 * v_exp<SEGS>(m2 - top);
+    a1 = m1 > m2 ? a1 : m2 > m1 ? a2 : min(a1, a2);
+    m1 = top;
+}
+
+// Forward: workgroup (row tile, split of the vocabulary).  A lane keeps (maximum, sum, lowest label of the maximum) of its 4 rows
+// over the labels it sees; they are joined over the lanes, the waves and (vocab_finish_kernel) the splits.
+template <bool BF, int SEGS, bool ARG>
+__global__ __launch_bounds__(256, 2) void vocab_forward_kernel(VocabArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char vlds[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+    const int i0 = blockIdx.x * VT, ib = i0 + (wave & 1) * 64 + c;
+    float m[4], s[4];
+    int arg[4], lab[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        m[j] = V_FLOOR; s[j] = 0.f; arg[j] = 0x7FFFFFFF;
+        lab[j] = !ARG && ib + 16 * j < a.n ? a.labels[ib + 16 * j] : -1;
+    }
+    const VocabOperand W = v_operand_w(a), X = v_operand_x(a);
+    const int t0 = blockIdx.y * a.tiles_per_split, t1 = min(t0 + a.tiles_per_split, a.Vk / VT);
+    for (int t = t0; t < t1; ++t) {
+        const int v0 = t * VT;
+        vt_f4 acc[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = vt_f4{0.f, 0.f, 0.f, 0.f};
+        vt_product<BF, SEGS>(W, X, v0, i0, 0, a.dk / VT_K, vlds, acc);
+        v_logits<SEGS>(a, acc, v0, i0);
+        const int vb = v0 + (wave >> 1) * 64 + 4 * g;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float top = m[j];
+            if constexpr (ARG) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (acc[i][j][r] > top) { top = acc[i][j][r]; arg[j] = vb + 16 * i + r; }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[i][j][r]);
+                const int at = lab[j] - (v0 + (wave >> 1) * 64);
+                if (__any(lab[j] >= 0 && at >= 0 && at < 64)) {  // (the label of one of the wave's rows is among these)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (lab[j] >= 0 && lab[j] == vb + 16 * i + r) a.tlogit[ib + 16 * j] = acc[i][j][r];
+                }
+            }
+            float sum = s[j] * v_exp<SEGS>(m[j] - top);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sum += v_exp<SEGS>(acc[i][j][r] - top);
+            m[j] = top;
+            s[j] = sum;
+        }
+    }
+    // join: lanes g (labels 4 g ..), then the two waves of the same rows
+    __syncthreads();
+    float* sh = reinterpret_cast<float*>(vlds);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int o = 16; o <= 32; o <<= 1) {
+            const float m2 = __shfl_xor(m[j], o, 64), s2 = __shfl_xor(s[j], o, 64);
+            const int a2 = __shfl_xor(arg[j], o, 64);
+            v_join<SEGS>(m[j], s[j], arg[j], m2, s2, a2);
+        }
+        if (wave >= 2 && g == 0) {
+            const int at = (wave & 1) * 64 + 16 * j + c;
+            sh[at] = m[j];
+            sh[VT + at] = s[j];
+            reinterpret_cast<int*>(sh)[2 * VT + at] = arg[j];
+        }
+    }
+    __syncthreads();
+    if (wave < 2 && g == 0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int at = wave * 64 + 16 * j + c;
+            v_join<SEGS>(m[j], s[j], arg[j], sh[at], sh[VT + at], reinterpret_cast<int*>(sh)[2 * VT + at]);
+            if (i0 + at < a.n) {
+                const long o = (long)(i0 + at) * a.splits + blockIdx.y;
+                a.part_ms[o] = make_float2(m[j], s[j]);
+                if constexpr (ARG) a.part_i[o] = arg[j];
+            }
+        }
+    }
+}
+
+// Forward for a few rows (n <= 16 NT): W is read once, straight into the matrix cores' operand, and that is all there is -- no staging, no
+// LDS tiles.  A wave takes 16 RT labels; lane (c, g) reads 16 bytes of label c's row a step (16-bit types: k = 32 s + 8 g ..; fp32, whose
+// products are the fp32 matrix instruction's: k = 16 s + 4 g ..), four consecutive lanes g a contiguous 64 bytes.  Rows that do not
+// begin and end on 16-byte borders (VEC false) are read element by element.
+template <int N>
+struct VInt { static constexpr int value = N; };
+template <int D, int RT, int NT, bool VEC, bool ARG>
+__global__ __launch_bounds__(256) void vocab_few_kernel(VocabArgs a) {
+    constexpr int SEGS = D == PIN_F32 ? 3 : 1, EL = D == PIN_F32 ? 4 : 8, KS = 4 * EL, U = RT == 1 ? 8 : RT == 2 ? 4 : 2;
+    __shared__ float sm[4][16 * NT], ss[4][16 * NT];
+    __shared__ int sa[4][16 * NT];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+    const int v0 = ((int)blockIdx.x * 4 + wave) * 16 * RT;
+    const char* w[RT];
+    const char* x[NT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) w[i] = reinterpret_cast<const char*>(v_row<D>(a.w, min(v0 + 16 * i + c, a.V - 1), a.ldw));
+#pragma unroll
+    for (int j = 0; j < NT; ++j) x[j] = reinterpret_cast<const char*>(v_row<D>(a.x, min(16 * j + c, a.n - 1), a.ldx));
+    vt_f4 acc[RT][NT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = vt_f4{0.f, 0.f, 0.f, 0.f};
+    auto get = [&](const char* row, int k, bool tail) {  // EL elements from k on as they are, zero behind the end of the row
+        vt_u4 u = {0u, 0u, 0u, 0u};
+        if constexpr (VEC) {  // (d is a multiple of EL)
+            if (!tail || k < a.d) u = *reinterpret_cast<const vt_u4*>(row + k * (D == PIN_F32 ? 4 : 2));
+        } else if constexpr (D == PIN_F32) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) u[e] = !tail || k + e < a.d ? reinterpret_cast<const unsigned*>(row)[k + e] : 0u;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                u[e >> 1] |= (!tail || k + e < a.d ? (unsigned)reinterpret_cast<const unsigned short*>(row)[k + e] : 0u) << (16 * (e & 1));
+        }
+        return u;
+    };
+    auto step = [&](int s, auto count, bool tail) {  // `count` steps from s on: all their reads, then their products
+        constexpr int N = decltype(count)::value;
+        vt_u4 wu[N][RT], xu[N][NT];
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const int k = (s + u) * KS + g * EL;
+#pragma unroll
+            for (int i = 0; i < RT; ++i) wu[u][i] = get(w[i], k, tail);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) xu[u][j] = get(x[j], k, tail);
+        }
+#pragma unroll
+        for (int u = 0; u < N; ++u)
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    if constexpr (D == PIN_F32) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(wu[u][i][e]), __uint_as_float(xu[u][j][e]), acc[i][j], 0, 0, 0);
+                    } else {
+                        acc[i][j] = vt_mfma<D == PIN_BF16>(wu[u][i], xu[u][j], acc[i][j]);
+                    }
+                }
+    };
+    const int full = a.d / KS;
+    int s0 = 0;
+    for (; s0 + U <= full; s0 += U) step(s0, VInt<U>{}, false);
+    if (s0 * KS < a.d) step(s0, VInt<U>{}, true);  // (the rest at once: a step at a time would wait for memory each time)
+    float m[NT], s[NT];
+    int arg[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        m[j] = V_FLOOR; s[j] = 0.f; arg[j] = 0x7FFFFFFF;
+        const int row = 16 * j + c, label = !ARG && row < a.n ? a.labels[row] : -1;
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int v = v0 + 16 * i + 4 * g + r;
+                float b = v >= a.V ? -INFINITY : a.bias == nullptr ? 0.f : v_get<D>(a.bias, v);
+                b = b <= V_FLOOR ? -INFINITY : SEGS == 1 ? b * V_LOG2E : b;
+                const float z = v_logit<SEGS>(acc[i][j][r], 1.f, 1.f, b);
+                acc[i][j][r] = z;
+                if (z > m[j]) { m[j] = z; arg[j] = v; }
+                if (!ARG && v == label) a.tlogit[row] = z;
+            }
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[j] += v_exp<SEGS>(acc[i][j][r] - m[j]);
+#pragma unroll
+        for (int o = 16; o <= 32; o <<= 1) {
+            const float m2 = __shfl_xor(m[j], o, 64), s2 = __shfl_xor(s[j], o, 64);
+            const int a2 = __shfl_xor(arg[j], o, 64);
+            v_join<SEGS>(m[j], s[j], arg[j], m2, s2, a2);
+        }
+        if (g == 0) { sm[wave][row] = m[j]; ss[wave][row] = s[j]; sa[wave][row] = arg[j]; }
+    }
+    __syncthreads();
+    const int row = threadIdx.x;
+    if (row < 16 * NT && row < a.n) {
+        float m1 = sm[0][row], s1 = ss[0][row];
+        int a1 = sa[0][row];
+#pragma unroll
+        for (int q = 1; q < 4; ++q) v_join<SEGS>(m1, s1, a1, sm[q][row], ss[q][row], sa[q][row]);
+        const long at = (long)row * a.splits + blockIdx.x;
+        a.part_ms[at] = make_float2(m1, s1);
+        if constexpr (ARG) a.part_i[at] = a1;
+    }
+}
+
+// what the gradient pass reads of a row: 2^14 p = exp2(s + gc) (log 2 units; gc = 14 - log2 sum exp2 s), or exp2((s - gm) / log 2 + gc)
+// with gm the maximum and gc = 14 - log2 of the sum over it
+template <int SEGS>
+__device__ __forceinline__ void v_row_of_gradient(const VocabArgs& a, int i, int label, float m, float log2_total, int eg) {
+    const bool none = i >= a.n || label < 0 || label >= a.V || log2_total == -INFINITY || a.bad[min(i, a.n - 1)] != 0;
+    a.part[i] = none ? -1 : label;
+    a.gm[i] = none || SEGS == 1 ? 0.f : m;
+    a.gc[i] = none ? -INFINITY : 14.f - (SEGS == 1 ? m + log2_total : log2_total);
+    const float g = none ? 0.f : isnan(log2_total) ? NAN : a.grad_nll[i];
+    a.g[i] = g;
+    a.gn[i] = ldexpf(g, eg);
+}
+
+// the exponents of the gradient pass, once for the launches behind (every workgroup of this one needs g's); returns g's
+template <int D>
+__device__ __forceinline__ int v_exponents(const VocabArgs& a, float* sh) {
+    const int eg = v_scale_exp(v_block_max(a.amax + 2 * V_AMAX, sh)) - 15;
+    if (blockIdx.x == 0) {
+        const float mx = v_block_max(a.amax, sh), mw = v_block_max(a.amax + V_AMAX, sh);
+        if (threadIdx.x == 0) {
+            a.exps[0] = eg;
+            a.exps[1] = D == PIN_F16 ? 0 : v_scale_exp(mx);
+            a.exps[2] = D == PIN_F16 ? 0 : v_scale_exp(mw);
+        }
+    }
+    return eg;
+}
+
+// Joins the splits of the forward pass, PER lanes a row (a call for one row has hundreds of splits).
+template <int D, bool ARG, bool GRAD, int PER>
+__global__ __launch_bounds__(256) void vocab_finish_kernel(VocabArgs a) {
+    constexpr int SEGS = D == PIN_F32 ? 3 : 1;
+    __shared__ float sh[4];
+    int eg = 0;
+    if constexpr (GRAD) eg = v_exponents<D>(a, sh);
+    const int part = threadIdx.x % PER, i = blockIdx.x * (256 / PER) + threadIdx.x / PER;
+    float m = V_FLOOR, s = 0.f;
+    int arg = 0x7FFFFFFF;
+    if (i < a.n)
+#pragma unroll 8
+        for (int p = part; p < a.splits; p += PER) {
+            const float2 ms = a.part_ms[(long)i * a.splits + p];
+            v_join<SEGS>(m, s, arg, ms.x, ms.y, ARG ? a.part_i[(long)i * a.splits + p] : 0);
+        }
+#pragma unroll
+    for (int o = PER / 2; o > 0; o >>= 1) {
+        const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64);
+        const int a2 = ARG ? __shfl_xor(arg, o, 64) : 0;
+        v_join<SEGS>(m, s, arg, m2, s2, a2);
+    }
+    if (part != 0 || i >= (GRAD ? a.nk + 64 : a.n)) return;
+    const float log2_total = log2f(s), unit = SEGS == 1 ? V_LN2 : 1.f;
+    if constexpr (ARG) {
+        if (i < a.n) {
+            const bool fine = s > 0.f && s < INFINITY;
+            a.label_out[i] = fine ? arg : -1;
+            a.logprob[i] = s == 0.f ? -INFINITY : fine ? -log2_total * V_LN2 : NAN;  // (the sum holds the largest as 1)
+        }
+    } else {
+        const int label = i < a.n ? a.labels[i] : -1;
+        if (i < a.n) {
+            const bool bad = GRAD && a.bad[i] != 0;
+            a.lse[i] = bad ? NAN : s == 0.f ? -INFINITY : m * unit + log2_total * V_LN2;
+            float nll = 0.f;
+            if (label >= a.V) {
+                nll = NAN;
+                atomicOr(a.status, PIN_STATUS_LABEL_RANGE);
+            } else if (label >= 0) {
+                nll = s == 0.f ? INFINITY : (m - a.tlogit[i]) * unit + log2_total * V_LN2;
+            }
+            a.nll[i] = nll;
+        }
+        if constexpr (GRAD)
+            v_row_of_gradient<SEGS>(a, i, label, m, log2_total, eg);
+    }
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void vocab_prepare_kernel(VocabArgs a) {  // the gradient pass alone, with the lse of an earlier call
+    constexpr int SEGS = D == PIN_F32 ? 3 : 1;
+    __shared__ float sh[4];
+    const int eg = v_exponents<D>(a, sh);
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= a.nk + 64) return;
+    const int label = i < a.n ? a.labels[i] : -1;
+    if (label >= a.V) atomicOr(a.status, PIN_STATUS_LABEL_RANGE);
+    const float lse = i < a.n ? a.lse[i] : 0.f;
+    const float log2_total = lse == -INFINITY ? -INFINITY : isnan(lse) ? NAN : 0.f;
+    v_row_of_gradient<SEGS>(a, i, label, SEGS == 1 ? lse * V_LOG2E : lse, log2_total, eg);
+}
+
+// D of one piece of the vocabulary: the logits again, D [n][piece] and D^T [piece][n] in fp16 (two pieces of fp32)
+template <bool BF, int SEGS>
+__global__ __launch_bounds__(256, 2) void vocab_probs_kernel(VocabArgs a, int p0) {
+    extern __shared__ __attribute__((aligned(16))) char vlds[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+    const int i0 = blockIdx.x * VT, v0 = p0 + blockIdx.y * VT;
+    vt_f4 acc[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = vt_f4{0.f, 0.f, 0.f, 0.f};
+    vt_product<BF, SEGS>(v_operand_w(a), v_operand_x(a), v0, i0, 0, a.dk / VT_K, vlds, acc);
+    const int vb = v0 + (wave >> 1) * 64 + 4 * g, ib = i0 + (wave & 1) * 64 + c;
+    const long plane = (long)a.nk * a.piece;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int row = ib + 16 * j;
+        const float gm = a.gm[row], gc = a.gc[row], gn = a.gn[row], xs = SEGS == 1 ? 1.f : a.xs[row];
+        const int lab = a.part[row];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const vt_f4 b2 = *reinterpret_cast<const vt_f4*>(a.b2 + vb + 16 * i);
+            float d[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float p = v_prob<SEGS>(acc[i][j][r], xs, SEGS == 1 ? 1.f : a.ws_[vb + 16 * i + r], b2[r], gm, gc);
+                d[r] = (lab == vb + 16 * i + r ? p - 0x1p14f : p) * gn;
+            }
+            unsigned h[2], l[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                if constexpr (SEGS > 1) v_split(d[2 * r], d[2 * r + 1], h[r], l[r]);
+                else h[r] = v_pack(d[2 * r], d[2 * r + 1]);
+                const long at = (long)(vb + 16 * i + 2 * r - p0) * a.nk + row;
+                a.pt[at] = (unsigned short)h[r];
+                a.pt[at + a.nk] = (unsigned short)(h[r] >> 16);
+                if constexpr (SEGS > 1) {
+                    a.pt[plane + at] = (unsigned short)l[r];
+                    a.pt[plane + at + a.nk] = (unsigned short)(l[r] >> 16);
+                }
+            }
+            const long at = (long)row * a.piece + vb + 16 * i - p0;
+            *reinterpret_cast<uint2*>(a.p + at) = make_uint2(h[0], h[1]);
+            if constexpr (SEGS > 1) *reinterpret_cast<uint2*>(a.p + plane + at) = make_uint2(l[0], l[1]);
+        }
+    }
+}
+
+// dx += D W over one piece: partial sums [split][n][d], a split of the piece's labels each
+template <int SEGS>
+__global__ __launch_bounds__(256, 2) void vocab_dx_kernel(VocabArgs a, int p0, int width) {
+    extern __shared__ __attribute__((aligned(16))) char vlds[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+    const int i0 = blockIdx.x * VT, k0 = blockIdx.y * VT;
+    const int steps = width / VT_K, per = (steps + a.dx_splits - 1) / a.dx_splits, s0 = min((int)blockIdx.z * per, steps), s1 = min(s0 + per, steps);
+    const VocabOperand P{a.p, a.piece, (long)a.nk * a.piece, a.nk}, WT{a.wt + p0, a.Vk, (long)a.d * a.Vk, a.d};
+    vt_f4 acc[4][4];
+    float* out = a.dxp + (long)blockIdx.z * a.nk * a.dk;
+    const int ib = i0 + (wave >> 1) * 64 + 4 * g, kb = k0 + (wave & 1) * 64 + c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                acc[i][j][r] = p0 > 0 && ib + 16 * i + r < a.n && kb + 16 * j < a.d ? out[(long)(ib + 16 * i + r) * a.dk + kb + 16 * j] : 0.f;
+    vt_product<false, SEGS>(P, WT, i0, k0, (long)s0 * VT_K, s1 - s0, vlds, acc);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (ib + 16 * i + r < a.n && kb + 16 * j < a.d) out[(long)(ib + 16 * i + r) * a.dk + kb + 16 * j] = acc[i][j][r];
+}
+
+// dW and db of one piece
+template <int D, int SEGS>
+__global__ __launch_bounds__(256, 2) void vocab_dw_kernel(VocabArgs a, int p0) {
+    extern __shared__ __attribute__((aligned(16))) char vlds[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+    const int v0 = blockIdx.x * VT, k0 = blockIdx.y * VT;
+    const VocabOperand PT{a.pt, a.nk, (long)a.nk * a.piece, a.piece}, XT{a.xt, a.nk, (long)a.d * a.nk, a.d};
+    vt_f4 acc[4][4], ones[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        ones[i] = vt_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = vt_f4{0.f, 0.f, 0.f, 0.f};
+    }
+    const bool bias = a.db != nullptr && k0 == 0 && (wave & 1) == 0;
+    vt_product<false, SEGS, true>(PT, XT, v0, k0, 0, a.nk / VT_K, vlds, acc, ones, bias);
+    const int eg = a.exps[0] + 14, e = eg + a.exps[1];  // (D holds 2^14 p and the scaled g)
+    const int vb = p0 + v0 + (wave >> 1) * 64 + 4 * g, kb = k0 + (wave & 1) * 64 + c;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int v = vb + 16 * i + r;
+            if (v >= a.V) continue;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (kb + 16 * j < a.d) v_put<D>(a.dw, (long)v * a.d + kb + 16 * j, ldexpf(acc[i][j][r], -e));
+            if (bias && c == 0) v_put<D>(a.db, v, ldexpf(ones[i][r], -eg));
+        }
+}
+
+// ---------------------------------------------------------------------------------------------------- streaming kernels
+template <int D, int KT, int MODE>
+__global__ __launch_bounds__(256, MODE >= VS_DX && KT == 8 && D != PIN_F32 ? 1 : 2) void vocab_stream_kernel(VocabArgs a) {
+    constexpr bool BF = D == PIN_BF16, GRAD = MODE >= VS_DX, OWN_X = MODE != VS_DW;
+    constexpr int PL = D == PIN_F32 ? 2 : 1, SEGS = D == PIN_F32 ? 3 : 1, NJ = vs_nj(PL, KT, MODE >= VS_DX);
+    typedef VsShape<PL, KT, MODE> S;
+    constexpr int TR = S::TR, TROW = S::DK * 2, TTROW = TR * 2, FT = S::DK / 16;
+    extern __shared__ __attribute__((aligned(16))) char vlds[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+    const int o0 = ((int)blockIdx.x * 4 + wave) * 16 * NJ;
+    const VocabOperand X = v_operand_x(a), W = v_operand_w(a);
+    const VocabOperand own = OWN_X ? X : W, str = OWN_X ? W : X;
+    const unsigned short* trans = OWN_X ? a.wt : a.xt;
+    const long trans_ld = OWN_X ? a.Vk : a.nk, trans_plane = (long)a.d * trans_ld;
+
+    // the owners' operand and their numbers
+    vt_u4 o[PL][NJ][KT];
+    float own_b[NJ], own_s[NJ], own_m[NJ];  // b2 or gc; power of two; gm
+    int own_l[NJ];                          // label of the row
+    float own_t[NJ];                        // logit of the row's label, if it is among the lane's
+    float m[NJ], s[NJ];
+    int arg[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        const int row = o0 + 16 * j + c, in = min(row, own.rows - 1);
+#pragma unroll
+        for (int p = 0; p < PL; ++p)
+#pragma unroll
+            for (int k = 0; k < KT; ++k) o[p][j][k] = *reinterpret_cast<const vt_u4*>(own.p + p * own.plane + in * own.ld + k * 32 + g * 8);
+        own_s[j] = PL == 1 ? 1.f : OWN_X ? a.xs[in] : a.ws_[in];
+        own_b[j] = MODE == VS_DX ? a.gc[in] : MODE == VS_DW ? a.b2[in] : 0.f;
+        own_m[j] = PL == 2 && MODE == VS_DX ? a.gm[in] : 0.f;
+        own_l[j] = MODE == VS_DX ? a.part[in] : MODE == VS_FORWARD && row < a.n ? a.labels[in] : -1;
+        m[j] = V_FLOOR; s[j] = 0.f; arg[j] = 0x7FFFFFFF; own_t[j] = -INFINITY;
+    }
+    vt_f4 acc2[GRAD ? FT : 1][NJ], ones[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        ones[j] = vt_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int f = 0; f < (GRAD ? FT : 1); ++f) acc2[f][j] = vt_f4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    const int tiles = (OWN_X ? a.Vk : a.nk) / TR, per = (tiles + (int)gridDim.y - 1) / (int)gridDim.y;
+    const int t0 = min((int)blockIdx.y * per, tiles), t1 = min(t0 + per, tiles);
+    auto load = [&](int t) {
+        char* at = vlds + (t & 1) * S::BUF;
+        const int r0 = t * TR;
+        // the streamed rows' numbers: 64 floats each, one instruction of one wave
+        const float* src[5] = {a.b2, a.ws_, nullptr, nullptr, nullptr};
+        if constexpr (MODE == VS_DW) {
+            src[0] = a.gc; src[1] = a.gn; src[2] = reinterpret_cast<const float*>(a.part); src[3] = a.gm; src[4] = a.xs;
+        }
+#pragma unroll
+        for (int k = 0; k < S::NC; ++k)
+            if (wave == (k & 3))
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src[k] + r0 + lane),
+                                                 (__attribute__((address_space(3))) void*)(at + S::T_BYTES + S::TT_BYTES + k * 256), 4, 0, 0);
+        vs_load<TR, TROW, PL>(str.p, str.ld, str.plane, r0, str.rows - 1, 0, at);
+        if constexpr (GRAD) vs_load<S::DK, TTROW, PL>(trans, trans_ld, trans_plane, 0, a.d - 1, r0, at + S::T_BYTES);
+    };
+    if (t0 < t1) load(t0);
+    for (int t = t0; t < t1; ++t) {
+        // this step has arrived and the other buffer's reads are done, for every wave
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        if (t + 1 < t1) load(t + 1);
+        const char* T = vlds + (t & 1) * S::BUF;
+        const char* TT = T + S::T_BYTES;
+        const float* K = reinterpret_cast<const float*>(TT + S::TT_BYTES);
+        const int r0 = t * TR;
+        // a label of these streamed rows and these owners meets: decided once a step, so that the loops below stay whole
+        bool hot = false;
+        if constexpr (MODE == VS_FORWARD || MODE == VS_DX) {
+            bool mine = false;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) mine |= (unsigned)(own_l[j] - r0) < (unsigned)TR;
+            hot = __any(mine);
+        }
+        if constexpr (MODE == VS_DW) hot = __any(lane < TR && (unsigned)(reinterpret_cast<const int*>(K)[2 * 64 + lane] - o0) < 16u * NJ);
+#pragma unroll 1
+        for (int q = 0; q < TR / 32; ++q) {
+            vt_f4 acc[2][NJ];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) acc[i][j] = vt_f4{0.f, 0.f, 0.f, 0.f};
+                if constexpr (PL == 2) {
+#pragma unroll
+                    for (int k = 0; k < KT; ++k) {
+                        const vt_u4 lo = vs_read<TROW>(T + TR * TROW, 32 * q + 16 * i + c, 4 * k + g);
+#pragma unroll
+                        for (int j = 0; j < NJ; ++j) acc[i][j] = vt_mfma<false>(lo, o[0][j][k], acc[i][j]);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < KT; ++k) {
+                    const vt_u4 hi = vs_read<TROW>(T, 32 * q + 16 * i + c, 4 * k + g);
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) {
+                        if constexpr (PL == 2) acc[i][j] = vt_mfma<false>(hi, o[1][j][k], acc[i][j]);
+                        acc[i][j] = vt_mfma<BF>(hi, o[0][j][k], acc[i][j]);
+                    }
+                }
+            }
+            const int rq = r0 + 32 * q;
+            if constexpr (!GRAD) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const vt_f4 b2 = *reinterpret_cast<const vt_f4*>(K + 32 * q + 16 * i + 4 * g);
+                    vt_f4 ws = {1.f, 1.f, 1.f, 1.f};
+                    if constexpr (PL == 2) ws = *reinterpret_cast<const vt_f4*>(K + 64 + 32 * q + 16 * i + 4 * g);
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) acc[i][j][r] = v_logit<SEGS>(acc[i][j][r], own_s[j], ws[r], b2[r]);
+                }
+                if (MODE == VS_FORWARD && hot) {
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) {
+                        const int at = own_l[j] - rq - 4 * g;
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) own_t[j] = at == 16 * i + r ? acc[i][j][r] : own_t[j];
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    float top = m[j];
+                    if constexpr (MODE == VS_ARGMAX) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                if (acc[i][j][r] > top) { top = acc[i][j][r]; arg[j] = rq + 16 * i + 4 * g + r; }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[i][j][r]);
+                    }
+                    float sum = s[j] * v_exp<SEGS>(m[j] - top);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) sum += v_exp<SEGS>(acc[i][j][r] - top);
+                    m[j] = top;
+                    s[j] = sum;
+                }
+            } else {
+                vt_u4 pb[PL][NJ];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int at = 32 * q + 16 * i + 4 * g;
+                    const vt_f4 k0 = *reinterpret_cast<const vt_f4*>(K + at);
+                    vt_f4 k1 = {1.f, 1.f, 1.f, 1.f}, km = {0.f, 0.f, 0.f, 0.f}, kx = {1.f, 1.f, 1.f, 1.f};
+                    if constexpr (MODE == VS_DW || PL == 2) k1 = *reinterpret_cast<const vt_f4*>(K + 64 + at);  // gn of the rows, or ws of the labels
+                    if constexpr (MODE == VS_DW && PL == 2) {
+                        km = *reinterpret_cast<const vt_f4*>(K + 3 * 64 + at);
+                        kx = *reinterpret_cast<const vt_f4*>(K + 4 * 64 + at);
+                    }
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            acc[i][j][r] = MODE == VS_DX ? v_prob<SEGS>(acc[i][j][r], own_s[j], k1[r], k0[r], own_m[j], own_b[j])
+                                                         : v_prob<SEGS>(acc[i][j][r], kx[r], own_s[j], own_b[j], km[r], k0[r]);
+                    // (the label's p loses its 1 before it is rounded: the gradient of a row that is nearly certain is that difference)
+                    if constexpr (MODE == VS_DX) {
+                        if (hot) {
+#pragma unroll
+                            for (int j = 0; j < NJ; ++j) {
+                                const int l = own_l[j] - rq - 16 * i - 4 * g;
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) acc[i][j][r] -= l == r ? 0x1p14f : 0.f;
+                            }
+                        }
+                    } else {
+                        if (hot) {
+                            const int* L = reinterpret_cast<const int*>(K) + 2 * 64 + at;
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                const int l = L[r];
+#pragma unroll
+                                for (int j = 0; j < NJ; ++j) acc[i][j][r] -= l == o0 + 16 * j + c ? 0x1p14f : 0.f;
+                            }
+                        }
+#pragma unroll
+                        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) acc[i][j][r] *= k1[r];
+                    }
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; r += 2) {
+                            unsigned h, l = 0;
+                            if constexpr (PL == 2) v_split(acc[i][j][r], acc[i][j][r + 1], h, l);
+                            else h = v_pack(acc[i][j][r], acc[i][j][r + 1]);
+                            pb[0][j][2 * i + r / 2] = h;
+                            if constexpr (PL == 2) pb[PL - 1][j][2 * i + r / 2] = l;
+                        }
+                }
+#pragma unroll
+                for (int f = 0; f < FT; ++f) {
+                    if constexpr (PL == 2) {
+                        const vt_u4 lo = vs_read<TTROW>(TT + S::DK * TTROW, 16 * f + c, 4 * q + g);
+#pragma unroll
+                        for (int j = 0; j < NJ; ++j) acc2[f][j] = vt_mfma<false>(lo, pb[0][j], acc2[f][j]);
+                    }
+                    const vt_u4 hi = vs_read<TTROW>(TT, 16 * f + c, 4 * q + g);
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) {
+                        if constexpr (PL == 2) acc2[f][j] = vt_mfma<false>(hi, pb[PL - 1][j], acc2[f][j]);
+                        acc2[f][j] = vt_mfma<false>(hi, pb[0][j], acc2[f][j]);
+                    }
+                }
+                if constexpr (MODE == VS_DW) {
+                    const vt_u4 one = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) {
+                        if constexpr (PL == 2) ones[j] = vt_mfma<false>(one, pb[PL - 1][j], ones[j]);
+                        ones[j] = vt_mfma<false>(one, pb[0][j], ones[j]);
+                    }
+                }
+            }
+        }
+    }
+    if constexpr (!GRAD) {  // join the lanes g of a row
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+#pragma unroll
+            for (int d = 16; d <= 32; d <<= 1) {
+                const float m2 = __shfl_xor(m[j], d, 64), s2 = __shfl_xor(s[j], d, 64);
+                const int a2 = __shfl_xor(arg[j], d, 64);
+                v_join<SEGS>(m[j], s[j], arg[j], m2, s2, a2);
+            }
+            const int row = o0 + 16 * j + c;
+            if (g == 0 && row < a.n) {
+                const long at = (long)row * a.splits + blockIdx.y;
+                a.part_ms[at] = make_float2(m[j], s[j]);
+                if constexpr (MODE == VS_ARGMAX) a.part_i[at] = arg[j];
+            }
+            // (one lane of one split has seen the label; a label that is switched off, or NaN, stays to be told apart by the others' silence)
+            if (MODE == VS_FORWARD && row < a.n && (unsigned)(own_l[j] - t0 * TR) < (unsigned)((t1 - t0) * TR) && ((own_l[j] >> 2) & 3) == g)
+                a.tlogit[row] = own_t[j];
+        }
+    } else {
+        const int rows = OWN_X ? a.n : a.V;
+        float* out = OWN_X ? a.dxp + (long)blockIdx.y * a.nk * a.dk : a.dwp + (long)blockIdx.y * a.Vk * a.dk;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int row = o0 + 16 * j + c;
+            if (row >= rows) continue;
+#pragma unroll
+            for (int f = 0; f < FT; ++f) *reinterpret_cast<vt_f4*>(out + (long)row * a.dk + 16 * f + 4 * g) = acc2[f][j];
+            if (MODE == VS_DW && g == 0) a.dbp[(long)blockIdx.y * a.Vk + row] = ones[j][0];
+        }
+    }
+}
+
+// Sums of the partial gradients, scaled back and rounded to the tensors' type.  A thread adds four neighbours over every GROUPS-th split, and
+// GROUPS threads are joined through LDS: few outputs with many splits still fill the card.  Workgroups: dx, then dW, then db.
+template <int D, int GROUPS>
+__global__ __launch_bounds__(256) void vocab_join_kernel(VocabArgs a, int x_blocks, int w_blocks, int streamed) {
+    constexpr int COLS = 256 / GROUPS;
+    __shared__ vt_f4 sum[GROUPS][COLS];
+    const int eg = a.exps[0] + 14, ex = a.exps[1], ew = a.exps[2];
+    const int b = blockIdx.x, kind = b < x_blocks ? 0 : b < x_blocks + w_blocks ? 1 : 2;
+    const int col = threadIdx.x % COLS, group = threadIdx.x / COLS;
+    const long at = ((long)(b - (kind == 0 ? 0 : kind == 1 ? x_blocks : x_blocks + w_blocks)) * COLS + col) * 4;
+    const long all = kind == 0 ? (long)a.n * a.dk : kind == 1 ? (long)a.V * a.dk : a.V;
+    const long plane = kind == 0 ? (long)a.nk * a.dk : kind == 1 ? (long)a.Vk * a.dk : a.Vk;
+    const float* part = kind == 0 ? a.dxp : kind == 1 ? a.dwp : a.dbp;
+    const int splits = kind == 0 ? a.dx_splits : a.dw_splits;
+    vt_f4 s = {0.f, 0.f, 0.f, 0.f};
+    if (at < all) {
+#pragma unroll 8
+        for (int p = group; p < splits; p += GROUPS) s += *reinterpret_cast<const vt_f4*>(part + p * plane + at);
+    }
+    if constexpr (GROUPS > 1) {
+        sum[group][col] = s;
+        __syncthreads();
+        if (group != 0) return;
+#pragma unroll
+        for (int p = 1; p < GROUPS; ++p) s += sum[p][col];
+    }
+    if (at >= all) return;
+    if (kind == 2) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (at + i < a.V) v_put<D>(a.db, at + i, ldexpf(s[i], -eg));
+        return;
+    }
+    const int row = (int)(at / a.dk), k = (int)(at - (long)row * a.dk), e = kind == 0 ? ew + (streamed ? 14 : eg) : ex + eg;
+    const float g = kind == 0 && streamed ? a.g[row] : 1.f;
+    void* out = kind == 0 ? a.dx : a.dw;
+    const long to = (long)row * a.d + k;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = ldexpf(s[i], -e) * g;
+    if (k + 4 <= a.d && (a.d & 3) == 0 && ((uintptr_t)out & 15) == 0) {
+        if constexpr (D == PIN_F32) *reinterpret_cast<vt_f4*>(reinterpret_cast<float*>(out) + to) = s;
+        else if constexpr (D == PIN_F16) *reinterpret_cast<uint2*>(reinterpret_cast<unsigned short*>(out) + to) = make_uint2(v_pack(s[0], s[1]), v_pack(s[2], s[3]));
+        else {
+            typedef __bf16 b4 __attribute__((ext_vector_type(4)));
+            *reinterpret_cast<b4*>(reinterpret_cast<__bf16*>(out) + to) = b4{(__bf16)s[0], (__bf16)s[1], (__bf16)s[2], (__bf16)s[3]};
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (k + i < a.d) v_put<D>(out, to + i, s[i]);
+    }
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void vocab_no_rows_kernel(VocabArgs a) {  // n = 0: the gradients of W and b are zero
+    const long all = (long)a.V * a.d;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long)gridDim.x * 256) v_put<D>(a.dw, i, 0.f);
+    if (a.db != nullptr)
+        for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < a.V; i += (long)gridDim.x * 256) v_put<D>(a.db, i, 0.f);
+}
+
+// ---------------------------------------------------------------------------------------------------- host
+enum { V_PREDICT = 0, V_NLL = 1, V_GRAD = 2, V_STEP = 3 };
+constexpr int V_STREAM_DIM = 256;  // features of the streaming kernels at most
+// Rows that vocab_few_kernel takes at most: its matrix instructions keep up with the reads of W to 64 rows (fp32: 32)
+inline int v_few_rows(int dtype) { return dtype == PIN_F32 ? 32 : 64; }
+constexpr int V_FILL = 512;        // workgroups a launch is split for: two a compute unit
+
+struct VocabPlan {
+    VocabArgs a;
+    int dtype, kt;  // kt: 32s of features of the streaming kernels, 0: the tiles of vocab_tile.h
+    int few;        // 16s of labels a wave of vocab_few_kernel, 0: another forward kernel
+    long bytes;
+};
+
+inline long v_up(long v, long m) { return (v + m - 1) / m * m; }
+// parts of a long axis: until the card is filled, but none shorter than `least` steps
+inline int v_splits(int workgroups, int steps, int least) {
+    const int s = workgroups >= V_FILL ? 1 : (V_FILL + workgroups - 1) / workgroups, most = (steps + least - 1) / least;
+    return s < most ? s : most;
+}
+inline int vs_owners(int dtype, int kt, bool grad) { return 64 * vs_nj(dtype == PIN_F32 ? 2 : 1, kt, grad); }  // of a workgroup
+
+inline VocabPlan v_plan(const pin_vocab_head* h, int mode, char* base) {
+    VocabPlan p;
+    memset(&p, 0, sizeof(p));
+    VocabArgs& a = p.a;
+    a.n = h->n; a.V = h->vocab; a.d = h->dim;
+    a.x = h->x; a.w = h->weight; a.bias = h->bias; a.ldx = h->x_stride; a.ldw = h->weight_stride;
+    p.kt = a.d <= V_STREAM_DIM ? (a.d + 31) / 32 : 0;
+    a.dk = p.kt > 0 ? 32 * p.kt : (int)v_up(a.d, VT_K); a.nk = (int)v_up(a.n > 0 ? a.n : 1, VT); a.Vk = (int)v_up(a.V, VT);
+    p.dtype = h->dtype;
+    a.order = p.kt > 0;
+    const bool two = h->dtype == PIN_F32, grads = mode == V_GRAD || mode == V_STEP;
+    // (a wave per 16 labels until there are eight waves a compute unit, then up to 64: the rows of x are read once for them)
+    p.few = grads || a.n > v_few_rows(h->dtype) ? 0 : a.V >= 131072 ? 4 : a.V >= 65536 ? 2 : 1;
+    const int planes = two ? 2 : 1;
+    // 16-bit rows that begin and end on 16-byte borders are read where they are
+    const bool copy_w = !p.few && (two || a.d != a.dk || a.ldw % 8 != 0 || (uintptr_t)a.w % 16 != 0);
+    const bool copy_x = !p.few && (grads || two || a.d != a.dk || a.ldx % 8 != 0 || (uintptr_t)a.x % 16 != 0);
+    const int rows = a.nk / VT, tiles = a.Vk / VT;
+    if (p.kt > 0) {
+        const int own = vs_owners(p.dtype, p.kt, false), grad = vs_owners(p.dtype, p.kt, true), tr = planes * p.kt <= 4 ? 64 : 32;
+        // (a part's sums are written and read again: 256 streamed rows at least)
+        a.splits = v_splits((a.nk + own - 1) / own, a.Vk / tr, 1);
+        a.dx_splits = v_splits((a.nk + grad - 1) / grad, a.Vk / tr, 256 / tr);
+        a.dw_splits = v_splits((a.Vk + grad - 1) / grad, a.nk / tr, 256 / tr);
+    } else {
+        a.splits = v_splits(rows, tiles, 1);
+        a.tiles_per_split = (tiles + a.splits - 1) / a.splits;
+        a.splits = (tiles + a.tiles_per_split - 1) / a.tiles_per_split;
+        const int dx_tiles = rows * (int)((a.d + VT - 1) / VT);
+        a.dx_splits = dx_tiles >= 512 ? 1 : (512 + dx_tiles - 1) / dx_tiles;
+        if (a.dx_splits > 16) a.dx_splits = 16;
+        a.dw_splits = 0;
+    }
+    if (p.few) a.splits = (a.V + 64 * p.few - 1) / (64 * p.few);
+    // pieces whose D and D^T take about 256 MB together
+    long piece = (128l << 20) / (2l * planes * a.nk) / VT * VT;
+    if (piece < VT) piece = VT;
+    if (piece > a.Vk) piece = a.Vk;
+    a.piece = (int)piece;
+    long at = 0;
+    auto take = [&](long bytes) {
+        char* q = base + at;
+        at += v_up(bytes, 256);
+        return q;
+    };
+    auto rows_of = [&](long count) { return (float*)take((count + 64) * 4); };  // (64 more: the streaming kernels read whole 64s)
+    a.amax = (float*)take(3 * V_AMAX * 4);
+    a.b2 = rows_of(a.Vk);
+    if (copy_x) a.xa = (unsigned short*)take((long)planes * a.n * a.dk * 2);
+    if (copy_w) a.wa = (unsigned short*)take((long)planes * a.V * a.dk * 2);
+    if (two && !p.few) {
+        a.xs = rows_of(a.nk);
+        a.ws_ = rows_of(a.Vk);
+    }
+    if (mode != V_GRAD) {
+        a.part_ms = (float2*)take((long)a.splits * a.n * 8);
+        if (mode == V_PREDICT) a.part_i = (int*)take((long)a.splits * a.n * 4);
+        else a.tlogit = (float*)take((long)a.nk * 4);
+    }
+    if (grads) {
+        a.xt = (unsigned short*)take((long)planes * a.d * a.nk * 2);
+        a.wt = (unsigned short*)take((long)planes * a.d * a.Vk * 2);
+        a.gm = rows_of(a.nk); a.gc = rows_of(a.nk); a.gn = rows_of(a.nk); a.g = rows_of(a.nk);
+        a.part = (int*)rows_of(a.nk);
+        a.bad = (int*)rows_of(a.nk);
+        a.exps = (int*)take(256);
+        a.dxp = (float*)take((long)a.dx_splits * a.nk * a.dk * 4);
+        if (p.kt > 0) {
+            a.dwp = (float*)take((long)a.dw_splits * a.Vk * a.dk * 4);
+            a.dbp = (float*)take((long)a.dw_splits * a.Vk * 4);
+        } else {
+            a.p = (unsigned short*)take((long)planes * a.nk * a.piece * 2);
+            a.pt = (unsigned short*)take((long)planes * a.nk * a.piece * 2);
+        }
+    }
+    p.bytes = at;
+    return p;
+}
+
+inline int v_check(const pin_vocab_head* h) {
+    PIN_CHECK_ARG(h != nullptr, "NULL head");
+    PIN_CHECK_ARG(h->n >= 0 && h->vocab >= 1 && h->dim >= 1, "n >= 0, vocab >= 1 and dim >= 1 are needed");
+    PIN_CHECK_ARG(h->n <= PIN_VOCAB_MAX && h->vocab <= PIN_VOCAB_MAX && h->dim <= PIN_VOCAB_MAX_DIM, "a size is over PIN_VOCAB_MAX / PIN_VOCAB_MAX_DIM");
+    PIN_CHECK_ARG(h->dtype >= PIN_F32 && h->dtype <= PIN_F16, "unknown dtype");
+    PIN_CHECK_ARG(h->weight && (h->n == 0 || h->x), "NULL tensor");
+    PIN_CHECK_ARG(h->weight_stride >= h->dim && (h->n == 0 || h->x_stride >= h->dim), "a row's stride is below dim");
+    return 0;
+}
+
+// more than 64 KB of LDS has to be asked for, once per kernel
+template <typename F>
+static int v_reserve(F* kernel, int bytes) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    return e == hipSuccess ? 0 : fail(-2, "label head: cannot reserve %d bytes of LDS: %s", bytes, hipGetErrorString(e));
+}
+#define V_RESERVE(kernel, bytes)                              \
+    do {                                                      \
+        static const int reserved = v_reserve(kernel, bytes); \
+        if (reserved != 0) return reserved;                   \
+    } while (0)
+#define V_LAUNCH(kernel, grid, lds, ...) hipLaunchKernelGGL(kernel, grid, dim3(256), lds, s, __VA_ARGS__)
+
+template <int D, int KT, int MODE>
+static int v_stream(const VocabPlan& p, hipStream_t s) {
+    const VocabArgs& a = p.a;
+    constexpr int lds = VsShape<D == PIN_F32 ? 2 : 1, KT, MODE>::LDS;
+    V_RESERVE((&vocab_stream_kernel<D, KT, MODE>), lds);
+    const int own = vs_owners(D, KT, MODE >= VS_DX), splits = MODE == VS_DW ? a.dw_splits : MODE == VS_DX ? a.dx_splits : a.splits;
+    V_LAUNCH((vocab_stream_kernel<D, KT, MODE>), dim3(((MODE == VS_DW ? a.V : a.n) + own - 1) / own, splits), lds, a);
+    return 0;
+}
+template <int D, int MODE>
+static int v_stream_kt(const VocabPlan& p, hipStream_t s) {
+    switch (p.kt) {
+        case 1: return v_stream<D, 1, MODE>(p, s);
+        case 2: return v_stream<D, 2, MODE>(p, s);
+        case 3: return v_stream<D, 3, MODE>(p, s);
+        case 4: return v_stream<D, 4, MODE>(p, s);
+        case 5: return v_stream<D, 5, MODE>(p, s);
+        case 6: return v_stream<D, 6, MODE>(p, s);
+        case 7: return v_stream<D, 7, MODE>(p, s);
+        default: return v_stream<D, 8, MODE>(p, s);
+    }
+}
+
+template <int D, int PER>
+static void v_finish_per(const VocabArgs& a, int mode, int rows, hipStream_t s) {
+    const dim3 grid(cdiv(rows, 256 / PER));
+    if (mode == V_PREDICT) V_LAUNCH((vocab_finish_kernel<D, true, false, PER>), grid, 0, a);
+    else if (mode == V_NLL) V_LAUNCH((vocab_finish_kernel<D, false, false, PER>), grid, 0, a);
+    else V_LAUNCH((vocab_finish_kernel<D, false, true, PER>), grid, 0, a);
+}
+template <int D>
+static void v_finish(const VocabArgs& a, int mode, int rows, hipStream_t s) {
+    if (a.splits > 16) v_finish_per<D, 64>(a, mode, rows, s);
+    else if (a.splits > 1) v_finish_per<D, 8>(a, mode, rows, s);
+    else v_finish_per<D, 1>(a, mode, rows, s);
+}
+
+template <int D, int RT, int NT, bool VEC>
+static void v_few_go(const VocabArgs& a, int mode, hipStream_t s) {
+    if (mode == V_PREDICT) V_LAUNCH((vocab_few_kernel<D, RT, NT, VEC, true>), dim3(a.splits), 0, a);
+    else V_LAUNCH((vocab_few_kernel<D, RT, NT, VEC, false>), dim3(a.splits), 0, a);
+}
+template <int D, int RT, int NT>
+static void v_few_rt(const VocabArgs& a, int mode, hipStream_t s) {
+    const int size = D == PIN_F32 ? 4 : 2;
+    if (((uintptr_t)a.x | (uintptr_t)a.w | (uintptr_t)(a.ldx * size) | (uintptr_t)(a.ldw * size) | (uintptr_t)((long)a.d * size)) % 16 == 0) v_few_go<D, RT, NT, true>(a, mode, s);
+    else v_few_go<D, RT, NT, false>(a, mode, s);
+}
+template <int D>
+static void v_few(const VocabPlan& p, int mode, hipStream_t s) {
+    const VocabArgs& a = p.a;
+    if (a.n <= 16) p.few == 4 ? v_few_rt<D, 4, 1>(a, mode, s) : p.few == 2 ? v_few_rt<D, 2, 1>(a, mode, s) : v_few_rt<D, 1, 1>(a, mode, s);
+    else if (a.n <= 32) p.few == 4 ? v_few_rt<D, 4, 2>(a, mode, s) : p.few == 2 ? v_few_rt<D, 2, 2>(a, mode, s) : v_few_rt<D, 1, 2>(a, mode, s);
+    else if constexpr (D != PIN_F32) p.few == 4 ? v_few_rt<D, 4, 4>(a, mode, s) : p.few == 2 ? v_few_rt<D, 2, 4>(a, mode, s) : v_few_rt<D, 1, 4>(a, mode, s);
+}
+
+template <int D, int GROUPS>
+static void v_join_partial(const VocabPlan& p, hipStream_t s) {
+    const VocabArgs& a = p.a;
+    const long cols = 256 / GROUPS * 4;
+    const int xb = (int)(((long)a.n * a.dk + cols - 1) / cols), wb = p.kt == 0 ? 0 : (int)(((long)a.V * a.dk + cols - 1) / cols);
+    const int bb = p.kt == 0 || a.db == nullptr ? 0 : (int)((a.V + cols - 1) / cols);
+    V_LAUNCH((vocab_join_kernel<D, GROUPS>), dim3(xb + wb + bb), 0, a, xb, wb, p.kt > 0 ? 1 : 0);
+}
+
+template <int D>
+int v_run_typed(const VocabPlan& p, int mode, hipStream_t s) {
+    constexpr int SEGS = D == PIN_F32 ? 3 : 1;
+    constexpr bool BF = D == PIN_BF16;
+    const VocabArgs& a = p.a;
+    const bool grads = mode == V_GRAD || mode == V_STEP;
+    if (p.few) {
+        v_few<D>(p, mode, s);
+        v_finish<D>(a, mode, a.n, s);
+        PIN_CHECK_LAUNCH();
+        return 0;
+    }
+    int lanes = 8;
+    while (lanes < 64 && lanes * 8 < a.dk) lanes *= 2;
+    V_LAUNCH((vocab_rows_kernel<D>), dim3(V_AMAX), 0, a, lanes, grads && D == PIN_BF16 ? 1 : 0);
+    if (grads) V_LAUNCH((vocab_transpose_kernel<D>), dim3(a.nk / 64 + a.Vk / 64, (a.dk + 63) / 64), 0, a, a.nk / 64);
+    PIN_CHECK_LAUNCH();
+    if (mode != V_GRAD) {
+        if (p.kt > 0) {
+            if (int e = mode == V_PREDICT ? v_stream_kt<D, VS_ARGMAX>(p, s) : v_stream_kt<D, VS_FORWARD>(p, s)) return e;
+        } else {
+            V_RESERVE((&vocab_forward_kernel<BF, SEGS, true>), VT_LDS);
+            V_RESERVE((&vocab_forward_kernel<BF, SEGS, false>), VT_LDS);
+            const dim3 grid(a.nk / VT, a.splits);
+            if (mode == V_PREDICT) V_LAUNCH((vocab_forward_kernel<BF, SEGS, true>), grid, VT_LDS, a);
+            else V_LAUNCH((vocab_forward_kernel<BF, SEGS, false>), grid, VT_LDS, a);
+        }
+        v_finish<D>(a, mode, mode == V_STEP ? a.nk + 64 : a.n, s);
+    } else {
+        V_LAUNCH((vocab_prepare_kernel<D>), dim3(cdiv(a.nk + 64, 256)), 0, a);
+    }
+    PIN_CHECK_LAUNCH();
+    if (!grads) return 0;
+    if (p.kt > 0) {
+        if (int e = v_stream_kt<D, VS_DX>(p, s)) return e;
+        if (int e = v_stream_kt<D, VS_DW>(p, s)) return e;
+    } else {
+        const int kt = cdiv(a.d, VT);
+        V_RESERVE((&vocab_probs_kernel<BF, SEGS>), VT_LDS);
+        V_RESERVE((&vocab_dx_kernel<SEGS>), VT_LDS);
+        V_RESERVE((&vocab_dw_kernel<D, SEGS>), VT_LDS);
+        for (int p0 = 0; p0 < a.Vk; p0 += a.piece) {
+            const int width = p0 + a.piece < a.Vk ? a.piece : a.Vk - p0;
+            V_LAUNCH((vocab_probs_kernel<BF, SEGS>), dim3(a.nk / VT, width / VT), VT_LDS, a, p0);
+            V_LAUNCH((vocab_dx_kernel<SEGS>), dim3(a.nk / VT, kt, a.dx_splits), VT_LDS, a, p0, width);
+            V_LAUNCH((vocab_dw_kernel<D, SEGS>), dim3(width / VT, kt), VT_LDS, a, p0);
+        }
+    }
+    const int most = a.dx_splits > a.dw_splits ? a.dx_splits : a.dw_splits;
+    if (most > 16) v_join_partial<D, 16>(p, s);
+    else if (most > 2) v_join_partial<D, 4>(p, s);
+    else v_join_partial<D, 1>(p, s);
+    PIN_CHECK_LAUNCH();
+    return 0;
+}
+
+}  // namespace pin

@@ -33,10 +33,9 @@ struct VsShape {
     static constexpr int BUF = T_BYTES + TT_BYTES + NC * 256;
     static constexpr int LDS = 2 * BUF;
 };
-// owners a wave holds, in tiles of 16: as many as leave the accumulators and the owners' operands in the 256 registers of two waves a SIMD
-template <int PL, int KT, int MODE>
-constexpr int vs_nj() {
-    return MODE < VS_DX ? (PL * KT <= 8 ? 4 : 2) : KT == 2 ? (PL == 1 ? 4 : 2) : PL * KT <= 8 ? 2 : 1;
+// owners a wave holds, in tiles of 16: as many as leave the owners' operands and the accumulators in the 256 registers of two waves a SIMD
+__host__ __device__ constexpr int vs_nj(int PL, int KT, bool grad) {
+    return !grad ? (PL * KT <= 8 ? 4 : 2) : PL == 1 ? (KT <= 3 ? 4 : 2) : KT == 1 ? 4 : KT <= 4 ? 2 : 1;
 }
 
 // position of chunk c (8 k) of row r: the 16 lanes that read one chunk of 16 rows touch every bank once
@@ -50,13 +49,14 @@ __device__ __forceinline__ int vs_place(int r, int c) {
 // `rows` rows of ROW_BYTES of every plane -> LDS, from row `first` on (row `last` again behind it)
 template <int ROWS, int ROW_BYTES, int PL>
 __device__ __forceinline__ void vs_load(const unsigned short* base, long ld, long plane, int first, int last, long k0, char* lds) {
-    constexpr int CH = ROW_BYTES / 16, PER = ROWS * CH / 256;
-    static_assert(ROWS * CH % 256 == 0, "whole instructions of four waves");
+    constexpr int CH = ROW_BYTES / 16, ALL = ROWS * CH / 64, PER = (ALL + 3) / 4;
+    static_assert(ROWS * CH % 64 == 0, "whole instructions");
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int p = 0; p < PL; ++p)
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
+            if (ALL % 4 != 0 && i == PER - 1 && wave >= ALL % 4) continue;  // (a last round that some waves have no part in)
             const int slot = (i * 4 + wave) * 64 + lane, r = slot / CH, c = vs_place<ROW_BYTES>(r, slot % CH);
             const unsigned short* src = base + p * plane + (long)min(first + r, last) * ld + k0 + c * 8;
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
