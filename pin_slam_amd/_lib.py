@@ -24,7 +24,7 @@ PIN_ADAM_ROW_EXCLUDED = -(1 << 31)
 PIN_COMM_ID_BYTES = 128
 PIN_F32, PIN_BF16, PIN_F16 = 0, 1, 2
 PIN_ADAMW_BLOCK = 256
-PIN_VOCAB_MAX = 1 << 24
+PIN_VOCAB_MAX = 1 << 22
 PIN_VOCAB_MAX_DIM = 1 << 16
 PIN_ADAMW_CLOCK_DOUBLES = 8
 

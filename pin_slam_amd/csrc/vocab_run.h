@@ -27,7 +27,7 @@ struct VocabArgs {
     const void* bias;
     long ldx, ldw;
     int n, V, d;
-    int dk, nk, Vk;          // d padded to 64, n and V to 128
+    int dk, nk, Vk;          // d padded to 64, n to 128, V to 128 or 256
     const int* labels;
     const float* grad_nll;
     float* nll;
@@ -38,7 +38,7 @@ struct VocabArgs {
     void* dw;
     void* db;
     // workspace
-    unsigned short *xa, *wa, *xt, *wt, *p, *pt;
+    unsigned short *xa, *wa, *xt, *wt, *p;
     float *xs, *ws_, *b2;
     float *amax;             // [3][V_AMAX] partial maxima of |x|, |W|, |g|
     float2* part_ms;         // (maximum, sum) of a row and split [n][splits]
@@ -283,31 +283,33 @@ __device__ __forceinline__ float v_prob(float acc, float xs, float ws, float b2,
     else return __builtin_amdgcn_exp2f(fmaf(fmaf(acc, xs * ws, b2) - m, V_LOG2E, c));
 }
 
-// the wave's 64 labels x 64 rows of logits from their products
+// the wave's 128 labels x 64 rows of logits from their products
 template <int SEGS>
-__device__ __forceinline__ void v_logits(const VocabArgs& a, vt_f4 (&acc)[4][4], int v0, int i0) {
+__device__ __forceinline__ void v_logits(const VocabArgs& a, vt_f4 (&acc)[VT_MI][VT_NI], int v0, int i0) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
-    const int vb = v0 + (wave >> 1) * 64 + 4 * g, ib = i0 + (wave & 1) * 64 + c;
-    float xs[4];
+    const int vb = v0 + (wave >> 1) * (VT_A / 2) + 4 * g, ib = i0 + (wave & 1) * (VT_B / 2) + c;
+    float xs[VT_NI];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) xs[j] = SEGS == 1 ? 1.f : a.xs[ib + 16 * j];
+    for (int j = 0; j < VT_NI; ++j) xs[j] = SEGS == 1 ? 1.f : a.xs[ib + 16 * j];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < VT_MI; ++i) {
         const vt_f4 b2 = *reinterpret_cast<const vt_f4*>(a.b2 + vb + 16 * i);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const float ws = SEGS == 1 ? 1.f : a.ws_[vb + 16 * i + r];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j][r] = v_logit<SEGS>(acc[i][j][r], xs[j], ws, b2[r]);
+            for (int j = 0; j < VT_NI; ++j) acc[i][j][r] = v_logit<SEGS>(acc[i][j][r], xs[j], ws, b2[r]);
         }
     }
 }
 
 __device__ __forceinline__ VocabOperand v_operand_w(const VocabArgs& a) {
-    return a.wa != nullptr ? VocabOperand{a.wa, a.dk, (long)a.V * a.dk, a.V} : VocabOperand{reinterpret_cast<const unsigned short*>(a.w), a.ldw, 0, a.V};
+    return a.wa != nullptr ? VocabOperand{a.wa, a.dk, (long)a.V * a.dk, a.V, a.dk}
+                           : VocabOperand{reinterpret_cast<const unsigned short*>(a.w), a.ldw, 0, a.V, a.d};
 }
 __device__ __forceinline__ VocabOperand v_operand_x(const VocabArgs& a) {
-    return a.xa != nullptr ? VocabOperand{a.xa, a.dk, (long)a.n * a.dk, a.n} : VocabOperand{reinterpret_cast<const unsigned short*>(a.x), a.ldx, 0, a.n};
+    return a.xa != nullptr ? VocabOperand{a.xa, a.dk, (long)a.n * a.dk, a.n, a.dk}
+                           : VocabOperand{reinterpret_cast<const unsigned short*>(a.x), a.ldx, 0, a.n, a.d};
 }
 
 // (maximum, sum, lowest label of the maximum) of two sets of labels
@@ -325,52 +327,56 @@ template <bool BF, int SEGS, bool ARG>
 __global__ __launch_bounds__(256, 2) void vocab_forward_kernel(VocabArgs a) {
     extern __shared__ __attribute__((aligned(16))) char vlds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
-    const int i0 = blockIdx.x * VT, ib = i0 + (wave & 1) * 64 + c;
-    float m[4], s[4];
-    int arg[4], lab[4];
+    const int i0 = blockIdx.x * VT_B, ib = i0 + (wave & 1) * (VT_B / 2) + c;
+    float m[VT_NI], s[VT_NI];
+    int arg[VT_NI], lab[VT_NI];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < VT_NI; ++j) {
         m[j] = V_FLOOR; s[j] = 0.f; arg[j] = 0x7FFFFFFF;
         lab[j] = !ARG && ib + 16 * j < a.n ? a.labels[ib + 16 * j] : -1;
     }
     const VocabOperand W = v_operand_w(a), X = v_operand_x(a);
-    const int t0 = blockIdx.y * a.tiles_per_split, t1 = min(t0 + a.tiles_per_split, a.Vk / VT);
+    const int t0 = blockIdx.y * a.tiles_per_split, t1 = min(t0 + a.tiles_per_split, a.Vk / VT_A);
     for (int t = t0; t < t1; ++t) {
-        const int v0 = t * VT;
-        vt_f4 acc[4][4];
+        const int v0 = t * VT_A;
+        vt_f4 acc[VT_MI][VT_NI];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < VT_MI; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = vt_f4{0.f, 0.f, 0.f, 0.f};
+            for (int j = 0; j < VT_NI; ++j) acc[i][j] = vt_f4{0.f, 0.f, 0.f, 0.f};
         vt_product<BF, SEGS>(W, X, v0, i0, 0, a.dk / VT_K, vlds, acc);
         v_logits<SEGS>(a, acc, v0, i0);
-        const int vb = v0 + (wave >> 1) * 64 + 4 * g;
+        const int vw = v0 + (wave >> 1) * (VT_A / 2), vb = vw + 4 * g;
+        bool mine = false;  // the label of one of the wave's rows is among these
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < VT_NI; ++j) mine |= (unsigned)(lab[j] - vw) < (unsigned)(VT_A / 2);
+        if (!ARG && __any(mine)) {
+#pragma unroll
+            for (int j = 0; j < VT_NI; ++j)
+#pragma unroll
+                for (int i = 0; i < VT_MI; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (lab[j] == vb + 16 * i + r) a.tlogit[ib + 16 * j] = acc[i][j][r];
+        }
+#pragma unroll
+        for (int j = 0; j < VT_NI; ++j) {
             float top = m[j];
             if constexpr (ARG) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < VT_MI; ++i)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                         if (acc[i][j][r] > top) { top = acc[i][j][r]; arg[j] = vb + 16 * i + r; }
             } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < VT_MI; ++i)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[i][j][r]);
-                const int at = lab[j] - (v0 + (wave >> 1) * 64);
-                if (__any(lab[j] >= 0 && at >= 0 && at < 64)) {  // (the label of one of the wave's rows is among these)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (lab[j] >= 0 && lab[j] == vb + 16 * i + r) a.tlogit[ib + 16 * j] = acc[i][j][r];
-                }
             }
             float sum = s[j] * v_exp<SEGS>(m[j] - top);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < VT_MI; ++i)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) sum += v_exp<SEGS>(acc[i][j][r] - top);
             m[j] = top;
@@ -381,7 +387,7 @@ __global__ __launch_bounds__(256, 2) void vocab_forward_kernel(VocabArgs a) {
     __syncthreads();
     float* sh = reinterpret_cast<float*>(vlds);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < VT_NI; ++j) {
 #pragma unroll
         for (int o = 16; o <= 32; o <<= 1) {
             const float m2 = __shfl_xor(m[j], o, 64), s2 = __shfl_xor(s[j], o, 64);
@@ -389,18 +395,18 @@ __global__ __launch_bounds__(256, 2) void vocab_forward_kernel(VocabArgs a) {
             v_join<SEGS>(m[j], s[j], arg[j], m2, s2, a2);
         }
         if (wave >= 2 && g == 0) {
-            const int at = (wave & 1) * 64 + 16 * j + c;
+            const int at = (wave & 1) * (VT_B / 2) + 16 * j + c;
             sh[at] = m[j];
-            sh[VT + at] = s[j];
-            reinterpret_cast<int*>(sh)[2 * VT + at] = arg[j];
+            sh[VT_B + at] = s[j];
+            reinterpret_cast<int*>(sh)[2 * VT_B + at] = arg[j];
         }
     }
     __syncthreads();
     if (wave < 2 && g == 0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int at = wave * 64 + 16 * j + c;
-            v_join<SEGS>(m[j], s[j], arg[j], sh[at], sh[VT + at], reinterpret_cast<int*>(sh)[2 * VT + at]);
+        for (int j = 0; j < VT_NI; ++j) {
+            const int at = wave * (VT_B / 2) + 16 * j + c;
+            v_join<SEGS>(m[j], s[j], arg[j], sh[at], sh[VT_B + at], reinterpret_cast<int*>(sh)[2 * VT_B + at]);
             if (i0 + at < a.n) {
                 const long o = (long)(i0 + at) * a.splits + blockIdx.y;
                 a.part_ms[o] = make_float2(m[j], s[j]);
@@ -560,10 +566,17 @@ __global__ __launch_bounds__(256) void vocab_finish_kernel(VocabArgs a) {
     float m = V_FLOOR, s = 0.f;
     int arg = 0x7FFFFFFF;
     if (i < a.n)
-#pragma unroll 8
-        for (int p = part; p < a.splits; p += PER) {
-            const float2 ms = a.part_ms[(long)i * a.splits + p];
-            v_join<SEGS>(m, s, arg, ms.x, ms.y, ARG ? a.part_i[(long)i * a.splits + p] : 0);
+        for (int p0 = part; p0 < a.splits; p0 += 8 * PER) {  // (eight reads on the way at a time)
+            float2 ms[8];
+            int at[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int p = p0 + u * PER;
+                ms[u] = p < a.splits ? a.part_ms[(long)i * a.splits + p] : make_float2(V_FLOOR, 0.f);
+                at[u] = ARG && p < a.splits ? a.part_i[(long)i * a.splits + p] : 0x7FFFFFFF;
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v_join<SEGS>(m, s, arg, ms[u].x, ms[u].y, at[u]);
         }
 #pragma unroll
     for (int o = PER / 2; o > 0; o >>= 1) {
@@ -612,108 +625,133 @@ __global__ __launch_bounds__(256) void vocab_prepare_kernel(VocabArgs a) {  // t
     v_row_of_gradient<SEGS>(a, i, label, SEGS == 1 ? lse * V_LOG2E : lse, log2_total, eg);
 }
 
-// D of one piece of the vocabulary: the logits again, D [n][piece] and D^T [piece][n] in fp16 (two pieces of fp32)
+// D of one piece of the vocabulary: the logits again, D [n][piece] in fp16 (two planes of fp32).  A wave's part goes through LDS, so that
+// rows are written 256 bytes at a time (as it lies in the registers it would be 8).
 template <bool BF, int SEGS>
 __global__ __launch_bounds__(256, 2) void vocab_probs_kernel(VocabArgs a, int p0) {
     extern __shared__ __attribute__((aligned(16))) char vlds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
-    const int i0 = blockIdx.x * VT, v0 = p0 + blockIdx.y * VT;
-    vt_f4 acc[4][4];
+    const int i0 = blockIdx.x * VT_B, v0 = p0 + blockIdx.y * VT_A;
+    vt_f4 acc[VT_MI][VT_NI];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < VT_MI; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = vt_f4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < VT_NI; ++j) acc[i][j] = vt_f4{0.f, 0.f, 0.f, 0.f};
     vt_product<BF, SEGS>(v_operand_w(a), v_operand_x(a), v0, i0, 0, a.dk / VT_K, vlds, acc);
-    const int vb = v0 + (wave >> 1) * 64 + 4 * g, ib = i0 + (wave & 1) * 64 + c;
-    const long plane = (long)a.nk * a.piece;
+    const int vb = v0 + (wave >> 1) * (VT_A / 2) + 4 * g, ib = i0 + (wave & 1) * (VT_B / 2) + c;
+    int lab[VT_NI];
+    float gm[VT_NI], gc[VT_NI], gn[VT_NI], xs[VT_NI];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < VT_NI; ++j) {
         const int row = ib + 16 * j;
-        const float gm = a.gm[row], gc = a.gc[row], gn = a.gn[row], xs = SEGS == 1 ? 1.f : a.xs[row];
-        const int lab = a.part[row];
+        lab[j] = a.part[row] - vb;
+        gm[j] = SEGS == 1 ? 0.f : a.gm[row];
+        gc[j] = a.gc[row];
+        gn[j] = a.gn[row];
+        xs[j] = SEGS == 1 ? 1.f : a.xs[row];
+    }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const vt_f4 b2 = *reinterpret_cast<const vt_f4*>(a.b2 + vb + 16 * i);
-            float d[4];
+    for (int i = 0; i < VT_MI; ++i) {
+        const vt_f4 b2 = *reinterpret_cast<const vt_f4*>(a.b2 + vb + 16 * i);
+        vt_f4 ws = {1.f, 1.f, 1.f, 1.f};
+        if constexpr (SEGS > 1) {
+            ws = *reinterpret_cast<const vt_f4*>(a.ws_ + vb + 16 * i);
+
+        }
+#pragma unroll
+        for (int j = 0; j < VT_NI; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                float p = v_prob<SEGS>(acc[i][j][r], xs, SEGS == 1 ? 1.f : a.ws_[vb + 16 * i + r], b2[r], gm, gc);
-                d[r] = (lab == vb + 16 * i + r ? p - 0x1p14f : p) * gn;
+                const float p = v_prob<SEGS>(acc[i][j][r], xs[j], ws[r], b2[r], gm[j], gc[j]);
+                acc[i][j][r] = (lab[j] == 16 * i + r ? p - 0x1p14f : p) * gn[j];
             }
-            unsigned h[2], l[2];
+    }
+    static_assert(4 * (VT_B / 2) * VT_A <= VT_LDS, "a wave's 64 rows of 128 labels");
+    __syncthreads();  // (the products' buffers are read)
+    char* mine = vlds + wave * (VT_B / 2) * VT_A;  // [64 rows][128 labels], 16-byte chunks in the order of vs_place
+    unsigned short* out = a.p + (long)(i0 + (wave & 1) * (VT_B / 2)) * a.piece + (v0 - p0) + (wave >> 1) * (VT_A / 2);
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                if constexpr (SEGS > 1) v_split(d[2 * r], d[2 * r + 1], h[r], l[r]);
-                else h[r] = v_pack(d[2 * r], d[2 * r + 1]);
-                const long at = (long)(vb + 16 * i + 2 * r - p0) * a.nk + row;
-                a.pt[at] = (unsigned short)h[r];
-                a.pt[at + a.nk] = (unsigned short)(h[r] >> 16);
-                if constexpr (SEGS > 1) {
-                    a.pt[plane + at] = (unsigned short)l[r];
-                    a.pt[plane + at + a.nk] = (unsigned short)(l[r] >> 16);
+    for (int plane = 0; plane < (SEGS == 1 ? 1 : 2); ++plane) {
+#pragma unroll
+        for (int j = 0; j < VT_NI; ++j)
+#pragma unroll
+            for (int i = 0; i < VT_MI; ++i) {
+                unsigned h[2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float x = acc[i][j][2 * r], y = acc[i][j][2 * r + 1];
+                    h[r] = v_pack(x, y);
+                    if (SEGS > 1 && plane == 0) {  // what is left is the second plane
+                        asm volatile("" : "+v"(h[r]));
+                        acc[i][j][2 * r] = x - (float)__builtin_bit_cast(_Float16, (unsigned short)h[r]);
+                        acc[i][j][2 * r + 1] = y - (float)__builtin_bit_cast(_Float16, (unsigned short)(h[r] >> 16));
+                    }
                 }
+                *reinterpret_cast<uint2*>(mine + (16 * j + c) * VT_A + (vs_place<VT_A>(16 * j + c, 2 * i + (g >> 1)) << 4) + (g & 1) * 8) =
+                    make_uint2(h[0], h[1]);
             }
-            const long at = (long)row * a.piece + vb + 16 * i - p0;
-            *reinterpret_cast<uint2*>(a.p + at) = make_uint2(h[0], h[1]);
-            if constexpr (SEGS > 1) *reinterpret_cast<uint2*>(a.p + plane + at) = make_uint2(l[0], l[1]);
+#pragma unroll(SEGS == 1 ? 16 : 2)
+        for (int it = 0; it < VT_B / 8; ++it) {
+            const int row = it * 4 + g;
+            *reinterpret_cast<vt_u4*>(out + (long)plane * a.nk * a.piece + (long)row * a.piece + c * 8) = vs_read<VT_A>(mine, row, c);
         }
     }
 }
 
-// dx += D W over one piece: partial sums [split][n][d], a split of the piece's labels each
+// dx += D W over one piece: partial sums [split][n][dk], a split of the piece's labels each
 template <int SEGS>
 __global__ __launch_bounds__(256, 2) void vocab_dx_kernel(VocabArgs a, int p0, int width) {
     extern __shared__ __attribute__((aligned(16))) char vlds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
-    const int i0 = blockIdx.x * VT, k0 = blockIdx.y * VT;
+    const int i0 = blockIdx.x * VT_A, k0 = blockIdx.y * VT_B;
     const int steps = width / VT_K, per = (steps + a.dx_splits - 1) / a.dx_splits, s0 = min((int)blockIdx.z * per, steps), s1 = min(s0 + per, steps);
-    const VocabOperand P{a.p, a.piece, (long)a.nk * a.piece, a.nk}, WT{a.wt + p0, a.Vk, (long)a.d * a.Vk, a.d};
-    vt_f4 acc[4][4];
+    const VocabOperand P{a.p, a.piece, (long)a.nk * a.piece, a.nk, a.piece}, WT{a.wt + p0, a.Vk, (long)a.d * a.Vk, a.d, a.Vk - p0};
+    vt_f4 acc[VT_MI][VT_NI];
     float* out = a.dxp + (long)blockIdx.z * a.nk * a.dk;
-    const int ib = i0 + (wave >> 1) * 64 + 4 * g, kb = k0 + (wave & 1) * 64 + c;
+    const int ib = i0 + (wave >> 1) * (VT_A / 2) + 4 * g, kb = k0 + (wave & 1) * (VT_B / 2) + c;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < VT_MI; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < VT_NI; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 acc[i][j][r] = p0 > 0 && ib + 16 * i + r < a.n && kb + 16 * j < a.d ? out[(long)(ib + 16 * i + r) * a.dk + kb + 16 * j] : 0.f;
     vt_product<false, SEGS>(P, WT, i0, k0, (long)s0 * VT_K, s1 - s0, vlds, acc);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < VT_MI; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < VT_NI; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 if (ib + 16 * i + r < a.n && kb + 16 * j < a.d) out[(long)(ib + 16 * i + r) * a.dk + kb + 16 * j] = acc[i][j][r];
 }
 
-// dW and db of one piece
+// dW and db of one piece: D is taken as it lies, by columns
 template <int D, int SEGS>
 __global__ __launch_bounds__(256, 2) void vocab_dw_kernel(VocabArgs a, int p0) {
     extern __shared__ __attribute__((aligned(16))) char vlds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
-    const int v0 = blockIdx.x * VT, k0 = blockIdx.y * VT;
-    const VocabOperand PT{a.pt, a.nk, (long)a.nk * a.piece, a.piece}, XT{a.xt, a.nk, (long)a.d * a.nk, a.d};
-    vt_f4 acc[4][4], ones[4];
+    const int v0 = blockIdx.x * VT_A, k0 = blockIdx.y * VT_B;
+    const VocabOperand P{a.p, a.piece, (long)a.nk * a.piece, a.nk, a.piece}, XT{a.xt, a.nk, (long)a.d * a.nk, a.d, a.nk};
+    vt_f4 acc[VT_MI][VT_NI], ones[VT_MI];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < VT_MI; ++i) {
         ones[i] = vt_f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = vt_f4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < VT_NI; ++j) acc[i][j] = vt_f4{0.f, 0.f, 0.f, 0.f};
     }
     const bool bias = a.db != nullptr && k0 == 0 && (wave & 1) == 0;
-    vt_product<false, SEGS, true>(PT, XT, v0, k0, 0, a.nk / VT_K, vlds, acc, ones, bias);
+    vt_product<false, SEGS, true, true>(P, XT, v0, k0, 0, a.nk / VT_K, vlds, acc, ones, bias);
     const int eg = a.exps[0] + 14, e = eg + a.exps[1];  // (D holds 2^14 p and the scaled g)
-    const int vb = p0 + v0 + (wave >> 1) * 64 + 4 * g, kb = k0 + (wave & 1) * 64 + c;
+    const int vb = p0 + v0 + (wave >> 1) * (VT_A / 2) + 4 * g, kb = k0 + (wave & 1) * (VT_B / 2) + c;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < VT_MI; ++i)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int v = vb + 16 * i + r;
             if (v >= a.V) continue;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < VT_NI; ++j)
                 if (kb + 16 * j < a.d) v_put<D>(a.dw, (long)v * a.d + kb + 16 * j, ldexpf(acc[i][j][r], -e));
             if (bias && c == 0) v_put<D>(a.db, v, ldexpf(ones[i][r], -eg));
         }
@@ -721,7 +759,7 @@ __global__ __launch_bounds__(256, 2) void vocab_dw_kernel(VocabArgs a, int p0) {
 
 // ---------------------------------------------------------------------------------------------------- streaming kernels
 template <int D, int KT, int MODE>
-__global__ __launch_bounds__(256, MODE >= VS_DX && KT == 8 && D != PIN_F32 ? 1 : 2) void vocab_stream_kernel(VocabArgs a) {
+__global__ __launch_bounds__(256, vs_waves(D == PIN_F32 ? 2 : 1, KT, MODE)) void vocab_stream_kernel(VocabArgs a) {
     constexpr bool BF = D == PIN_BF16, GRAD = MODE >= VS_DX, OWN_X = MODE != VS_DW;
     constexpr int PL = D == PIN_F32 ? 2 : 1, SEGS = D == PIN_F32 ? 3 : 1, NJ = vs_nj(PL, KT, MODE >= VS_DX);
     typedef VsShape<PL, KT, MODE> S;
@@ -754,16 +792,25 @@ __global__ __launch_bounds__(256, MODE >= VS_DX && KT == 8 && D != PIN_F32 ? 1 :
         own_l[j] = MODE == VS_DX ? a.part[in] : MODE == VS_FORWARD && row < a.n ? a.labels[in] : -1;
         m[j] = V_FLOOR; s[j] = 0.f; arg[j] = 0x7FFFFFFF; own_t[j] = -INFINITY;
     }
-    vt_f4 acc2[GRAD ? FT : 1][NJ], ones[NJ];
+    vt_f4 acc2[GRAD ? FT : 1][NJ], ones = {0.f, 0.f, 0.f, 0.f};
+    // what a product of 16-bit inputs starts from: the owner's part of the exponent costs no instruction there (but registers)
+    constexpr bool START = PL == 1 && GRAD && KT < 7;
+    vt_f4 start[NJ];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-        ones[j] = vt_f4{0.f, 0.f, 0.f, 0.f};
+        const float b = START ? own_b[j] * V_LN2 : 0.f;
+        start[j] = vt_f4{b, b, b, b};
 #pragma unroll
         for (int f = 0; f < (GRAD ? FT : 1); ++f) acc2[f][j] = vt_f4{0.f, 0.f, 0.f, 0.f};
     }
 
     const int tiles = (OWN_X ? a.Vk : a.nk) / TR, per = (tiles + (int)gridDim.y - 1) / (int)gridDim.y;
     const int t0 = min((int)blockIdx.y * per, tiles), t1 = min(t0 + per, tiles);
+    VtLoader<TR, TROW> lt;
+    VtLoader<S::DK, TTROW> ltt;
+    lt.init(str.ld);
+    if constexpr (GRAD) ltt.init(trans_ld);
+    const VocabOperand str_t{trans, trans_ld, trans_plane, a.d, (int)trans_ld};
     auto load = [&](int t) {
         char* at = vlds + (t & 1) * S::BUF;
         const int r0 = t * TR;
@@ -777,8 +824,11 @@ __global__ __launch_bounds__(256, MODE >= VS_DX && KT == 8 && D != PIN_F32 ? 1 :
             if (wave == (k & 3))
                 __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src[k] + r0 + lane),
                                                  (__attribute__((address_space(3))) void*)(at + S::T_BYTES + S::TT_BYTES + k * 256), 4, 0, 0);
-        vs_load<TR, TROW, PL>(str.p, str.ld, str.plane, r0, str.rows - 1, 0, at);
-        if constexpr (GRAD) vs_load<S::DK, TTROW, PL>(trans, trans_ld, trans_plane, 0, a.d - 1, r0, at + S::T_BYTES);
+#pragma unroll
+        for (int p = 0; p < PL; ++p) {
+            lt.load(str.p + p * str.plane + r0 * str.ld, vt_left(str, r0, 0), str.ld, at + p * TR * TROW);
+            if constexpr (GRAD) ltt.load(trans + p * trans_plane + r0, vt_left(str_t, 0, r0), trans_ld, at + S::T_BYTES + p * S::DK * TTROW);
+        }
     };
     if (t0 < t1) load(t0);
     for (int t = t0; t < t1; ++t) {
@@ -805,7 +855,7 @@ __global__ __launch_bounds__(256, MODE >= VS_DX && KT == 8 && D != PIN_F32 ? 1 :
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
 #pragma unroll
-                for (int j = 0; j < NJ; ++j) acc[i][j] = vt_f4{0.f, 0.f, 0.f, 0.f};
+                for (int j = 0; j < NJ; ++j) acc[i][j] = START ? start[j] : vt_f4{0.f, 0.f, 0.f, 0.f};
                 if constexpr (PL == 2) {
 #pragma unroll
                     for (int k = 0; k < KT; ++k) {
@@ -885,7 +935,8 @@ __global__ __launch_bounds__(256, MODE >= VS_DX && KT == 8 && D != PIN_F32 ? 1 :
                     for (int j = 0; j < NJ; ++j)
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
-                            acc[i][j][r] = MODE == VS_DX ? v_prob<SEGS>(acc[i][j][r], own_s[j], k1[r], k0[r], own_m[j], own_b[j])
+                            if constexpr (START) acc[i][j][r] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], V_LOG2E, k0[r]));
+                            else acc[i][j][r] = MODE == VS_DX ? v_prob<SEGS>(acc[i][j][r], own_s[j], k1[r], k0[r], own_m[j], own_b[j])
                                                          : v_prob<SEGS>(acc[i][j][r], kx[r], own_s[j], own_b[j], km[r], k0[r]);
                     // (the label's p loses its 1 before it is rounded: the gradient of a row that is nearly certain is that difference)
                     if constexpr (MODE == VS_DX) {
@@ -938,11 +989,14 @@ __global__ __launch_bounds__(256, MODE >= VS_DX && KT == 8 && D != PIN_F32 ? 1 :
                     }
                 }
                 if constexpr (MODE == VS_DW) {
-                    const vt_u4 one = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
+                    // db: a product with ones; those of tile j stand in every fourth row, so that register j of one accumulator takes its sums
 #pragma unroll
                     for (int j = 0; j < NJ; ++j) {
-                        if constexpr (PL == 2) ones[j] = vt_mfma<false>(one, pb[PL - 1][j], ones[j]);
-                        ones[j] = vt_mfma<false>(one, pb[0][j], ones[j]);
+                        unsigned u = (c & 3) == j ? 0x3C003C00u : 0u;
+                        asm volatile("" : "+v"(u));  // (made again each time: kept, it takes registers)
+                        const vt_u4 one = {u, u, u, u};
+                        if constexpr (PL == 2) ones = vt_mfma<false>(one, pb[PL - 1][j], ones);
+                        ones = vt_mfma<false>(one, pb[0][j], ones);
                     }
                 }
             }
@@ -976,7 +1030,7 @@ __global__ __launch_bounds__(256, MODE >= VS_DX && KT == 8 && D != PIN_F32 ? 1 :
             if (row >= rows) continue;
 #pragma unroll
             for (int f = 0; f < FT; ++f) *reinterpret_cast<vt_f4*>(out + (long)row * a.dk + 16 * f + 4 * g) = acc2[f][j];
-            if (MODE == VS_DW && g == 0) a.dbp[(long)blockIdx.y * a.Vk + row] = ones[j][0];
+            if (MODE == VS_DW && g == 0) a.dbp[(long)blockIdx.y * a.Vk + row] = ones[j];
         }
     }
 }
@@ -1057,11 +1111,21 @@ struct VocabPlan {
 };
 
 inline long v_up(long v, long m) { return (v + m - 1) / m * m; }
-// parts of a long axis: until the card is filled, but none shorter than `least` steps
-inline int v_splits(int workgroups, int steps, int least) {
-    const int s = workgroups >= V_FILL ? 1 : (V_FILL + workgroups - 1) / workgroups, most = (steps + least - 1) / least;
-    return s < most ? s : most;
+// Parts of a long axis, none shorter than `least` of its steps, for the shortest time: rounds of `fill` workgroups (a few more than places
+// cost a whole round), and `cost` of the undivided time for each part's sums, written and read again.
+inline int v_splits(int workgroups, int steps, int least, int fill, float cost) {
+    const int most = (steps + least - 1) / least;
+    int best = 1;
+    float best_time = 1e30f;
+    for (int s = 1; s <= most && (s == 1 || (long)workgroups * s <= 4l * fill); ++s) {
+        const long all = (long)workgroups * s, rounds = (all + fill - 1) / fill;
+        const float time = (float)(rounds * fill) / (float)all + cost * s;
+        if (time < best_time) { best_time = time; best = s; }
+    }
+    return best;
 }
+// What a part costs next to the whole of a gradient product over `length`: 8 bytes an output at 3 TB/s against 4 length operations at 600 TFLOP/s
+inline float v_part_cost(int length) { return 400.f / length; }
 inline int vs_owners(int dtype, int kt, bool grad) { return 64 * vs_nj(dtype == PIN_F32 ? 2 : 1, kt, grad); }  // of a workgroup
 
 inline VocabPlan v_plan(const pin_vocab_head* h, int mode, char* base) {
@@ -1071,7 +1135,7 @@ inline VocabPlan v_plan(const pin_vocab_head* h, int mode, char* base) {
     a.n = h->n; a.V = h->vocab; a.d = h->dim;
     a.x = h->x; a.w = h->weight; a.bias = h->bias; a.ldx = h->x_stride; a.ldw = h->weight_stride;
     p.kt = a.d <= V_STREAM_DIM ? (a.d + 31) / 32 : 0;
-    a.dk = p.kt > 0 ? 32 * p.kt : (int)v_up(a.d, VT_K); a.nk = (int)v_up(a.n > 0 ? a.n : 1, VT); a.Vk = (int)v_up(a.V, VT);
+    a.dk = p.kt > 0 ? 32 * p.kt : (int)v_up(a.d, VT_K); a.nk = (int)v_up(a.n > 0 ? a.n : 1, VT_B); a.Vk = (int)v_up(a.V, p.kt > 0 ? 128 : VT_A);
     p.dtype = h->dtype;
     a.order = p.kt > 0;
     const bool two = h->dtype == PIN_F32, grads = mode == V_GRAD || mode == V_STEP;
@@ -1081,28 +1145,28 @@ inline VocabPlan v_plan(const pin_vocab_head* h, int mode, char* base) {
     // 16-bit rows that begin and end on 16-byte borders are read where they are
     const bool copy_w = !p.few && (two || a.d != a.dk || a.ldw % 8 != 0 || (uintptr_t)a.w % 16 != 0);
     const bool copy_x = !p.few && (grads || two || a.d != a.dk || a.ldx % 8 != 0 || (uintptr_t)a.x % 16 != 0);
-    const int rows = a.nk / VT, tiles = a.Vk / VT;
+    const int rows = a.nk / VT_B, tiles = a.Vk / VT_A;
     if (p.kt > 0) {
         const int own = vs_owners(p.dtype, p.kt, false), grad = vs_owners(p.dtype, p.kt, true), tr = planes * p.kt <= 4 ? 64 : 32;
-        // (a part's sums are written and read again: 256 streamed rows at least)
-        a.splits = v_splits((a.nk + own - 1) / own, a.Vk / tr, 1);
-        a.dx_splits = v_splits((a.nk + grad - 1) / grad, a.Vk / tr, 256 / tr);
-        a.dw_splits = v_splits((a.Vk + grad - 1) / grad, a.nk / tr, 256 / tr);
+        a.splits = v_splits((a.nk + own - 1) / own, a.Vk / tr, 1, 256 * vs_waves(planes, p.kt, VS_FORWARD), 0.001f);
+        a.dx_splits = v_splits((a.nk + grad - 1) / grad, a.Vk / tr, 128 / tr, 256 * vs_waves(planes, p.kt, VS_DX), v_part_cost(a.V));
+        a.dw_splits = v_splits((a.Vk + grad - 1) / grad, a.nk / tr, 128 / tr, 256 * vs_waves(planes, p.kt, VS_DW), v_part_cost(a.n));
     } else {
-        a.splits = v_splits(rows, tiles, 1);
+        a.splits = v_splits(rows, tiles, 1, V_FILL, 0.001f);
         a.tiles_per_split = (tiles + a.splits - 1) / a.splits;
         a.splits = (tiles + a.tiles_per_split - 1) / a.tiles_per_split;
-        const int dx_tiles = rows * (int)((a.d + VT - 1) / VT);
-        a.dx_splits = dx_tiles >= 512 ? 1 : (512 + dx_tiles - 1) / dx_tiles;
-        if (a.dx_splits > 16) a.dx_splits = 16;
+        const int features = (a.d + VT_B - 1) / VT_B;
+        // pieces whose D takes half a gigabyte at most and whose dW fills the card, if it can be had
+        long piece = (512l << 20) / (2l * planes * a.nk) / VT_A * VT_A;
+        const long want = v_up((V_FILL + features - 1) / features, 1) * VT_A;
+        if (piece > want) piece = want;
+        if (piece < VT_A) piece = VT_A;
+        if (piece > a.Vk) piece = a.Vk;
+        a.piece = (int)piece;
+        a.dx_splits = v_splits((a.nk + VT_A - 1) / VT_A * features, (int)(piece / VT_K), 8, V_FILL, v_part_cost((int)piece));
         a.dw_splits = 0;
     }
     if (p.few) a.splits = (a.V + 64 * p.few - 1) / (64 * p.few);
-    // pieces whose D and D^T take about 256 MB together
-    long piece = (128l << 20) / (2l * planes * a.nk) / VT * VT;
-    if (piece < VT) piece = VT;
-    if (piece > a.Vk) piece = a.Vk;
-    a.piece = (int)piece;
     long at = 0;
     auto take = [&](long bytes) {
         char* q = base + at;
@@ -1136,8 +1200,7 @@ inline VocabPlan v_plan(const pin_vocab_head* h, int mode, char* base) {
             a.dbp = (float*)take((long)a.dw_splits * a.Vk * 4);
         } else {
             a.p = (unsigned short*)take((long)planes * a.nk * a.piece * 2);
-            a.pt = (unsigned short*)take((long)planes * a.nk * a.piece * 2);
-        }
+            }
     }
     p.bytes = at;
     return p;
@@ -1254,7 +1317,7 @@ int v_run_typed(const VocabPlan& p, int mode, hipStream_t s) {
         } else {
             V_RESERVE((&vocab_forward_kernel<BF, SEGS, true>), VT_LDS);
             V_RESERVE((&vocab_forward_kernel<BF, SEGS, false>), VT_LDS);
-            const dim3 grid(a.nk / VT, a.splits);
+            const dim3 grid(a.nk / VT_B, a.splits);
             if (mode == V_PREDICT) V_LAUNCH((vocab_forward_kernel<BF, SEGS, true>), grid, VT_LDS, a);
             else V_LAUNCH((vocab_forward_kernel<BF, SEGS, false>), grid, VT_LDS, a);
         }
@@ -1268,15 +1331,15 @@ int v_run_typed(const VocabPlan& p, int mode, hipStream_t s) {
         if (int e = v_stream_kt<D, VS_DX>(p, s)) return e;
         if (int e = v_stream_kt<D, VS_DW>(p, s)) return e;
     } else {
-        const int kt = cdiv(a.d, VT);
+        const int kt = cdiv(a.d, VT_B);
         V_RESERVE((&vocab_probs_kernel<BF, SEGS>), VT_LDS);
         V_RESERVE((&vocab_dx_kernel<SEGS>), VT_LDS);
         V_RESERVE((&vocab_dw_kernel<D, SEGS>), VT_LDS);
         for (int p0 = 0; p0 < a.Vk; p0 += a.piece) {
             const int width = p0 + a.piece < a.Vk ? a.piece : a.Vk - p0;
-            V_LAUNCH((vocab_probs_kernel<BF, SEGS>), dim3(a.nk / VT, width / VT), VT_LDS, a, p0);
-            V_LAUNCH((vocab_dx_kernel<SEGS>), dim3(a.nk / VT, kt, a.dx_splits), VT_LDS, a, p0, width);
-            V_LAUNCH((vocab_dw_kernel<D, SEGS>), dim3(width / VT, kt), VT_LDS, a, p0);
+            V_LAUNCH((vocab_probs_kernel<BF, SEGS>), dim3(a.nk / VT_B, width / VT_A), VT_LDS, a, p0);
+            V_LAUNCH((vocab_dx_kernel<SEGS>), dim3(cdiv(a.nk, VT_A), kt, a.dx_splits), VT_LDS, a, p0, width);
+            V_LAUNCH((vocab_dw_kernel<D, SEGS>), dim3(width / VT_A, kt), VT_LDS, a, p0);
         }
     }
     const int most = a.dx_splits > a.dw_splits ? a.dx_splits : a.dw_splits;

@@ -38,41 +38,12 @@ __host__ __device__ constexpr int vs_nj(int PL, int KT, bool grad) {
     return !grad ? (PL * KT <= 8 ? 4 : 2) : PL == 1 ? (KT <= 3 ? 4 : 2) : KT == 1 ? 4 : KT <= 4 ? 2 : 1;
 }
 
-// position of chunk c (8 k) of row r: the 16 lanes that read one chunk of 16 rows touch every bank once
-template <int ROW_BYTES>
-__device__ __forceinline__ int vs_place(int r, int c) {
-    if constexpr (ROW_BYTES % 256 == 0) return c ^ (r & 15);
-    else if constexpr (ROW_BYTES % 128 == 0) return c ^ ((r >> 1) & 7);
-    else return c ^ ((r >> 2) & 3);
+// waves a SIMD that their registers leave room for (512 a lane): what hides the way from product to exponential to product in each of them
+__host__ __device__ constexpr int vs_waves(int PL, int KT, int mode) {
+    if (mode < VS_DX) return PL * KT <= 2 ? 4 : PL == 1 && KT == 3 ? 3 : 2;
+    if (PL == 1) return KT == 1 ? 3 : KT == 8 ? 1 : 2;
+    return KT == 1 && mode == VS_DX ? 3 : 2;
 }
-
-// `rows` rows of ROW_BYTES of every plane -> LDS, from row `first` on (row `last` again behind it)
-template <int ROWS, int ROW_BYTES, int PL>
-__device__ __forceinline__ void vs_load(const unsigned short* base, long ld, long plane, int first, int last, long k0, char* lds) {
-    constexpr int CH = ROW_BYTES / 16, ALL = ROWS * CH / 64, PER = (ALL + 3) / 4;
-    static_assert(ROWS * CH % 64 == 0, "whole instructions");
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int p = 0; p < PL; ++p)
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            if (ALL % 4 != 0 && i == PER - 1 && wave >= ALL % 4) continue;  // (a last round that some waves have no part in)
-            const int slot = (i * 4 + wave) * 64 + lane, r = slot / CH, c = vs_place<ROW_BYTES>(r, slot % CH);
-            const unsigned short* src = base + p * plane + (long)min(first + r, last) * ld + k0 + c * 8;
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                             (__attribute__((address_space(3))) void*)(lds + p * ROWS * ROW_BYTES + (i * 4 + wave) * 1024), 16, 0, 0);
-        }
-}
-template <int ROW_BYTES>
-__device__ __forceinline__ vt_u4 vs_read(const char* lds, int r, int c) {
-    return *reinterpret_cast<const vt_u4*>(lds + r * ROW_BYTES + (vs_place<ROW_BYTES>(r, c) << 4));
-}
-
-struct VsSide {
-    VocabOperand op;              // [plane][row][k]
-    const unsigned short* trans;  // [plane][feature][row], in the order of v_stream_row
-    long trans_ld, trans_plane;
-};
 
 // two fp32 -> two fp16, the first in the low half
 __device__ __forceinline__ unsigned v_pack(float x, float y) {

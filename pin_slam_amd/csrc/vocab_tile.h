@@ -1,13 +1,17 @@
-// The matrix-core tile of the label head (vocab.hip): C[a][b] = sum_k A[a][k] B[b][k] over 16-bit operands with k contiguous,
-// accumulated in fp32.
+// The matrix-core tile of the label head (vocab_run.h): C[a][b] = sum_k A[a][k] B[b][k] over 16-bit operands, accumulated in fp32.
 //
-// Operands lie in memory as [plane][row][k], rows padded with zeros to a multiple of 64 k.  A value of fp32 is two planes of fp16,
+// Operands lie in memory as [plane][row][k], rows padded with zeros to a multiple of 32 k.  A value of fp32 is two planes of fp16,
 // x 2^e = h + l (11 bits each), and its product three matrix products, l h + h l + h h, accumulated in that order: l l, at
-// most 2^-22 of the product, is left out.
+// most 2^-22 of the product, is left out.  A may also lie as [plane][k][row] (TRANS): its operand is then put together by the
+// LDS' transposing reads (each takes a 4 x 16 block of 16-bit values by columns).
 //
-// LDS: a row's 64 k of one step are 8 chunks of 16 bytes; chunk c of row r is kept at position c ^ ((r >> 1) & 7), so that the 16
-// lanes that read one chunk of 16 rows touch every bank once.  The loads write LDS directly (the lane's place is fixed, so the
-// permutation is in the addresses they read).
+// 256 x 128 a workgroup, 128 x 64 a wave: each operand read from LDS feeds 4 or 8 matrix instructions, three quarters of what LDS can give
+// at their full rate.  Steps of 32 k, three buffers: a step's loads are on the way while two others are worked on, and two workgroups
+// fit a compute unit, so that the epilogue of one (exponentials, stores) runs beside the products of the other.
+//
+// LDS: the loads write it directly, so the order within a row is in the addresses they read from: chunk c (16 bytes) of row r is kept at
+// vs_place(r, c), such that the 16 lanes that read one chunk of 16 rows touch every bank once.  Rows behind an operand's end read
+// as zeros (the buffer's own bound).
 #pragma once
 #include "pin_common.h"
 
@@ -18,16 +22,17 @@ typedef __bf16 vt_b8 __attribute__((ext_vector_type(8)));
 typedef float vt_f4 __attribute__((ext_vector_type(4)));
 typedef unsigned int vt_u4 __attribute__((ext_vector_type(4)));
 
-constexpr int VT = 128;        // rows of A and of B a workgroup
-constexpr int VT_K = 64;       // k of one step
-constexpr int VT_SIDE = VT * VT_K * 2;     // bytes of one operand's step
-constexpr int VT_LDS = 2 * 2 * VT_SIDE;    // two operands, two buffers
+constexpr int VT_A = 256, VT_B = 128;      // rows of A and of B a workgroup
+constexpr int VT_K = 32, VT_STEPS = 3;     // k of one step, buffers
+constexpr int VT_MI = VT_A / 32, VT_NI = VT_B / 32;  // 16 x 16 tiles of a wave
+constexpr int VT_A_BYTES = VT_A * VT_K * 2, VT_BUF = VT_A_BYTES + VT_B * VT_K * 2, VT_LDS = VT_STEPS * VT_BUF;
 
 struct VocabOperand {
     const unsigned short* p;
     long ld;     // elements from row to row
     long plane;  // elements from plane to plane
-    int rows;
+    int rows;    // of a plane
+    int cols;    // valid elements of a row
 };
 
 template <bool BF>
@@ -36,73 +41,128 @@ __device__ __forceinline__ vt_f4 vt_mfma(vt_u4 a, vt_u4 b, vt_f4 c) {
     else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(vt_h8, a), __builtin_bit_cast(vt_h8, b), c, 0, 0, 0);
 }
 
-// one operand's step: 128 rows from `row0` on (rows behind the last one read the last one again: their results are not used), 64 k
-__device__ __forceinline__ void vt_load(const VocabOperand& o, int plane, int row0, long k0, char* lds) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+template <int ROW_BYTES, bool TRANS = false>
+__device__ __forceinline__ int vs_place(int r, int c) {
+    if constexpr (TRANS) return c ^ ((((r & 3) | ((r >> 1) & 4)) << 1));  // (16 rows at once, 32 bytes of each)
+    else if constexpr (ROW_BYTES % 256 == 0) return c ^ (r & 15);
+    else if constexpr (ROW_BYTES % 128 == 0) return c ^ ((r >> 1) & 7);
+    else return c ^ ((r >> 2) & 3);
+}
+
+// ROWS rows of ROW_BYTES each, global memory -> LDS, by the workgroup's four waves.  What a lane reads is its offset from the tile's first
+// byte, the same in every step: the step is in the (scalar) base.
+template <int ROWS, int ROW_BYTES, bool TRANS = false>
+struct VtLoader {
+    static constexpr int CH = ROW_BYTES / 16, ALL = ROWS * CH / 64, PER = (ALL + 3) / 4;
+    static_assert(ROWS * CH % 64 == 0, "whole instructions");
+    // a round of the four waves takes whole rows, and as many as the places repeat after: the rounds differ by a scalar alone
+    static constexpr bool EVEN = 256 % CH == 0 && (256 / CH) % 16 == 0;
+    unsigned off[EVEN ? 1 : PER];
+    __device__ __forceinline__ void init(long ld) {  // elements from row to row; 256 rows of 2^22 elements still fit 32 bits
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int slot = (wave * 4 + i) * 64 + lane, r = slot >> 3, c = (slot & 7) ^ ((r >> 1) & 7);
-        const unsigned short* src = o.p + plane * o.plane + (long)min(row0 + r, o.rows - 1) * o.ld + k0 + c * 8;
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                         (__attribute__((address_space(3))) void*)(lds + (wave * 4 + i) * 1024), 16, 0, 0);
+        for (int i = 0; i < (EVEN ? 1 : PER); ++i) {
+            const int slot = (i * 4 + wave) * 64 + lane, r = slot / CH;
+            off[i] = (unsigned)r * (unsigned)(ld * 2) + vs_place<ROW_BYTES, TRANS>(r, slot % CH) * 16;
+        }
     }
+    // first: the tile's first element (of a plane); left: bytes from there to the end of what may be read; ld: as for init
+    __device__ __forceinline__ void load(const unsigned short* first, long left, long ld, char* lds) const {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            if (ALL % 4 != 0 && i == PER - 1 && wave >= ALL % 4) continue;  // (a last round that some waves have no part in)
+#if defined(__HIP_DEVICE_COMPILE__)  // (the host pass has no buffer resources)
+            const long rows = EVEN ? (long)i * (256 / CH) * ld : 0, rest = left - 2 * rows;
+            const unsigned bytes = rest <= 0 ? 0u : rest > 0xFFFFFFFFl ? 0xFFFFFFFFu : (unsigned)rest;
+            const auto buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned short*>(first + rows), 0, (int)bytes, 0x00027000);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (__attribute__((address_space(3))) void*)(lds + (i * 4 + wave) * 1024), 16,
+                                                     off[EVEN ? 0 : i], 0, 0, 0);
+#endif
+        }
+    }
+};
+template <int ROW_BYTES>
+__device__ __forceinline__ vt_u4 vs_read(const char* lds, int r, int c) {
+    return *reinterpret_cast<const vt_u4*>(lds + r * ROW_BYTES + (vs_place<ROW_BYTES>(r, c) << 4));
+}
+// bytes from element (row, col) of a plane to its end
+__device__ __forceinline__ long vt_left(const VocabOperand& o, long row, long col) { return ((o.rows - 1 - row) * o.ld + o.cols - col) * 2; }
+
+// operand over k of 16 columns from `col` on of a tile [32 k][VT_A]: the lane's k = 8 g ..
+__device__ __forceinline__ vt_u4 vt_read_trans(const char* lds, int col) {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    const int lane = threadIdx.x & 63, g = lane >> 4, row = 8 * g + ((lane >> 2) & 3);
+    const int at = row * (VT_A * 2) + (vs_place<VT_A * 2, true>(row, col / 8 + ((lane >> 1) & 1)) << 4) + (lane & 1) * 8;
+    typedef __attribute__((address_space(3))) s4* ptr;
+    const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(lds + at));
+    const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(lds + at + 4 * VT_A * 2));  // (four rows on: the same place)
+    typedef short s8 __attribute__((ext_vector_type(8)));
+    return __builtin_bit_cast(vt_u4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-// the lane's 8 k (chunk) of row r
-__device__ __forceinline__ vt_u4 vt_read(const char* lds, int r, int chunk) {
-    return *reinterpret_cast<const vt_u4*>(lds + r * 128 + ((chunk ^ ((r >> 1) & 7)) << 4));
-}
-
-// acc[i][j]: 16 x 16 tiles of the wave's 64 x 64 quarter; lane (n = lane & 15, g = lane >> 4), register r holds row 16 i + 4 g + r of A's
-// and row 16 j + n of B's quarter.  ONES (and `sum`, of a whole wave): also sum_k A[a][k] in `ones`, a product with ones.
-template <bool BF, int SEGS, bool ONES = false>
+// acc[i][j]: 16 x 16 tiles of the wave's 128 x 64; lane (n = lane & 15, g = lane >> 4), register r holds row 16 i + 4 g + r of A's and row
+// 16 j + n of B's part.  ONES (and `sum`, of a whole wave): also sum_k A[a][k] in `ones`, a product with ones.
+template <bool BF, int SEGS, bool TRANS, bool ONES>
 __device__ __forceinline__ void vt_product(const VocabOperand& A, const VocabOperand& B, int a0, int b0, long k0, int steps, char* lds,
-                                           vt_f4 (&acc)[4][4], vt_f4 (&ones)[ONES ? 4 : 1], bool sum = false) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wa = (wave >> 1) * 64, wb = (wave & 1) * 64;
-    auto load = [&](int t) {
-        const int seg = SEGS == 1 ? 0 : t / steps;
-        const long k = k0 + (long)(SEGS == 1 ? t : t - seg * steps) * VT_K;
-        char* at = lds + (t & 1) * 2 * VT_SIDE;
-        vt_load(A, SEGS > 1 && seg == 0 ? 1 : 0, a0, k, at);
-        vt_load(B, SEGS > 1 && seg == 1 ? 1 : 0, b0, k, at + VT_SIDE);
-    };
+                                           vt_f4 (&acc)[VT_MI][VT_NI], vt_f4 (&ones)[ONES ? VT_MI : 1], bool sum) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wa = (wave >> 1) * (VT_A / 2), wb = (wave & 1) * (VT_B / 2);
+    VtLoader<TRANS ? VT_K : VT_A, TRANS ? VT_A * 2 : VT_K * 2, TRANS> la;
+    VtLoader<VT_B, VT_K * 2> lb;
+    la.init(A.ld);
+    lb.init(B.ld);
+    constexpr int LOADS = decltype(la)::PER + decltype(lb)::PER;
+    static_assert(LOADS == 6, "the wait below counts a step's loads");
     const int all = SEGS * steps;
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();  // the last reads of an earlier product are done
-    if (all > 0) load(0);
+    int seg = 0, at = 0, put = 0;  // of the next step to load: its product and place in it, and the buffer it goes to
+    auto load = [&]() {
+        const long k = k0 + (long)at * VT_K;
+        const int pa = SEGS > 1 && seg == 0 ? 1 : 0, pb = SEGS > 1 && seg == 1 ? 1 : 0;
+        char* to = lds + put * VT_BUF;
+        if constexpr (TRANS) la.load(A.p + pa * A.plane + k * A.ld + a0, vt_left(A, k, a0), A.ld, to);
+        else la.load(A.p + pa * A.plane + a0 * A.ld + k, vt_left(A, a0, k), A.ld, to);
+        lb.load(B.p + pb * B.plane + b0 * B.ld + k, vt_left(B, b0, k), B.ld, to + VT_A_BYTES);
+        if (++at == steps) { at = 0; ++seg; }
+        put = put == VT_STEPS - 1 ? 0 : put + 1;
+    };
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();  // the last reads of what LDS held before are done
+    if (all > 0) load();
+    if (all > 1) load();
+    int get = 0;
     for (int t = 0; t < all; ++t) {
-        // this step's tiles have arrived and the other buffer's reads are done, for every wave
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        // this step has arrived (the one behind it may be on its way), and every wave is done with the buffer that the next one goes to
+        if (t + 1 < all) asm volatile("s_waitcnt vmcnt(6) lgkmcnt(0)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
-        if (t + 1 < all) load(t + 1);
-        const char* la = lds + (t & 1) * 2 * VT_SIDE;
-        const char* lb = la + VT_SIDE;
+        if (t + 2 < all) load();
+        const char* ta = lds + get * VT_BUF;
+        const char* tb = ta + VT_A_BYTES;
+        get = get == VT_STEPS - 1 ? 0 : get + 1;
+        vt_u4 a[VT_MI], b[VT_NI];
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            vt_u4 a[4], b[4];
+        for (int j = 0; j < VT_NI; ++j) b[j] = vs_read<VT_K * 2>(tb, wb + 16 * j + (lane & 15), lane >> 4);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                a[i] = vt_read(la, wa + 16 * i + (lane & 15), kk * 4 + (lane >> 4));
-                b[i] = vt_read(lb, wb + 16 * i + (lane & 15), kk * 4 + (lane >> 4));
-            }
+        for (int i = 0; i < VT_MI; ++i) {
+            if constexpr (TRANS) a[i] = vt_read_trans(ta, wa + 16 * i);
+            else a[i] = vs_read<VT_K * 2>(ta, wa + 16 * i + (lane & 15), lane >> 4);
+        }
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < VT_MI; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = vt_mfma<BF>(a[i], b[j], acc[i][j]);
-            if (ONES && sum && (SEGS == 1 || t < steps || t >= 2 * steps)) {  // (of two pieces each once: segment 0 has l, segment 2 h)
-                const vt_u4 one = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
+            for (int j = 0; j < VT_NI; ++j) acc[i][j] = vt_mfma<BF>(a[i], b[j], acc[i][j]);
+        if (ONES && sum && (SEGS == 1 || t < steps || t >= 2 * steps)) {  // (of two pieces each once: the first product has l, the last h)
+            const vt_u4 one = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
 #pragma unroll
-                for (int i = 0; i < (ONES ? 4 : 1); ++i) ones[i] = vt_mfma<BF>(a[i], one, ones[i]);
-            }
+            for (int i = 0; i < (ONES ? VT_MI : 1); ++i) ones[i] = vt_mfma<BF>(a[i], one, ones[i]);
         }
     }
 }
-
 template <bool BF, int SEGS>
 __device__ __forceinline__ void vt_product(const VocabOperand& A, const VocabOperand& B, int a0, int b0, long k0, int steps, char* lds,
-                                           vt_f4 (&acc)[4][4]) {
+                                           vt_f4 (&acc)[VT_MI][VT_NI]) {
     vt_f4 none[1];
-    vt_product<BF, SEGS, false>(A, B, a0, b0, k0, steps, lds, acc, none);
+    vt_product<BF, SEGS, false, false>(A, B, a0, b0, k0, steps, lds, acc, none, false);
 }
 
 }  // namespace pin

@@ -52,7 +52,7 @@ def test_entry_points_refuse_bad_arguments():
     need = L.pin_vocab_workspace_bytes(128, 256, 64, 0, 1)
     assert need > 0
     for bad in (dict(n=-1), dict(vocab=0), dict(dim=0), dict(dtype=3), dict(x=None), dict(weight=None), dict(x_stride=63), dict(weight_stride=1),
-                dict(n=(1 << 24) + 1), dict(vocab=(1 << 24) + 1), dict(dim=(1 << 16) + 1)):
+                dict(n=(1 << 22) + 1), dict(vocab=(1 << 22) + 1), dict(dim=(1 << 16) + 1)):
         assert L.pin_vocab_nll_step(head(**bad), at, at, at, at, at, at, at, at, need, None) < 0, bad
         assert L.pin_vocab_predict(head(**bad), at, at, at, need, None) < 0, bad
     assert L.pin_vocab_nll_step(head(), at, at, at, at, at, at, at, at, need - 256, None) < 0  # workspace too small
