@@ -49,6 +49,7 @@ struct VocabArgs {
     int* bad;                // 1: no label and not finite (its copy in xa is zero)
     float *dxp, *dwp, *dbp;  // partial sums [splits][nk][dk], [splits][Vk][dk], [splits][Vk]
     int splits, tiles_per_split, dx_splits, dw_splits, piece;
+    long ldp, ldxt, ldwt;    // rows of D, x^T, W^T: 128 bytes longer than a power of two of them may be, or their columns share a few channels
     int* exps;               // exponents: of the scaled g (below 1), of x^T's and of W^T's power of two
     int order;               // 1: the transposed operands in the order of v_stream_row
     int* status;
@@ -222,7 +223,8 @@ __global__ __launch_bounds__(256) void vocab_transpose_kernel(VocabArgs a, int x
     const bool is_x = (int)blockIdx.x < x_tiles;
     const int e = D == PIN_F16 ? 0 : v_scale_exp(v_block_max(a.amax + (is_x ? 0 : V_AMAX), sh));
     const int r0 = ((int)blockIdx.x - (is_x ? 0 : x_tiles)) * 64, k0 = blockIdx.y * 64;
-    const int rows = is_x ? a.n : a.V, padded = is_x ? a.nk : a.Vk;
+    const int rows = is_x ? a.n : a.V;
+    const long padded = is_x ? a.ldxt : a.ldwt;
     const void* base = is_x ? a.x : a.w;
     const long ld = is_x ? a.ldx : a.ldw;
     const bool vec = v_aligned<D>(base, ld);
@@ -240,8 +242,8 @@ __global__ __launch_bounds__(256) void vocab_transpose_kernel(VocabArgs a, int x
     __syncthreads();
     const int k = threadIdx.x >> 2;
     if (k0 + k >= a.d) return;
-    unsigned short* out = (is_x ? a.xt : a.wt) + (long)(k0 + k) * padded + r0;
-    const long plane = (long)a.d * padded;
+    unsigned short* out = (is_x ? a.xt : a.wt) + (k0 + k) * padded + r0;
+    const long plane = a.d * padded;
 #pragma unroll
     for (int half = 0; half < 16; half += 8) {
         const int at = (threadIdx.x & 3) * 16 + half;
@@ -287,7 +289,7 @@ __device__ __forceinline__ float v_prob(float acc, float xs, float ws, float b2,
 template <int SEGS>
 __device__ __forceinline__ void v_logits(const VocabArgs& a, vt_f4 (&acc)[VT_MI][VT_NI], int v0, int i0) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
-    const int vb = v0 + (wave >> 1) * (VT_A / 2) + 4 * g, ib = i0 + (wave & 1) * (VT_B / 2) + c;
+    const int vb = v0 + (wave / VT_WB) * VT_TA + 4 * g, ib = i0 + (wave % VT_WB) * VT_TB + c;
     float xs[VT_NI];
 #pragma unroll
     for (int j = 0; j < VT_NI; ++j) xs[j] = SEGS == 1 ? 1.f : a.xs[ib + 16 * j];
@@ -300,6 +302,7 @@ __device__ __forceinline__ void v_logits(const VocabArgs& a, vt_f4 (&acc)[VT_MI]
 #pragma unroll
             for (int j = 0; j < VT_NI; ++j) acc[i][j][r] = v_logit<SEGS>(acc[i][j][r], xs[j], ws, b2[r]);
         }
+        if constexpr (SEGS > 1) __builtin_amdgcn_sched_barrier(0);  // (four labels' numbers at a time: registers)
     }
 }
 
@@ -324,10 +327,10 @@ __device__ __forceinline__ void v_join(float& m1, float& s1, int& a1, float m2, 
 // Forward: workgroup (row tile, split of the vocabulary).  A lane keeps (maximum, sum, lowest label of the maximum) of its 4 rows
 // over the labels it sees; they are joined over the lanes, the waves and (vocab_finish_kernel) the splits.
 template <bool BF, int SEGS, bool ARG>
-__global__ __launch_bounds__(256, 2) void vocab_forward_kernel(VocabArgs a) {
+__global__ __launch_bounds__(VT_THREADS, VT_WGS * VT_WAVES / 4) void vocab_forward_kernel(VocabArgs a) {
     extern __shared__ __attribute__((aligned(16))) char vlds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
-    const int i0 = blockIdx.x * VT_B, ib = i0 + (wave & 1) * (VT_B / 2) + c;
+    const int i0 = blockIdx.x * VT_B, ib = i0 + (wave % VT_WB) * VT_TB + c;
     float m[VT_NI], s[VT_NI];
     int arg[VT_NI], lab[VT_NI];
 #pragma unroll
@@ -346,10 +349,10 @@ __global__ __launch_bounds__(256, 2) void vocab_forward_kernel(VocabArgs a) {
             for (int j = 0; j < VT_NI; ++j) acc[i][j] = vt_f4{0.f, 0.f, 0.f, 0.f};
         vt_product<BF, SEGS>(W, X, v0, i0, 0, a.dk / VT_K, vlds, acc);
         v_logits<SEGS>(a, acc, v0, i0);
-        const int vw = v0 + (wave >> 1) * (VT_A / 2), vb = vw + 4 * g;
+        const int vw = v0 + (wave / VT_WB) * VT_TA, vb = vw + 4 * g;
         bool mine = false;  // the label of one of the wave's rows is among these
 #pragma unroll
-        for (int j = 0; j < VT_NI; ++j) mine |= (unsigned)(lab[j] - vw) < (unsigned)(VT_A / 2);
+        for (int j = 0; j < VT_NI; ++j) mine |= (unsigned)(lab[j] - vw) < (unsigned)VT_TA;
         if (!ARG && __any(mine)) {
 #pragma unroll
             for (int j = 0; j < VT_NI; ++j)
@@ -362,17 +365,17 @@ __global__ __launch_bounds__(256, 2) void vocab_forward_kernel(VocabArgs a) {
 #pragma unroll
         for (int j = 0; j < VT_NI; ++j) {
             float top = m[j];
+#pragma unroll
+            for (int i = 0; i < VT_MI; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[i][j][r]);
             if constexpr (ARG) {
+                int at = 0;  // the lowest label of the maximum, counted from vb: a constant each
 #pragma unroll
-                for (int i = 0; i < VT_MI; ++i)
+                for (int i = VT_MI - 1; i >= 0; --i)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (acc[i][j][r] > top) { top = acc[i][j][r]; arg[j] = vb + 16 * i + r; }
-            } else {
-#pragma unroll
-                for (int i = 0; i < VT_MI; ++i)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[i][j][r]);
+                    for (int r = 3; r >= 0; --r) at = acc[i][j][r] == top ? 16 * i + r : at;
+                if (top > m[j]) arg[j] = vb + at;
             }
             float sum = s[j] * v_exp<SEGS>(m[j] - top);
 #pragma unroll
@@ -383,7 +386,7 @@ __global__ __launch_bounds__(256, 2) void vocab_forward_kernel(VocabArgs a) {
             s[j] = sum;
         }
     }
-    // join: lanes g (labels 4 g ..), then the two waves of the same rows
+    // join: lanes g (labels 4 g ..), then the waves of the same rows
     __syncthreads();
     float* sh = reinterpret_cast<float*>(vlds);
 #pragma unroll
@@ -394,19 +397,21 @@ __global__ __launch_bounds__(256, 2) void vocab_forward_kernel(VocabArgs a) {
             const int a2 = __shfl_xor(arg[j], o, 64);
             v_join<SEGS>(m[j], s[j], arg[j], m2, s2, a2);
         }
-        if (wave >= 2 && g == 0) {
-            const int at = (wave & 1) * (VT_B / 2) + 16 * j + c;
+        if (wave >= VT_WB && g == 0) {
+            const int at = (wave / VT_WB * VT_B) + (wave % VT_WB) * VT_TB + 16 * j + c;
             sh[at] = m[j];
-            sh[VT_B + at] = s[j];
-            reinterpret_cast<int*>(sh)[2 * VT_B + at] = arg[j];
+            sh[VT_WA * VT_B + at] = s[j];
+            reinterpret_cast<int*>(sh)[2 * VT_WA * VT_B + at] = arg[j];
         }
     }
     __syncthreads();
-    if (wave < 2 && g == 0) {
+    if (wave < VT_WB && g == 0) {
 #pragma unroll
         for (int j = 0; j < VT_NI; ++j) {
-            const int at = wave * (VT_B / 2) + 16 * j + c;
-            v_join<SEGS>(m[j], s[j], arg[j], sh[at], sh[VT_B + at], reinterpret_cast<int*>(sh)[2 * VT_B + at]);
+            const int at = wave * VT_TB + 16 * j + c;
+#pragma unroll
+            for (int q = VT_B; q < VT_WA * VT_B; q += VT_B)
+                v_join<SEGS>(m[j], s[j], arg[j], sh[q + at], sh[VT_WA * VT_B + q + at], reinterpret_cast<int*>(sh)[2 * VT_WA * VT_B + q + at]);
             if (i0 + at < a.n) {
                 const long o = (long)(i0 + at) * a.splits + blockIdx.y;
                 a.part_ms[o] = make_float2(m[j], s[j]);
@@ -628,7 +633,7 @@ __global__ __launch_bounds__(256) void vocab_prepare_kernel(VocabArgs a) {  // t
 // D of one piece of the vocabulary: the logits again, D [n][piece] in fp16 (two planes of fp32).  A wave's part goes through LDS, so that
 // rows are written 256 bytes at a time (as it lies in the registers it would be 8).
 template <bool BF, int SEGS>
-__global__ __launch_bounds__(256, 2) void vocab_probs_kernel(VocabArgs a, int p0) {
+__global__ __launch_bounds__(VT_THREADS, VT_WGS * VT_WAVES / 4) void vocab_probs_kernel(VocabArgs a, int p0) {
     extern __shared__ __attribute__((aligned(16))) char vlds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
     const int i0 = blockIdx.x * VT_B, v0 = p0 + blockIdx.y * VT_A;
@@ -638,7 +643,7 @@ __global__ __launch_bounds__(256, 2) void vocab_probs_kernel(VocabArgs a, int p0
 #pragma unroll
         for (int j = 0; j < VT_NI; ++j) acc[i][j] = vt_f4{0.f, 0.f, 0.f, 0.f};
     vt_product<BF, SEGS>(v_operand_w(a), v_operand_x(a), v0, i0, 0, a.dk / VT_K, vlds, acc);
-    const int vb = v0 + (wave >> 1) * (VT_A / 2) + 4 * g, ib = i0 + (wave & 1) * (VT_B / 2) + c;
+    const int vb = v0 + (wave / VT_WB) * VT_TA + 4 * g, ib = i0 + (wave % VT_WB) * VT_TB + c;
     int lab[VT_NI];
     float gm[VT_NI], gc[VT_NI], gn[VT_NI], xs[VT_NI];
 #pragma unroll
@@ -666,10 +671,11 @@ __global__ __launch_bounds__(256, 2) void vocab_probs_kernel(VocabArgs a, int p0
                 acc[i][j][r] = (lab[j] == 16 * i + r ? p - 0x1p14f : p) * gn[j];
             }
     }
-    static_assert(4 * (VT_B / 2) * VT_A <= VT_LDS, "a wave's 64 rows of 128 labels");
+    constexpr int RB = VT_TA * 2, RC = RB / 16;  // bytes and chunks of a row of the wave's part
+    static_assert(VT_WAVES * VT_TB * RB <= VT_LDS, "every wave's rows");
     __syncthreads();  // (the products' buffers are read)
-    char* mine = vlds + wave * (VT_B / 2) * VT_A;  // [64 rows][128 labels], 16-byte chunks in the order of vs_place
-    unsigned short* out = a.p + (long)(i0 + (wave & 1) * (VT_B / 2)) * a.piece + (v0 - p0) + (wave >> 1) * (VT_A / 2);
+    char* mine = vlds + wave * VT_TB * RB;  // [VT_TB rows][VT_TA labels], 16-byte chunks in the order of vs_place
+    unsigned short* out = a.p + (long)(i0 + (wave % VT_WB) * VT_TB) * a.ldp + (v0 - p0) + (wave / VT_WB) * VT_TA;
 #pragma unroll
     for (int plane = 0; plane < (SEGS == 1 ? 1 : 2); ++plane) {
 #pragma unroll
@@ -687,28 +693,28 @@ __global__ __launch_bounds__(256, 2) void vocab_probs_kernel(VocabArgs a, int p0
                         acc[i][j][2 * r + 1] = y - (float)__builtin_bit_cast(_Float16, (unsigned short)(h[r] >> 16));
                     }
                 }
-                *reinterpret_cast<uint2*>(mine + (16 * j + c) * VT_A + (vs_place<VT_A>(16 * j + c, 2 * i + (g >> 1)) << 4) + (g & 1) * 8) =
+                *reinterpret_cast<uint2*>(mine + (16 * j + c) * RB + (vs_place<RB>(16 * j + c, 2 * i + (g >> 1)) << 4) + (g & 1) * 8) =
                     make_uint2(h[0], h[1]);
             }
 #pragma unroll(SEGS == 1 ? 16 : 2)
-        for (int it = 0; it < VT_B / 8; ++it) {
-            const int row = it * 4 + g;
-            *reinterpret_cast<vt_u4*>(out + (long)plane * a.nk * a.piece + (long)row * a.piece + c * 8) = vs_read<VT_A>(mine, row, c);
+        for (int it = 0; it < VT_TB * RC / 64; ++it) {
+            const int row = it * (64 / RC) + lane / RC, chunk = lane % RC;
+            *reinterpret_cast<vt_u4*>(out + (long)plane * a.nk * a.ldp + (long)row * a.ldp + chunk * 8) = vs_read<RB>(mine, row, chunk);
         }
     }
 }
 
 // dx += D W over one piece: partial sums [split][n][dk], a split of the piece's labels each
 template <int SEGS>
-__global__ __launch_bounds__(256, 2) void vocab_dx_kernel(VocabArgs a, int p0, int width) {
+__global__ __launch_bounds__(VT_THREADS, VT_WGS * VT_WAVES / 4) void vocab_dx_kernel(VocabArgs a, int p0, int width) {
     extern __shared__ __attribute__((aligned(16))) char vlds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
     const int i0 = blockIdx.x * VT_A, k0 = blockIdx.y * VT_B;
     const int steps = width / VT_K, per = (steps + a.dx_splits - 1) / a.dx_splits, s0 = min((int)blockIdx.z * per, steps), s1 = min(s0 + per, steps);
-    const VocabOperand P{a.p, a.piece, (long)a.nk * a.piece, a.nk, a.piece}, WT{a.wt + p0, a.Vk, (long)a.d * a.Vk, a.d, a.Vk - p0};
+    const VocabOperand P{a.p, a.ldp, (long)a.nk * a.ldp, a.nk, a.piece}, WT{a.wt + p0, a.ldwt, a.d * a.ldwt, a.d, a.Vk - p0};
     vt_f4 acc[VT_MI][VT_NI];
     float* out = a.dxp + (long)blockIdx.z * a.nk * a.dk;
-    const int ib = i0 + (wave >> 1) * (VT_A / 2) + 4 * g, kb = k0 + (wave & 1) * (VT_B / 2) + c;
+    const int ib = i0 + (wave / VT_WB) * VT_TA + 4 * g, kb = k0 + (wave % VT_WB) * VT_TB + c;
 #pragma unroll
     for (int i = 0; i < VT_MI; ++i)
 #pragma unroll
@@ -728,11 +734,11 @@ __global__ __launch_bounds__(256, 2) void vocab_dx_kernel(VocabArgs a, int p0, i
 
 // dW and db of one piece: D is taken as it lies, by columns
 template <int D, int SEGS>
-__global__ __launch_bounds__(256, 2) void vocab_dw_kernel(VocabArgs a, int p0) {
+__global__ __launch_bounds__(VT_THREADS, VT_WGS * VT_WAVES / 4) void vocab_dw_kernel(VocabArgs a, int p0) {
     extern __shared__ __attribute__((aligned(16))) char vlds[];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
     const int v0 = blockIdx.x * VT_A, k0 = blockIdx.y * VT_B;
-    const VocabOperand P{a.p, a.piece, (long)a.nk * a.piece, a.nk, a.piece}, XT{a.xt, a.nk, (long)a.d * a.nk, a.d, a.nk};
+    const VocabOperand P{a.p, a.ldp, (long)a.nk * a.ldp, a.nk, a.piece}, XT{a.xt, a.ldxt, a.d * a.ldxt, a.d, a.nk};
     vt_f4 acc[VT_MI][VT_NI], ones[VT_MI];
 #pragma unroll
     for (int i = 0; i < VT_MI; ++i) {
@@ -740,10 +746,10 @@ __global__ __launch_bounds__(256, 2) void vocab_dw_kernel(VocabArgs a, int p0) {
 #pragma unroll
         for (int j = 0; j < VT_NI; ++j) acc[i][j] = vt_f4{0.f, 0.f, 0.f, 0.f};
     }
-    const bool bias = a.db != nullptr && k0 == 0 && (wave & 1) == 0;
+    const bool bias = a.db != nullptr && k0 == 0 && wave % VT_WB == 0;
     vt_product<false, SEGS, true, true>(P, XT, v0, k0, 0, a.nk / VT_K, vlds, acc, ones, bias);
     const int eg = a.exps[0] + 14, e = eg + a.exps[1];  // (D holds 2^14 p and the scaled g)
-    const int vb = p0 + v0 + (wave >> 1) * (VT_A / 2) + 4 * g, kb = k0 + (wave & 1) * (VT_B / 2) + c;
+    const int vb = p0 + v0 + (wave / VT_WB) * VT_TA + 4 * g, kb = k0 + (wave % VT_WB) * VT_TB + c;
 #pragma unroll
     for (int i = 0; i < VT_MI; ++i)
 #pragma unroll
@@ -770,7 +776,7 @@ __global__ __launch_bounds__(256, vs_waves(D == PIN_F32 ? 2 : 1, KT, MODE)) void
     const VocabOperand X = v_operand_x(a), W = v_operand_w(a);
     const VocabOperand own = OWN_X ? X : W, str = OWN_X ? W : X;
     const unsigned short* trans = OWN_X ? a.wt : a.xt;
-    const long trans_ld = OWN_X ? a.Vk : a.nk, trans_plane = (long)a.d * trans_ld;
+    const long trans_ld = OWN_X ? a.ldwt : a.ldxt, trans_plane = a.d * trans_ld;
 
     // the owners' operand and their numbers
     vt_u4 o[PL][NJ][KT];
@@ -806,11 +812,11 @@ __global__ __launch_bounds__(256, vs_waves(D == PIN_F32 ? 2 : 1, KT, MODE)) void
 
     const int tiles = (OWN_X ? a.Vk : a.nk) / TR, per = (tiles + (int)gridDim.y - 1) / (int)gridDim.y;
     const int t0 = min((int)blockIdx.y * per, tiles), t1 = min(t0 + per, tiles);
-    VtLoader<TR, TROW> lt;
-    VtLoader<S::DK, TTROW> ltt;
+    VtLoader<TR, TROW, false, 4, (KT >= 7)> lt;
+    VtLoader<S::DK, TTROW, false, 4, (KT >= 7)> ltt;
     lt.init(str.ld);
     if constexpr (GRAD) ltt.init(trans_ld);
-    const VocabOperand str_t{trans, trans_ld, trans_plane, a.d, (int)trans_ld};
+    const VocabOperand str_t{trans, trans_ld, trans_plane, a.d, OWN_X ? a.Vk : a.nk};
     auto load = [&](int t) {
         char* at = vlds + (t & 1) * S::BUF;
         const int r0 = t * TR;
@@ -826,8 +832,8 @@ __global__ __launch_bounds__(256, vs_waves(D == PIN_F32 ? 2 : 1, KT, MODE)) void
                                                  (__attribute__((address_space(3))) void*)(at + S::T_BYTES + S::TT_BYTES + k * 256), 4, 0, 0);
 #pragma unroll
         for (int p = 0; p < PL; ++p) {
-            lt.load(str.p + p * str.plane + r0 * str.ld, vt_left(str, r0, 0), str.ld, at + p * TR * TROW);
-            if constexpr (GRAD) ltt.load(trans + p * trans_plane + r0, vt_left(str_t, 0, r0), trans_ld, at + S::T_BYTES + p * S::DK * TTROW);
+            lt.load(vt_span(str.p + p * str.plane + r0 * str.ld, vt_left(str, r0, 0)), 0, str.ld, at + p * TR * TROW);
+            if constexpr (GRAD) ltt.load(vt_span(trans + p * trans_plane + r0, vt_left(str_t, 0, r0)), 0, trans_ld, at + S::T_BYTES + p * S::DK * TTROW);
         }
     };
     if (t0 < t1) load(t0);
@@ -873,6 +879,7 @@ __global__ __launch_bounds__(256, vs_waves(D == PIN_F32 ? 2 : 1, KT, MODE)) void
                         acc[i][j] = vt_mfma<BF>(hi, o[0][j][k], acc[i][j]);
                     }
                 }
+                if constexpr (!GRAD && PL == 1 && KT == 7) __builtin_amdgcn_sched_barrier(0);  // (the second half's reads go no further ahead: registers)
             }
             const int rq = r0 + 32 * q;
             if constexpr (!GRAD) {
@@ -900,11 +907,13 @@ __global__ __launch_bounds__(256, vs_waves(D == PIN_F32 ? 2 : 1, KT, MODE)) void
                 for (int j = 0; j < NJ; ++j) {
                     float top = m[j];
                     if constexpr (MODE == VS_ARGMAX) {
+                        int at = -1;  // counted from the lane's first label: a constant each
 #pragma unroll
                         for (int i = 0; i < 2; ++i)
 #pragma unroll
                             for (int r = 0; r < 4; ++r)
-                                if (acc[i][j][r] > top) { top = acc[i][j][r]; arg[j] = rq + 16 * i + 4 * g + r; }
+                                if (acc[i][j][r] > top) { top = acc[i][j][r]; at = 16 * i + r; }
+                        if (at >= 0) arg[j] = rq + 4 * g + at;
                     } else {
 #pragma unroll
                         for (int i = 0; i < 2; ++i)
@@ -1101,7 +1110,6 @@ enum { V_PREDICT = 0, V_NLL = 1, V_GRAD = 2, V_STEP = 3 };
 constexpr int V_STREAM_DIM = 256;  // features of the streaming kernels at most
 // Rows that vocab_few_kernel takes at most: its matrix instructions keep up with the reads of W to 64 rows (fp32: 32)
 inline int v_few_rows(int dtype) { return dtype == PIN_F32 ? 32 : 64; }
-constexpr int V_FILL = 512;        // workgroups a launch is split for: two a compute unit
 
 struct VocabPlan {
     VocabArgs a;
@@ -1135,7 +1143,7 @@ inline VocabPlan v_plan(const pin_vocab_head* h, int mode, char* base) {
     a.n = h->n; a.V = h->vocab; a.d = h->dim;
     a.x = h->x; a.w = h->weight; a.bias = h->bias; a.ldx = h->x_stride; a.ldw = h->weight_stride;
     p.kt = a.d <= V_STREAM_DIM ? (a.d + 31) / 32 : 0;
-    a.dk = p.kt > 0 ? 32 * p.kt : (int)v_up(a.d, VT_K); a.nk = (int)v_up(a.n > 0 ? a.n : 1, VT_B); a.Vk = (int)v_up(a.V, p.kt > 0 ? 128 : VT_A);
+    a.dk = p.kt > 0 ? 32 * p.kt : (int)v_up(a.d, 64); a.nk = (int)v_up(a.n > 0 ? a.n : 1, 128); a.Vk = (int)v_up(a.V, p.kt > 0 || VT_A < 128 ? 128 : VT_A);
     p.dtype = h->dtype;
     a.order = p.kt > 0;
     const bool two = h->dtype == PIN_F32, grads = mode == V_GRAD || mode == V_STEP;
@@ -1152,18 +1160,16 @@ inline VocabPlan v_plan(const pin_vocab_head* h, int mode, char* base) {
         a.dx_splits = v_splits((a.nk + grad - 1) / grad, a.Vk / tr, 128 / tr, 256 * vs_waves(planes, p.kt, VS_DX), v_part_cost(a.V));
         a.dw_splits = v_splits((a.Vk + grad - 1) / grad, a.nk / tr, 128 / tr, 256 * vs_waves(planes, p.kt, VS_DW), v_part_cost(a.n));
     } else {
-        a.splits = v_splits(rows, tiles, 1, V_FILL, 0.001f);
+        a.splits = v_splits(rows, tiles, 1, 256 * VT_WGS, 0.001f);
         a.tiles_per_split = (tiles + a.splits - 1) / a.splits;
         a.splits = (tiles + a.tiles_per_split - 1) / a.tiles_per_split;
         const int features = (a.d + VT_B - 1) / VT_B;
-        // pieces whose D takes half a gigabyte at most and whose dW fills the card, if it can be had
+        // pieces whose D takes half a gigabyte at most (the sums of dx are read and written once a piece)
         long piece = (512l << 20) / (2l * planes * a.nk) / VT_A * VT_A;
-        const long want = v_up((V_FILL + features - 1) / features, 1) * VT_A;
-        if (piece > want) piece = want;
         if (piece < VT_A) piece = VT_A;
         if (piece > a.Vk) piece = a.Vk;
         a.piece = (int)piece;
-        a.dx_splits = v_splits((a.nk + VT_A - 1) / VT_A * features, (int)(piece / VT_K), 8, V_FILL, v_part_cost((int)piece));
+        a.dx_splits = v_splits((a.nk + VT_A - 1) / VT_A * features, (int)(piece / VT_K), 8, 256 * VT_WGS, v_part_cost((int)piece));
         a.dw_splits = 0;
     }
     if (p.few) a.splits = (a.V + 64 * p.few - 1) / (64 * p.few);
@@ -1188,8 +1194,9 @@ inline VocabPlan v_plan(const pin_vocab_head* h, int mode, char* base) {
         else a.tlogit = (float*)take((long)a.nk * 4);
     }
     if (grads) {
-        a.xt = (unsigned short*)take((long)planes * a.d * a.nk * 2);
-        a.wt = (unsigned short*)take((long)planes * a.d * a.Vk * 2);
+        a.ldxt = a.nk + 64; a.ldwt = a.Vk + 64; a.ldp = a.piece + 64;
+        a.xt = (unsigned short*)take(planes * a.d * a.ldxt * 2);
+        a.wt = (unsigned short*)take(planes * a.d * a.ldwt * 2);
         a.gm = rows_of(a.nk); a.gc = rows_of(a.nk); a.gn = rows_of(a.nk); a.g = rows_of(a.nk);
         a.part = (int*)rows_of(a.nk);
         a.bad = (int*)rows_of(a.nk);
@@ -1199,7 +1206,7 @@ inline VocabPlan v_plan(const pin_vocab_head* h, int mode, char* base) {
             a.dwp = (float*)take((long)a.dw_splits * a.Vk * a.dk * 4);
             a.dbp = (float*)take((long)a.dw_splits * a.Vk * 4);
         } else {
-            a.p = (unsigned short*)take((long)planes * a.nk * a.piece * 2);
+            a.p = (unsigned short*)take((long)planes * a.nk * a.ldp * 2);
             }
     }
     p.bytes = at;
@@ -1228,6 +1235,7 @@ static int v_reserve(F* kernel, int bytes) {
         if (reserved != 0) return reserved;                   \
     } while (0)
 #define V_LAUNCH(kernel, grid, lds, ...) hipLaunchKernelGGL(kernel, grid, dim3(256), lds, s, __VA_ARGS__)
+#define V_TILES(kernel, grid, ...) hipLaunchKernelGGL(kernel, grid, dim3(VT_THREADS), VT_LDS, s, __VA_ARGS__)
 
 template <int D, int KT, int MODE>
 static int v_stream(const VocabPlan& p, hipStream_t s) {
@@ -1318,8 +1326,8 @@ int v_run_typed(const VocabPlan& p, int mode, hipStream_t s) {
             V_RESERVE((&vocab_forward_kernel<BF, SEGS, true>), VT_LDS);
             V_RESERVE((&vocab_forward_kernel<BF, SEGS, false>), VT_LDS);
             const dim3 grid(a.nk / VT_B, a.splits);
-            if (mode == V_PREDICT) V_LAUNCH((vocab_forward_kernel<BF, SEGS, true>), grid, VT_LDS, a);
-            else V_LAUNCH((vocab_forward_kernel<BF, SEGS, false>), grid, VT_LDS, a);
+            if (mode == V_PREDICT) V_TILES((vocab_forward_kernel<BF, SEGS, true>), grid, a);
+            else V_TILES((vocab_forward_kernel<BF, SEGS, false>), grid, a);
         }
         v_finish<D>(a, mode, mode == V_STEP ? a.nk + 64 : a.n, s);
     } else {
@@ -1337,9 +1345,9 @@ int v_run_typed(const VocabPlan& p, int mode, hipStream_t s) {
         V_RESERVE((&vocab_dw_kernel<D, SEGS>), VT_LDS);
         for (int p0 = 0; p0 < a.Vk; p0 += a.piece) {
             const int width = p0 + a.piece < a.Vk ? a.piece : a.Vk - p0;
-            V_LAUNCH((vocab_probs_kernel<BF, SEGS>), dim3(a.nk / VT_B, width / VT_A), VT_LDS, a, p0);
-            V_LAUNCH((vocab_dx_kernel<SEGS>), dim3(cdiv(a.nk, VT_A), kt, a.dx_splits), VT_LDS, a, p0, width);
-            V_LAUNCH((vocab_dw_kernel<D, SEGS>), dim3(width / VT_A, kt), VT_LDS, a, p0);
+            V_TILES((vocab_probs_kernel<BF, SEGS>), dim3(a.nk / VT_B, width / VT_A), a, p0);
+            V_TILES((vocab_dx_kernel<SEGS>), dim3(cdiv(a.nk, VT_A), kt, a.dx_splits), a, p0, width);
+            V_TILES((vocab_dw_kernel<D, SEGS>), dim3(width / VT_A, kt), a, p0);
         }
     }
     const int most = a.dx_splits > a.dw_splits ? a.dx_splits : a.dw_splits;

@@ -40,7 +40,7 @@ __host__ __device__ constexpr int vs_nj(int PL, int KT, bool grad) {
 
 // waves a SIMD that their registers leave room for (512 a lane): what hides the way from product to exponential to product in each of them
 __host__ __device__ constexpr int vs_waves(int PL, int KT, int mode) {
-    if (mode < VS_DX) return PL * KT <= 2 ? 4 : PL == 1 && KT == 3 ? 3 : 2;
+    if (mode < VS_DX) return PL == 1 && KT <= 2 ? 4 : PL == 1 ? (KT == 3 ? 3 : 2) : KT == 1 ? 3 : 2;
     if (PL == 1) return KT == 1 ? 3 : KT == 8 ? 1 : 2;
     return KT == 1 && mode == VS_DX ? 3 : 2;
 }

@@ -10,8 +10,9 @@
 // fit a compute unit, so that the epilogue of one (exponentials, stores) runs beside the products of the other.
 //
 // LDS: the loads write it directly, so the order within a row is in the addresses they read from: chunk c (16 bytes) of row r is kept at
-// vs_place(r, c), such that the 16 lanes that read one chunk of 16 rows touch every bank once.  Rows behind an operand's end read
-// as zeros (the buffer's own bound).
+// vs_place(r, c).  A 16-byte read serves 16 lanes a cycle, not 16 neighbours but lanes 0-3, 12-15, 20-23, 24-27 (4-7, 8-11, 16-19,
+// 28-31; the same in the upper half): the places are such that these touch every bank once (SQ_LDS_BANK_CONFLICT 0; with places that suit 16
+// neighbours half of the LDS cycles of 64-byte rows were conflicts).  Rows behind an operand's end read as zeros (the buffer's own bound).
 #pragma once
 #include "pin_common.h"
 
@@ -23,8 +24,10 @@ typedef float vt_f4 __attribute__((ext_vector_type(4)));
 typedef unsigned int vt_u4 __attribute__((ext_vector_type(4)));
 
 constexpr int VT_A = 256, VT_B = 128;      // rows of A and of B a workgroup
+constexpr int VT_WA = 2, VT_WB = 2;        // waves along A and along B
 constexpr int VT_K = 32, VT_STEPS = 3;     // k of one step, buffers
-constexpr int VT_MI = VT_A / 32, VT_NI = VT_B / 32;  // 16 x 16 tiles of a wave
+constexpr int VT_WAVES = VT_WA * VT_WB, VT_THREADS = 64 * VT_WAVES, VT_WGS = VT_WAVES == 4 ? 2 : 1;  // workgroups a compute unit
+constexpr int VT_TA = VT_A / VT_WA, VT_TB = VT_B / VT_WB, VT_MI = VT_TA / 16, VT_NI = VT_TB / 16;    // of a wave, in rows and in 16 x 16 tiles
 constexpr int VT_A_BYTES = VT_A * VT_K * 2, VT_BUF = VT_A_BYTES + VT_B * VT_K * 2, VT_LDS = VT_STEPS * VT_BUF;
 
 struct VocabOperand {
@@ -46,38 +49,48 @@ __device__ __forceinline__ int vs_place(int r, int c) {
     if constexpr (TRANS) return c ^ ((((r & 3) | ((r >> 1) & 4)) << 1));  // (16 rows at once, 32 bytes of each)
     else if constexpr (ROW_BYTES % 256 == 0) return c ^ (r & 15);
     else if constexpr (ROW_BYTES % 128 == 0) return c ^ ((r >> 1) & 7);
-    else return c ^ ((r >> 2) & 3);
+    else return c ^ ((((r >> 2) ^ (r >> 3)) & 1) << 1 | ((r >> 3) & 1));
 }
 
-// ROWS rows of ROW_BYTES each, global memory -> LDS, by the workgroup's four waves.  What a lane reads is its offset from the tile's first
-// byte, the same in every step: the step is in the (scalar) base.
-template <int ROWS, int ROW_BYTES, bool TRANS = false>
+// The part of a plane that a workgroup reads: what its loads count from, and where they end (reads behind it give zeros).
+struct VtSpan {
+    const unsigned short* first;
+    unsigned bytes;
+};
+__device__ __forceinline__ VtSpan vt_span(const unsigned short* first, long bytes) {
+    return VtSpan{first, bytes <= 0 ? 0u : bytes > 0xFFFFFFFFl ? 0xFFFFFFFFu : (unsigned)bytes};
+}
+
+// ROWS rows of ROW_BYTES each, global memory -> LDS, by the workgroup's WAVES waves.  What a lane reads is its offset from the tile's first
+// byte, the same in every step: the step is a scalar.  (A buffer's bound is compared with the lane's offset alone or with all of
+// it; rows behind the end are behind it either way.)
+template <int ROWS, int ROW_BYTES, bool TRANS = false, int WAVES = 4, bool SAVE = false>
 struct VtLoader {
-    static constexpr int CH = ROW_BYTES / 16, ALL = ROWS * CH / 64, PER = (ALL + 3) / 4;
+    static constexpr int CH = ROW_BYTES / 16, ALL = ROWS * CH / 64, PER = (ALL + WAVES - 1) / WAVES, ROUND = 64 * WAVES;
     static_assert(ROWS * CH % 64 == 0, "whole instructions");
-    // a round of the four waves takes whole rows, and as many as the places repeat after: the rounds differ by a scalar alone
-    static constexpr bool EVEN = 256 % CH == 0 && (256 / CH) % 16 == 0;
+    // SAVE, where a round of the waves takes whole rows, and as many as the places repeat after: the rounds differ by a scalar alone, one register
+    // instead of one each
+    static constexpr bool EVEN = SAVE && ROUND % CH == 0 && (ROUND / CH) % 16 == 0;
     unsigned off[EVEN ? 1 : PER];
-    __device__ __forceinline__ void init(long ld) {  // elements from row to row; 256 rows of 2^22 elements still fit 32 bits
+    __device__ __forceinline__ void init(long ld) {  // elements from row to row; 256 rows of 2^22 elements fit 32 bits
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
         for (int i = 0; i < (EVEN ? 1 : PER); ++i) {
-            const int slot = (i * 4 + wave) * 64 + lane, r = slot / CH;
+            const int slot = i * ROUND + wave * 64 + lane, r = slot / CH;
             off[i] = (unsigned)r * (unsigned)(ld * 2) + vs_place<ROW_BYTES, TRANS>(r, slot % CH) * 16;
         }
     }
-    // first: the tile's first element (of a plane); left: bytes from there to the end of what may be read; ld: as for init
-    __device__ __forceinline__ void load(const unsigned short* first, long left, long ld, char* lds) const {
+    __device__ __forceinline__ void load(const VtSpan& s, unsigned step, long ld, char* lds) const {  // step: bytes from the span's first
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            if (ALL % 4 != 0 && i == PER - 1 && wave >= ALL % 4) continue;  // (a last round that some waves have no part in)
+            if (ALL % WAVES != 0 && i == PER - 1 && wave >= ALL % WAVES) continue;  // (a last round that some waves have no part in)
 #if defined(__HIP_DEVICE_COMPILE__)  // (the host pass has no buffer resources)
-            const long rows = EVEN ? (long)i * (256 / CH) * ld : 0, rest = left - 2 * rows;
-            const unsigned bytes = rest <= 0 ? 0u : rest > 0xFFFFFFFFl ? 0xFFFFFFFFu : (unsigned)rest;
-            const auto buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned short*>(first + rows), 0, (int)bytes, 0x00027000);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (__attribute__((address_space(3))) void*)(lds + (i * 4 + wave) * 1024), 16,
-                                                     off[EVEN ? 0 : i], 0, 0, 0);
+            const long rows = EVEN ? (long)i * (ROUND / CH) * ld : 0;
+            const VtSpan q = EVEN ? vt_span(s.first + rows, (long)s.bytes - 2 * rows) : s;
+            const auto buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned short*>(q.first), 0, (int)q.bytes, 0x00027000);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (__attribute__((address_space(3))) void*)(lds + (i * WAVES + wave) * 1024), 16,
+                                                     off[EVEN ? 0 : i], step, 0, 0);
 #endif
         }
     }
@@ -89,10 +102,10 @@ __device__ __forceinline__ vt_u4 vs_read(const char* lds, int r, int c) {
 // bytes from element (row, col) of a plane to its end
 __device__ __forceinline__ long vt_left(const VocabOperand& o, long row, long col) { return ((o.rows - 1 - row) * o.ld + o.cols - col) * 2; }
 
-// operand over k of 16 columns from `col` on of a tile [32 k][VT_A]: the lane's k = 8 g ..
-__device__ __forceinline__ vt_u4 vt_read_trans(const char* lds, int col) {
+// operand over 32 k from row k0 on, of 16 columns from `col` on, of a tile [VT_K][VT_A]: the lane's k = k0 + 8 g ..
+__device__ __forceinline__ vt_u4 vt_read_trans(const char* lds, int k0, int col) {
     typedef short s4 __attribute__((ext_vector_type(4)));
-    const int lane = threadIdx.x & 63, g = lane >> 4, row = 8 * g + ((lane >> 2) & 3);
+    const int lane = threadIdx.x & 63, g = lane >> 4, row = k0 + 8 * g + ((lane >> 2) & 3);
     const int at = row * (VT_A * 2) + (vs_place<VT_A * 2, true>(row, col / 8 + ((lane >> 1) & 1)) << 4) + (lane & 1) * 8;
     typedef __attribute__((address_space(3))) s4* ptr;
     const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ptr)(lds + at));
@@ -101,60 +114,71 @@ __device__ __forceinline__ vt_u4 vt_read_trans(const char* lds, int col) {
     return __builtin_bit_cast(vt_u4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-// acc[i][j]: 16 x 16 tiles of the wave's 128 x 64; lane (n = lane & 15, g = lane >> 4), register r holds row 16 i + 4 g + r of A's and row
-// 16 j + n of B's part.  ONES (and `sum`, of a whole wave): also sum_k A[a][k] in `ones`, a product with ones.
+// acc[i][j]: 16 x 16 tiles of the wave's VT_TA x VT_TB; lane (n = lane & 15, g = lane >> 4), register r holds row 16 i + 4 g + r of A's and
+// row 16 j + n of B's part.  ONES (and `sum`, of a whole wave): also sum_k A[a][k] in `ones`, a product with ones.
 template <bool BF, int SEGS, bool TRANS, bool ONES>
 __device__ __forceinline__ void vt_product(const VocabOperand& A, const VocabOperand& B, int a0, int b0, long k0, int steps, char* lds,
                                            vt_f4 (&acc)[VT_MI][VT_NI], vt_f4 (&ones)[ONES ? VT_MI : 1], bool sum) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wa = (wave >> 1) * (VT_A / 2), wb = (wave & 1) * (VT_B / 2);
-    VtLoader<TRANS ? VT_K : VT_A, TRANS ? VT_A * 2 : VT_K * 2, TRANS> la;
-    VtLoader<VT_B, VT_K * 2> lb;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wa = (wave / VT_WB) * VT_TA, wb = (wave % VT_WB) * VT_TB;
+    VtLoader<TRANS ? VT_K : VT_A, TRANS ? VT_A * 2 : VT_K * 2, TRANS, VT_WAVES> la;
+    VtLoader<VT_B, VT_K * 2, false, VT_WAVES> lb;
     la.init(A.ld);
     lb.init(B.ld);
     constexpr int LOADS = decltype(la)::PER + decltype(lb)::PER;
-    static_assert(LOADS == 6, "the wait below counts a step's loads");
+    static_assert(LOADS == 6 || VT_STEPS == 2, "the wait below counts a step's loads");
     const int all = SEGS * steps;
+    VtSpan sa[2], sb[2];  // of the planes
+#pragma unroll
+    for (int p = 0; p < (SEGS > 1 ? 2 : 1); ++p) {
+        if constexpr (TRANS) sa[p] = vt_span(A.p + p * A.plane + k0 * A.ld + a0, vt_left(A, k0, a0));
+        else sa[p] = vt_span(A.p + p * A.plane + a0 * A.ld + k0, vt_left(A, a0, k0));
+        sb[p] = vt_span(B.p + p * B.plane + b0 * B.ld + k0, vt_left(B, b0, k0));
+    }
+    const unsigned step_a = TRANS ? (unsigned)(A.ld * (VT_K * 2)) : VT_K * 2;
     int seg = 0, at = 0, put = 0;  // of the next step to load: its product and place in it, and the buffer it goes to
     auto load = [&]() {
-        const long k = k0 + (long)at * VT_K;
-        const int pa = SEGS > 1 && seg == 0 ? 1 : 0, pb = SEGS > 1 && seg == 1 ? 1 : 0;
         char* to = lds + put * VT_BUF;
-        if constexpr (TRANS) la.load(A.p + pa * A.plane + k * A.ld + a0, vt_left(A, k, a0), A.ld, to);
-        else la.load(A.p + pa * A.plane + a0 * A.ld + k, vt_left(A, a0, k), A.ld, to);
-        lb.load(B.p + pb * B.plane + b0 * B.ld + k, vt_left(B, b0, k), B.ld, to + VT_A_BYTES);
+        la.load(SEGS > 1 && seg == 0 ? sa[1] : sa[0], at * step_a, A.ld, to);
+        lb.load(SEGS > 1 && seg == 1 ? sb[1] : sb[0], at * (VT_K * 2), B.ld, to + VT_A_BYTES);
         if (++at == steps) { at = 0; ++seg; }
         put = put == VT_STEPS - 1 ? 0 : put + 1;
     };
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();  // the last reads of what LDS held before are done
     if (all > 0) load();
-    if (all > 1) load();
+    if (VT_STEPS > 2 && all > 1) load();
     int get = 0;
     for (int t = 0; t < all; ++t) {
         // this step has arrived (the one behind it may be on its way), and every wave is done with the buffer that the next one goes to
-        if (t + 1 < all) asm volatile("s_waitcnt vmcnt(6) lgkmcnt(0)" ::: "memory");
+        if (VT_STEPS > 2 && t + 1 < all) asm volatile("s_waitcnt vmcnt(6) lgkmcnt(0)" ::: "memory");
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
-        if (t + 2 < all) load();
+        if (t + VT_STEPS - 1 < all) load();
         const char* ta = lds + get * VT_BUF;
         const char* tb = ta + VT_A_BYTES;
         get = get == VT_STEPS - 1 ? 0 : get + 1;
-        vt_u4 a[VT_MI], b[VT_NI];
 #pragma unroll
-        for (int j = 0; j < VT_NI; ++j) b[j] = vs_read<VT_K * 2>(tb, wb + 16 * j + (lane & 15), lane >> 4);
+        for (int kk = 0; kk < VT_K / 32; ++kk) {
+            vt_u4 a[VT_MI], b[VT_NI];
 #pragma unroll
-        for (int i = 0; i < VT_MI; ++i) {
-            if constexpr (TRANS) a[i] = vt_read_trans(ta, wa + 16 * i);
-            else a[i] = vs_read<VT_K * 2>(ta, wa + 16 * i + (lane & 15), lane >> 4);
-        }
+            for (int j = 0; j < VT_NI; ++j) b[j] = vs_read<VT_K * 2>(tb, wb + 16 * j + (lane & 15), 4 * kk + (lane >> 4));
 #pragma unroll
-        for (int i = 0; i < VT_MI; ++i)
+            for (int i = 0; i < VT_MI; ++i) {
+                if constexpr (TRANS) a[i] = vt_read_trans(ta, 32 * kk, wa + 16 * i);
+                else a[i] = vs_read<VT_K * 2>(ta, wa + 16 * i + (lane & 15), 4 * kk + (lane >> 4));
+            }
+            // the wave that has its operands goes first, the other one of its SIMD loads meanwhile (2425 -> 2385 us at 8192 x 32768 x 1024)
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-            for (int j = 0; j < VT_NI; ++j) acc[i][j] = vt_mfma<BF>(a[i], b[j], acc[i][j]);
-        if (ONES && sum && (SEGS == 1 || t < steps || t >= 2 * steps)) {  // (of two pieces each once: the first product has l, the last h)
-            const vt_u4 one = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
+            for (int i = 0; i < VT_MI; ++i)
 #pragma unroll
-            for (int i = 0; i < (ONES ? VT_MI : 1); ++i) ones[i] = vt_mfma<BF>(a[i], one, ones[i]);
+                for (int j = 0; j < VT_NI; ++j) acc[i][j] = vt_mfma<BF>(a[i], b[j], acc[i][j]);
+            __builtin_amdgcn_s_setprio(0);
+            if (ONES && sum && (SEGS == 1 || t < steps || t >= 2 * steps)) {  // (of two pieces each once: the first product has l, the last h)
+                const vt_u4 one = {0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u};
+#pragma unroll
+                for (int i = 0; i < (ONES ? VT_MI : 1); ++i) ones[i] = vt_mfma<BF>(a[i], one, ones[i]);
+            }
         }
     }
 }
