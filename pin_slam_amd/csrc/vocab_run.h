@@ -46,6 +46,8 @@ struct VocabArgs {
     float* tlogit;
     float *gm, *gc, *gn, *g; // of a row: reference of the exponent, its offset, the upstream gradient scaled below 1 and as it is
     int* part;               // its label, -1 where it takes no part in the gradient
+    float* rest;             // fp16: what the rounding of D at the row's label left out (dx adds it times W's row: it is the largest part of a
+                             // row's D, and outputs of fp16's own step would show it; 6.1e-4 of a step's dx at 3 x 13203 x 16 without)
     int* bad;                // 1: no label and not finite (its copy in xa is zero)
     float *dxp, *dwp, *dbp;  // partial sums [splits][nk][dk], [splits][Vk][dk], [splits][Vk]
     int splits, tiles_per_split, dx_splits, dw_splits, piece;
@@ -538,6 +540,7 @@ template <int SEGS>
 __device__ __forceinline__ void v_row_of_gradient(const VocabArgs& a, int i, int label, float m, float log2_total, int eg) {
     const bool none = i >= a.n || label < 0 || label >= a.V || log2_total == -INFINITY || a.bad[min(i, a.n - 1)] != 0;
     a.part[i] = none ? -1 : label;
+    a.rest[i] = 0.f;
     a.gm[i] = none || SEGS == 1 ? 0.f : m;
     a.gc[i] = none ? -INFINITY : 14.f - (SEGS == 1 ? m + log2_total : log2_total);
     const float g = none ? 0.f : isnan(log2_total) ? NAN : a.grad_nll[i];
@@ -670,6 +673,24 @@ __global__ __launch_bounds__(VT_THREADS, VT_WGS * VT_WAVES / 4) void vocab_probs
                 const float p = v_prob<SEGS>(acc[i][j][r], xs[j], ws[r], b2[r], gm[j], gc[j]);
                 acc[i][j][r] = (lab[j] == 16 * i + r ? p - 0x1p14f : p) * gn[j];
             }
+    }
+    if constexpr (!BF && SEGS == 1) {
+        bool mine = false;  // the label of one of the wave's rows is among these
+#pragma unroll
+        for (int j = 0; j < VT_NI; ++j) mine |= (unsigned)(lab[j] + 4 * g) < (unsigned)VT_TA;
+        if (__any(mine)) {
+#pragma unroll
+            for (int j = 0; j < VT_NI; ++j)
+#pragma unroll
+                for (int i = 0; i < VT_MI; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float y = acc[i][j][r];
+                        const float rest = v_rest(y);
+                        acc[i][j][r] = y;
+                        if (lab[j] == 16 * i + r) a.rest[ib + 16 * j] = rest;
+                    }
+        }
     }
     constexpr int RB = VT_TA * 2, RC = RB / 16;  // bytes and chunks of a row of the wave's part
     static_assert(VT_WAVES * VT_TB * RB <= VT_LDS, "every wave's rows");
@@ -954,7 +975,16 @@ __global__ __launch_bounds__(256, vs_waves(D == PIN_F32 ? 2 : 1, KT, MODE)) void
                             for (int j = 0; j < NJ; ++j) {
                                 const int l = own_l[j] - rq - 16 * i - 4 * g;
 #pragma unroll
-                                for (int r = 0; r < 4; ++r) acc[i][j][r] -= l == r ? 0x1p14f : 0.f;
+                                for (int r = 0; r < 4; ++r) {
+                                    acc[i][j][r] -= l == r ? 0x1p14f : 0.f;
+                                    if constexpr (D == PIN_F16) {
+                                        const int row = o0 + 16 * j + c;
+                                        float y = acc[i][j][r];
+                                        const float rest = v_rest(y);
+                                        acc[i][j][r] = y;
+                                        if (l == r && row < a.n) a.rest[row] = rest;
+                                    }
+                                }
                             }
                         }
                     } else {
@@ -1082,7 +1112,18 @@ __global__ __launch_bounds__(256) void vocab_join_kernel(VocabArgs a, int x_bloc
     void* out = kind == 0 ? a.dx : a.dw;
     const long to = (long)row * a.d + k;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) s[i] = ldexpf(s[i], -e) * g;
+    for (int i = 0; i < 4; ++i) s[i] = ldexpf(s[i], -e);
+    if constexpr (D == PIN_F16) {
+        const float rest = kind == 0 ? a.rest[row] : 0.f;
+        if (rest != 0.f) {
+            const void* w = v_row<D>(a.w, a.part[row], a.ldw);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (k + i < a.d) s[i] = fmaf(ldexpf(rest, ew - e), v_get<D>(w, k + i), s[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] *= g;
     if (k + 4 <= a.d && (a.d & 3) == 0 && ((uintptr_t)out & 15) == 0) {
         if constexpr (D == PIN_F32) *reinterpret_cast<vt_f4*>(reinterpret_cast<float*>(out) + to) = s;
         else if constexpr (D == PIN_F16) *reinterpret_cast<uint2*>(reinterpret_cast<unsigned short*>(out) + to) = make_uint2(v_pack(s[0], s[1]), v_pack(s[2], s[3]));
@@ -1199,6 +1240,7 @@ inline VocabPlan v_plan(const pin_vocab_head* h, int mode, char* base) {
         a.wt = (unsigned short*)take(planes * a.d * a.ldwt * 2);
         a.gm = rows_of(a.nk); a.gc = rows_of(a.nk); a.gn = rows_of(a.nk); a.g = rows_of(a.nk);
         a.part = (int*)rows_of(a.nk);
+        a.rest = rows_of(a.nk);
         a.bad = (int*)rows_of(a.nk);
         a.exps = (int*)take(256);
         a.dxp = (float*)take((long)a.dx_splits * a.nk * a.dk * 4);

@@ -45,6 +45,12 @@ __host__ __device__ constexpr int vs_waves(int PL, int KT, int mode) {
     return KT == 1 && mode == VS_DX ? 3 : 2;
 }
 
+// what the rounding of x to fp16 leaves of it (x is pinned, and with it the bits that the product takes: see v_split)
+__device__ __forceinline__ float v_rest(float& x) {
+    asm volatile("" : "+v"(x));
+    return x - (float)(_Float16)x;
+}
+
 // two fp32 -> two fp16, the first in the low half
 __device__ __forceinline__ unsigned v_pack(float x, float y) {
     typedef _Float16 h2 __attribute__((ext_vector_type(2)));

@@ -433,3 +433,28 @@ def test_training_a_head_runs_as_its_user_would():
     assert eager[4].steps == cap[4].steps == 5 - 1
     label, logprob = ops.vocab_predict(cap[0], cap[1], cap[2])
     assert ((label >= 0) & (label < 1203)).all() and (logprob <= 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(3, 13203, 16), (70, 5001, 64), (130, 900, 200), (5, 4100, 250), (67, 3001, 257), (200, 999, 520)])
+def test_float16_dx_is_rounded_once_at_the_label(shape):
+    """dx_i = g (sum_v p_v W_v - W_label): the label's factor p - 1 is kept in more than fp16, so that what is left is the rounding of the
+    result (2^-11), of the other labels' factors (2^-11 of each one's part) and the probabilities' own error: a logit of d products
+    and a bias in fp32 (2^-24 (d + 3) of the sum of their magnitudes, twice: of the maximum's too), and some steps of the exponential and the factors (2^-19)."""
+    n, vocab, dim = shape
+    x, w, b, labels, _ = _inputs(n, vocab, dim, torch.float16, 5, scale=1.0)
+    labels = torch.arange(n, device=x.device, dtype=torch.int32) * 7 % vocab
+    x = (x.float() + 3.0 * w[labels.long()].float()).to(torch.float16)
+    g = torch.rand(n, device=x.device) + 0.5
+    dx = ops.vocab_nll_step(x, w, b, labels, g)[2].double()
+    X, W, B = x.double(), w.double(), b.double()
+    s = X @ W.t() + B
+    p = torch.softmax(s, 1)
+    hot = torch.zeros_like(p)
+    hot[torch.arange(n, device=x.device), labels.long()] = 1.0
+    G = g.double()[:, None]
+    want = ((p - hot) @ W) * G
+    rel = (X.abs() @ W.t().abs() + B.abs()).amax(1, keepdim=True) * (2.0 ** -24 * (dim + 3) * 2) + 2.0 ** -19
+    bound = want.abs() * 2.0 ** -11 + 2.0 ** -25 + ((p * (1 - hot)) @ W.abs()) * (G * (2.0 ** -11 + rel)) + ((p * hot) @ W.abs()) * G * rel
+    bound = bound + ((p - hot).abs() @ W.abs()) * G * (F32 * (vocab / 32 + 40)) + W.abs().sum(0) * G.max() * 2.0 ** -39  # sums; tiny factors
+    assert ((dx - want).abs() <= bound).all(), float(((dx - want).abs() / bound).max())
