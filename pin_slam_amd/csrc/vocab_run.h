@@ -284,7 +284,7 @@ __device__ __forceinline__ float v_exp(float diff) {
 template <int SEGS>
 __device__ __forceinline__ float v_prob(float acc, float xs, float ws, float b2, float m, float c) {
     if constexpr (SEGS == 1) return __builtin_amdgcn_exp2f(fmaf(acc, V_LOG2E, b2 + c));
-    else return __builtin_amdgcn_exp2f(fmaf(fmaf(acc, xs * ws, b2) - m, V_LOG2E, c));
+    else return __builtin_amdgcn_exp2f((fmaf(acc, xs * ws, b2) - m) * V_LOG2E) * c;
 }
 
 // the wave's 128 labels x 64 rows of logits from their products
@@ -534,15 +534,15 @@ __global__ __launch_bounds__(256) void vocab_few_kernel(VocabArgs a) {
     }
 }
 
-// what the gradient pass reads of a row: 2^14 p = exp2(s + gc) (log 2 units; gc = 14 - log2 sum exp2 s), or exp2((s - gm) / log 2 + gc)
-// with gm the maximum and gc = 14 - log2 of the sum over it
+// what the gradient pass reads of a row: 2^14 p = exp2(s + gc) (log 2 units; gc = 14 - log2 sum exp2 s), or of fp32 exp2((s - gm) / log 2) gc
+// with gm the maximum and gc = 2^14 / the sum over it (as a part of the exponent its rounding, 2^-21 there, would be the largest error of p)
 template <int SEGS>
-__device__ __forceinline__ void v_row_of_gradient(const VocabArgs& a, int i, int label, float m, float log2_total, int eg) {
+__device__ __forceinline__ void v_row_of_gradient(const VocabArgs& a, int i, int label, float m, float total, float log2_total, int eg) {
     const bool none = i >= a.n || label < 0 || label >= a.V || log2_total == -INFINITY || a.bad[min(i, a.n - 1)] != 0;
     a.part[i] = none ? -1 : label;
     a.rest[i] = 0.f;
-    a.gm[i] = none || SEGS == 1 ? 0.f : m;
-    a.gc[i] = none ? -INFINITY : 14.f - (SEGS == 1 ? m + log2_total : log2_total);
+    a.gm[i] = SEGS == 1 ? 0.f : none ? INFINITY : m;
+    a.gc[i] = SEGS == 1 ? (none ? -INFINITY : 14.f - (m + log2_total)) : none ? 0.f : 0x1p14f / total;
     const float g = none ? 0.f : isnan(log2_total) ? NAN : a.grad_nll[i];
     a.g[i] = g;
     a.gn[i] = ldexpf(g, eg);
@@ -615,7 +615,7 @@ __global__ __launch_bounds__(256) void vocab_finish_kernel(VocabArgs a) {
             a.nll[i] = nll;
         }
         if constexpr (GRAD)
-            v_row_of_gradient<SEGS>(a, i, label, m, log2_total, eg);
+            v_row_of_gradient<SEGS>(a, i, label, m, s, log2_total, eg);
     }
 }
 
@@ -630,7 +630,7 @@ __global__ __launch_bounds__(256) void vocab_prepare_kernel(VocabArgs a) {  // t
     if (label >= a.V) atomicOr(a.status, PIN_STATUS_LABEL_RANGE);
     const float lse = i < a.n ? a.lse[i] : 0.f;
     const float log2_total = lse == -INFINITY ? -INFINITY : isnan(lse) ? NAN : 0.f;
-    v_row_of_gradient<SEGS>(a, i, label, SEGS == 1 ? lse * V_LOG2E : lse, log2_total, eg);
+    v_row_of_gradient<SEGS>(a, i, label, SEGS == 1 ? lse * V_LOG2E : lse, isnan(lse) ? NAN : 1.f, log2_total, eg);
 }
 
 // D of one piece of the vocabulary: the logits again, D [n][piece] in fp16 (two planes of fp32).  A wave's part goes through LDS, so that
@@ -753,7 +753,8 @@ __global__ __launch_bounds__(VT_THREADS, VT_WGS * VT_WAVES / 4) void vocab_dx_ke
                 if (ib + 16 * i + r < a.n && kb + 16 * j < a.d) out[(long)(ib + 16 * i + r) * a.dk + kb + 16 * j] = acc[i][j][r];
 }
 
-// dW and db of one piece: D is taken as it lies, by columns
+// dW and db of one piece: D is taken as it lies, by columns.  Few labels and many rows would leave most of the card idle: the rows are
+// split then, into partial sums (4686 x 672 x 352 fp32, a step: 516 us without)
 template <int D, int SEGS>
 __global__ __launch_bounds__(VT_THREADS, VT_WGS * VT_WAVES / 4) void vocab_dw_kernel(VocabArgs a, int p0) {
     extern __shared__ __attribute__((aligned(16))) char vlds[];
@@ -768,7 +769,8 @@ __global__ __launch_bounds__(VT_THREADS, VT_WGS * VT_WAVES / 4) void vocab_dw_ke
         for (int j = 0; j < VT_NI; ++j) acc[i][j] = vt_f4{0.f, 0.f, 0.f, 0.f};
     }
     const bool bias = a.db != nullptr && k0 == 0 && wave % VT_WB == 0;
-    vt_product<false, SEGS, true, true>(P, XT, v0, k0, 0, a.nk / VT_K, vlds, acc, ones, bias);
+    const int steps = a.nk / VT_K, per = (steps + a.dw_splits - 1) / a.dw_splits, s0 = min((int)blockIdx.z * per, steps), s1 = min(s0 + per, steps);
+    vt_product<false, SEGS, true, true>(P, XT, v0, k0, (long)s0 * VT_K, s1 - s0, vlds, acc, ones, bias);
     const int eg = a.exps[0] + 14, e = eg + a.exps[1];  // (D holds 2^14 p and the scaled g)
     const int vb = p0 + v0 + (wave / VT_WB) * VT_TA + 4 * g, kb = k0 + (wave % VT_WB) * VT_TB + c;
 #pragma unroll
@@ -777,6 +779,14 @@ __global__ __launch_bounds__(VT_THREADS, VT_WGS * VT_WAVES / 4) void vocab_dw_ke
         for (int r = 0; r < 4; ++r) {
             const int v = vb + 16 * i + r;
             if (v >= a.V) continue;
+            if (a.dw_splits > 1) {
+                float* out = a.dwp + ((long)blockIdx.z * a.Vk + v) * a.dk;
+#pragma unroll
+                for (int j = 0; j < VT_NI; ++j)
+                    if (kb + 16 * j < a.d) out[kb + 16 * j] = acc[i][j][r];
+                if (bias && c == 0) a.dbp[(long)blockIdx.z * a.Vk + v] = ones[i][r];
+                continue;
+            }
 #pragma unroll
             for (int j = 0; j < VT_NI; ++j)
                 if (kb + 16 * j < a.d) v_put<D>(a.dw, (long)v * a.d + kb + 16 * j, ldexpf(acc[i][j][r], -e));
@@ -883,20 +893,23 @@ __global__ __launch_bounds__(256, vs_waves(D == PIN_F32 ? 2 : 1, KT, MODE)) void
             for (int i = 0; i < 2; ++i) {
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) acc[i][j] = START ? start[j] : vt_f4{0.f, 0.f, 0.f, 0.f};
+                // fp32: W_l x_h first, then W_h x_l and W_h x_h, whichever side owns: every pass has the same logits to the last bit (the
+                // label's p - 1 of a row that is nearly certain is a difference, and a step of a logit of 16 is 1e-6 of p)
                 if constexpr (PL == 2) {
 #pragma unroll
                     for (int k = 0; k < KT; ++k) {
-                        const vt_u4 lo = vs_read<TROW>(T + TR * TROW, 32 * q + 16 * i + c, 4 * k + g);
+                        const vt_u4 first = vs_read<TROW>(T + (OWN_X ? TR * TROW : 0), 32 * q + 16 * i + c, 4 * k + g);
 #pragma unroll
-                        for (int j = 0; j < NJ; ++j) acc[i][j] = vt_mfma<false>(lo, o[0][j][k], acc[i][j]);
+                        for (int j = 0; j < NJ; ++j) acc[i][j] = vt_mfma<false>(first, o[OWN_X ? 0 : PL - 1][j][k], acc[i][j]);
                     }
                 }
 #pragma unroll
                 for (int k = 0; k < KT; ++k) {
                     const vt_u4 hi = vs_read<TROW>(T, 32 * q + 16 * i + c, 4 * k + g);
+                    const vt_u4 lo = PL == 2 && !OWN_X ? vs_read<TROW>(T + TR * TROW, 32 * q + 16 * i + c, 4 * k + g) : hi;
 #pragma unroll
                     for (int j = 0; j < NJ; ++j) {
-                        if constexpr (PL == 2) acc[i][j] = vt_mfma<false>(hi, o[1][j][k], acc[i][j]);
+                        if constexpr (PL == 2) acc[i][j] = vt_mfma<false>(lo, o[OWN_X ? PL - 1 : 0][j][k], acc[i][j]);
                         acc[i][j] = vt_mfma<BF>(hi, o[0][j][k], acc[i][j]);
                     }
                 }
@@ -1211,7 +1224,7 @@ inline VocabPlan v_plan(const pin_vocab_head* h, int mode, char* base) {
         if (piece > a.Vk) piece = a.Vk;
         a.piece = (int)piece;
         a.dx_splits = v_splits((a.nk + VT_A - 1) / VT_A * features, (int)(piece / VT_K), 8, 256 * VT_WGS, v_part_cost((int)piece));
-        a.dw_splits = 0;
+        a.dw_splits = piece < a.Vk ? 1 : v_splits(tiles * features, a.nk / VT_K, 8, 256 * VT_WGS, v_part_cost(a.n));
     }
     if (p.few) a.splits = (a.V + 64 * p.few - 1) / (64 * p.few);
     long at = 0;
@@ -1244,12 +1257,11 @@ inline VocabPlan v_plan(const pin_vocab_head* h, int mode, char* base) {
         a.bad = (int*)rows_of(a.nk);
         a.exps = (int*)take(256);
         a.dxp = (float*)take((long)a.dx_splits * a.nk * a.dk * 4);
-        if (p.kt > 0) {
+        if (p.kt > 0 || a.dw_splits > 1) {
             a.dwp = (float*)take((long)a.dw_splits * a.Vk * a.dk * 4);
             a.dbp = (float*)take((long)a.dw_splits * a.Vk * 4);
-        } else {
-            a.p = (unsigned short*)take((long)planes * a.nk * a.ldp * 2);
-            }
+        }
+        if (p.kt == 0) a.p = (unsigned short*)take((long)planes * a.nk * a.ldp * 2);
     }
     p.bytes = at;
     return p;
@@ -1339,8 +1351,8 @@ template <int D, int GROUPS>
 static void v_join_partial(const VocabPlan& p, hipStream_t s) {
     const VocabArgs& a = p.a;
     const long cols = 256 / GROUPS * 4;
-    const int xb = (int)(((long)a.n * a.dk + cols - 1) / cols), wb = p.kt == 0 ? 0 : (int)(((long)a.V * a.dk + cols - 1) / cols);
-    const int bb = p.kt == 0 || a.db == nullptr ? 0 : (int)((a.V + cols - 1) / cols);
+    const int xb = (int)(((long)a.n * a.dk + cols - 1) / cols), wb = p.kt == 0 && a.dw_splits == 1 ? 0 : (int)(((long)a.V * a.dk + cols - 1) / cols);
+    const int bb = wb == 0 || a.db == nullptr ? 0 : (int)((a.V + cols - 1) / cols);
     V_LAUNCH((vocab_join_kernel<D, GROUPS>), dim3(xb + wb + bb), 0, a, xb, wb, p.kt > 0 ? 1 : 0);
 }
 
@@ -1389,7 +1401,7 @@ int v_run_typed(const VocabPlan& p, int mode, hipStream_t s) {
             const int width = p0 + a.piece < a.Vk ? a.piece : a.Vk - p0;
             V_TILES((vocab_probs_kernel<BF, SEGS>), dim3(a.nk / VT_B, width / VT_A), a, p0);
             V_TILES((vocab_dx_kernel<SEGS>), dim3(cdiv(a.nk, VT_A), kt, a.dx_splits), a, p0, width);
-            V_TILES((vocab_dw_kernel<D, SEGS>), dim3(width / VT_A, kt), a, p0);
+            V_TILES((vocab_dw_kernel<D, SEGS>), dim3(width / VT_A, kt, a.dw_splits), a, p0);
         }
     }
     const int most = a.dx_splits > a.dw_splits ? a.dx_splits : a.dw_splits;
