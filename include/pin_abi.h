@@ -1145,7 +1145,8 @@ int pin_adamw_step(const pin_adamw_tensor* tensors_host, int32_t n_tensors, cons
  * the NLL term, utils/mapper.py:782-800), for any features x [n][dim] and any number of labels: s = x W^T + b, log-softmax,
  * NLL and its gradients, or the most probable label -- without the n x vocab logits in memory.
  * x, weight and bias are of one type (PIN_F32, PIN_BF16, PIN_F16); sums, maxima and statistics are fp32.  A bias of -inf (or
- * below -1e30) switches a label off.  A row whose labels are all switched off has lse -inf, nll +inf, gradient 0 and the label -1. */
+ * below -1e30) switches a label off.  A row whose labels are all switched off has lse -inf, nll +inf, gradient 0 and the label -1.
+ * Outputs and workspace overlap neither each other nor an input. */
 #define PIN_VOCAB_MAX (1 << 22)      /* largest n, vocab */
 #define PIN_VOCAB_MAX_DIM (1 << 16)  /* largest dim */
 typedef struct pin_vocab_head {

@@ -16,7 +16,7 @@
 //
 // Memory-bound: 28 bytes an element with fp32 p, g and moments, 16.06 with 8-bit moments, 10.06 with p and g in 16 bits.  One
 // wave takes 256 elements (4 a lane: 16-byte loads of fp32, and the wave is the block of a scale, whose maximum is a reduction in
-// registers), a workgroup CHUNK of them per round; one launch serves up to 64 tensors, whose addresses travel as
+// registers), a workgroup CHUNK of them per round; one launch serves up to 96 tensors, whose addresses travel as
 // kernel arguments -- no table to upload, nothing to keep alive, and the call can be captured.  The step count lives on the device (the
 // clock): a captured step counts on when it is replayed.
 #include "pin_common.h"

@@ -1205,8 +1205,9 @@ inline VocabPlan v_plan(const pin_vocab_head* h, int mode, char* base) {
     p.few = grads || a.n > v_few_rows(h->dtype) ? 0 : a.V >= 131072 ? 4 : a.V >= 65536 ? 2 : 1;
     const int planes = two ? 2 : 1;
     // 16-bit rows that begin and end on 16-byte borders are read where they are
-    const bool copy_w = !p.few && (two || a.d != a.dk || a.ldw % 8 != 0 || (uintptr_t)a.w % 16 != 0);
-    const bool copy_x = !p.few && (grads || two || a.d != a.dk || a.ldx % 8 != 0 || (uintptr_t)a.x % 16 != 0);
+    // (and not so far apart that a tile's offsets would pass 32 bits)
+    const bool copy_w = !p.few && (two || a.d != a.dk || a.ldw % 8 != 0 || a.ldw > PIN_VOCAB_MAX || (uintptr_t)a.w % 16 != 0);
+    const bool copy_x = !p.few && (grads || two || a.d != a.dk || a.ldx % 8 != 0 || a.ldx > PIN_VOCAB_MAX || (uintptr_t)a.x % 16 != 0);
     const int rows = a.nk / VT_B, tiles = a.Vk / VT_A;
     if (p.kt > 0) {
         const int own = vs_owners(p.dtype, p.kt, false), grad = vs_owners(p.dtype, p.kt, true), tr = planes * p.kt <= 4 ? 64 : 32;

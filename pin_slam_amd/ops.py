@@ -928,8 +928,8 @@ def _vocab_workspace(h, gradients, ws, device):
     need = int(_lib.lib().pin_vocab_workspace_bytes(h.n, h.vocab, h.dim, h.dtype, int(gradients)))
     if ws is None:
         return torch.empty((max(need, 1),), dtype=torch.uint8, device=device)
-    if ws.dtype != torch.uint8 or ws.device != device or ws.numel() < need:
-        raise RuntimeError(f"the workspace must hold {need} bytes (uint8) on {device}")
+    if ws.dtype != torch.uint8 or ws.device != device or ws.numel() < need or not ws.is_contiguous():
+        raise RuntimeError(f"the workspace must hold {need} contiguous bytes (uint8) on {device}")
     return ws
 
 
@@ -1090,6 +1090,14 @@ class AdamW:
             if g.numel() != p.numel() or g.device != self.device:
                 raise RuntimeError(f"gradient {i}: {tuple(g.shape)} on {g.device} for a parameter {tuple(p.shape)} on {self.device}")
             t.grad_dtype = _DTYPE_CODES[g.dtype]
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), k) for k, ts in ((0, self.params), (1, grads)) for t in ts
+                       if t is not None and t.numel())
+        self._shared, end = False, [0, 0]  # (a gradient that serves two parameters is fine until it is to be cleared)
+        for a, b, k in spans:
+            if a < end[1 - k] or (k == 0 and a < end[0]):
+                raise RuntimeError("a gradient shares memory with a parameter, or two parameters do")
+            self._shared |= k == 1 and a < end[1]
+            end[k] = max(end[k], b)
         self.grads = grads
         self._bound = self.params + [g for g in grads if g is not None]
         self._addresses = [t.data_ptr() for t in self._bound]
@@ -1104,6 +1112,8 @@ class AdamW:
             raise RuntimeError("no gradients: pass them to AdamW() or to step()")
         elif list(map(torch.Tensor.data_ptr, self._bound)) != self._addresses:  # (a buffer was replaced behind its tensor, e.g. by .data = ...)
             self._bind(self.grads)
+        if zero_grad and self._shared:
+            raise RuntimeError("zero_grad: two parameters share a gradient buffer, which one of them would find cleared")
         if not self._any:
             return
         self._state.zero_grad = int(bool(zero_grad))

@@ -43,6 +43,17 @@ def test_refusals(host, kw, word):
         ops.AdamW(kw.pop("params"), kw.pop("grads", None), **kw)
 
 
+def test_gradients_that_share_memory(host):
+    flat = torch.zeros(20)
+    with pytest.raises(RuntimeError, match="shares memory"):
+        ops.AdamW([flat[:8]], [flat[4:12]])
+    with pytest.raises(RuntimeError, match="shares memory"):
+        ops.AdamW([flat[8:16], torch.zeros(12)], [torch.zeros(8), flat[4:16]])
+    opt = ops.AdamW([torch.zeros(8), torch.zeros(8)], [flat[:8], flat[:8]])
+    with pytest.raises(RuntimeError, match="zero_grad"):
+        opt.step(zero_grad=True)
+
+
 def test_shared_memory_and_missing_gradients_are_refused(host):
     flat = torch.zeros(10)
     with pytest.raises(RuntimeError, match="share memory"):

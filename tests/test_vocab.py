@@ -458,3 +458,58 @@ def test_float16_dx_is_rounded_once_at_the_label(shape):
     bound = want.abs() * 2.0 ** -11 + 2.0 ** -25 + ((p * (1 - hot)) @ W.abs()) * (G * (2.0 ** -11 + rel)) + ((p * hot) @ W.abs()) * G * rel
     bound = bound + ((p - hot).abs() @ W.abs()) * G * (F32 * (vocab / 32 + 40)) + W.abs().sum(0) * G.max() * 2.0 ** -39  # sums; tiny factors
     assert ((dx - want).abs() <= bound).all(), float(((dx - want).abs() / bound).max())
+
+
+@gpu
+def test_rows_far_apart():
+    """Rows 2^23 + 2^17 elements apart: 256 of them pass 32 bits of bytes."""
+    n, vocab, dim, ld = 70, 300, 512, (1 << 23) + (1 << 17)
+    x, w, b, labels, g = _inputs(n, vocab, dim, torch.bfloat16, 9)
+    far = torch.empty(vocab * ld, dtype=torch.bfloat16, device="cuda").view(vocab, ld)[:, :dim]
+    far.copy_(w)
+    for a, c in zip(ops.vocab_predict(x, w, b) + ops.vocab_nll_step(x, w, b, labels, g), ops.vocab_predict(x, far, b) + ops.vocab_nll_step(x, far, b, labels, g)):
+        assert torch.equal(a, c)
+    x = torch.cat([x, x, x, x, x])[:vocab]
+    far.copy_(x)
+    for a, c in zip(ops.vocab_predict(x, w, b), ops.vocab_predict(far, w, b)):
+        assert torch.equal(a, c)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(2000, 90, 300), (4686, 672, 352)])
+def test_few_labels_and_many_rows(shape, dtype):
+    x, w, b, labels, g = _inputs(*shape, dtype, 12, masked=True)
+    _check(x, w, b, labels, g, ops.vocab_nll_step(x, w, b, labels, g))
+
+
+@gpu
+def test_a_workspace_in_pieces_is_refused():
+    x, w, b, labels, g = _inputs(4, 50, 16, torch.float32, 1)
+    ws = ops.vocab_workspace(4, 50, 16)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        ops.vocab_predict(x, w, b, ws=torch.empty(2 * ws.numel(), dtype=torch.uint8, device="cuda")[::2])
+    with pytest.raises(RuntimeError, match="must hold"):
+        ops.vocab_nll_step(x, w, b, labels, g, ws=ws[:100])
+
+
+@gpu
+def test_float32_passes_agree_to_the_last_bit_of_a_logit():
+    """Rows that are nearly certain: db at a label is p - 1 of its row (and little of the others), a difference that a step of the label's
+    logit (2^-20 at 16) would move by 1e-6 whatever is left of it.  With logits of the same bits in every pass p is 1 / total rounded
+    (half a step, 2^-24), and nll = log total (within 2^-21 of itself: logarithm, product) tells the same total: db = expm1(-nll) + the
+    other rows' p, whose errors are delta of their size; D is two pieces (2^-21) and summed in fp32."""
+    n, vocab, dim = 64, 128, 64
+    x, w, b, _, _ = _inputs(n, vocab, dim, torch.float32, 3)
+    labels = torch.arange(n, device="cuda", dtype=torch.int32)
+    w = torch.nn.functional.normalize(w, dim=1)
+    x = w[:n] * 16 + 0.1 * x
+    nll, _, _, _, db = ops.vocab_nll_step(x, w, b, labels, torch.ones(n, device="cuda"))
+    X, W = x.double(), w.double()
+    p = torch.softmax(X @ W.t() + b.double(), 1)
+    others = p.sum(0)[:n] - p.diagonal()
+    label = torch.expm1(-nll.double())
+    delta = 2 * (X.norm(dim=1).max() * W.norm(dim=1).max() + b.double().abs().max()) * (dim * F32 + 2.0 ** -19)
+    bound = 2 * F32 + label.abs() * (2.0 ** -20 + 42 * F32) + others * (2 * delta + 2.0 ** -20 + 42 * F32) + n * 2.0 ** -39
+    off = (db.double()[:n] - (label + others)).abs()
+    assert (off <= bound).all(), float((off / bound).max())
