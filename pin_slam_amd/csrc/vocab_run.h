@@ -96,17 +96,23 @@ __device__ float v_block_max(const float* part, float* sh) {  // the maximum of 
 
 __device__ __forceinline__ bool v_takes_part(const VocabArgs& a, long row) { return a.labels[row] >= 0 && a.labels[row] < a.V; }
 
-// eight consecutive elements of a row from k on, zero behind its end; VEC: they begin on a 16-byte border
+// eight consecutive elements of a row from k on, zero behind its end.  The whole eight are one read each 16 bytes, wherever the row
+// begins (global reads need not be aligned; element by element 94047 x 675 fp32 took 249 us)
+__device__ __forceinline__ vt_u4 v_read16(const void* at) {
+    vt_u4 u;
+    __builtin_memcpy(&u, at, 16);
+    return u;
+}
 template <int D>
-__device__ __forceinline__ void v_chunk(const void* row, int k, int d, bool vec, float (&x)[8]) {
-    if (vec && k + 8 <= d) {
+__device__ __forceinline__ void v_chunk(const void* row, int k, int d, float (&x)[8]) {
+    if (k + 8 <= d) {
         if constexpr (D == PIN_F32) {
-            const vt_f4 p = *reinterpret_cast<const vt_f4*>(reinterpret_cast<const float*>(row) + k);
-            const vt_f4 q = *reinterpret_cast<const vt_f4*>(reinterpret_cast<const float*>(row) + k + 4);
+            const vt_f4 p = __builtin_bit_cast(vt_f4, v_read16(reinterpret_cast<const float*>(row) + k));
+            const vt_f4 q = __builtin_bit_cast(vt_f4, v_read16(reinterpret_cast<const float*>(row) + k + 4));
 #pragma unroll
             for (int i = 0; i < 4; ++i) { x[i] = p[i]; x[4 + i] = q[i]; }
         } else {
-            const vt_u4 u = *reinterpret_cast<const vt_u4*>(reinterpret_cast<const unsigned short*>(row) + k);
+            const vt_u4 u = v_read16(reinterpret_cast<const unsigned short*>(row) + k);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if constexpr (D == PIN_BF16) {
@@ -127,10 +133,6 @@ template <int D>
 __device__ __forceinline__ const void* v_row(const void* p, long row, long ld) {
     return reinterpret_cast<const char*>(p) + row * ld * (D == PIN_F32 ? 4 : 2);
 }
-template <int D>
-__device__ __forceinline__ bool v_aligned(const void* p, long ld) {
-    return ((uintptr_t)p | (uintptr_t)(ld * (D == PIN_F32 ? 4 : 2))) % 16 == 0;
-}
 
 // Staging, first launch.  The largest |x| (of the rows that take part), |W|, |g|; the padded bias (-inf: switched off, and behind the
 // last label); the operands of the logit product where they have to be made: two fp16 pieces of fp32 times the row's power of two, or a padded
@@ -140,7 +142,7 @@ __device__ __forceinline__ bool v_aligned(const void* p, long ld) {
 template <int D>
 __global__ __launch_bounds__(256) void vocab_rows_kernel(VocabArgs a, int lanes, int scan_w) {  // scan_w: W's largest value is wanted
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, per = 64 / lanes, mine = lane & (lanes - 1);
-    const bool copy_x = a.xa != nullptr, copy_w = a.wa != nullptr, vx = v_aligned<D>(a.x, a.ldx), vw = v_aligned<D>(a.w, a.ldw);
+    const bool copy_x = a.xa != nullptr, copy_w = a.wa != nullptr;
     float mx = 0.f, mw = 0.f, mg = 0.f;
     const long rx = copy_x ? a.n : 0, rw = copy_w || scan_w ? a.V : 0, waves = (long)gridDim.x * 4;
     for (long base = ((long)blockIdx.x * 4 + wave) * per; base < rx + rw; base += waves * per) {
@@ -149,11 +151,10 @@ __global__ __launch_bounds__(256) void vocab_rows_kernel(VocabArgs a, int lanes,
         const bool is_x = r < rx, copy = is_x || copy_w;
         const long row = is_x ? r : r - rx;
         const void* src = v_row<D>(is_x ? a.x : a.w, row, is_x ? a.ldx : a.ldw);
-        const bool vec = is_x ? vx : vw;
         float x[8], m = 0.f;
         bool odd = false;
         for (int k = mine * 8; k < a.dk; k += lanes * 8) {
-            v_chunk<D>(src, k, a.d, vec, x);
+            v_chunk<D>(src, k, a.d, x);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 m = fmaxf(m, fabsf(x[i]));
@@ -175,7 +176,7 @@ __global__ __launch_bounds__(256) void vocab_rows_kernel(VocabArgs a, int lanes,
             if (mine == 0) (is_x ? a.xs : a.ws_)[row] = ldexpf(1.f, -e);
         }
         for (int k = mine * 8; k < a.dk; k += lanes * 8) {
-            if (a.dk > lanes * 8) v_chunk<D>(src, k, a.d, vec, x);  // (else they are still in registers)
+            if (a.dk > lanes * 8) v_chunk<D>(src, k, a.d, x);  // (else they are still in registers)
             vt_u4 h, l;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -229,14 +230,13 @@ __global__ __launch_bounds__(256) void vocab_transpose_kernel(VocabArgs a, int x
     const long padded = is_x ? a.ldxt : a.ldwt;
     const void* base = is_x ? a.x : a.w;
     const long ld = is_x ? a.ldx : a.ldw;
-    const bool vec = v_aligned<D>(base, ld);
     {
         const int r = threadIdx.x >> 2, k = (threadIdx.x & 3) * 16;
         const bool in = r0 + r < rows && (!is_x || v_takes_part(a, r0 + r));
 #pragma unroll
         for (int half = 0; half < 16; half += 8) {
             float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            if (in && k0 + k + half < a.d) v_chunk<D>(v_row<D>(base, r0 + r, ld), k0 + k + half, a.d, vec, x);
+            if (in && k0 + k + half < a.d) v_chunk<D>(v_row<D>(base, r0 + r, ld), k0 + k + half, a.d, x);
 #pragma unroll
             for (int i = 0; i < 8; ++i) tile[r][k + half + i] = x[i];
         }
@@ -426,7 +426,7 @@ __global__ __launch_bounds__(VT_THREADS, VT_WGS * VT_WAVES / 4) void vocab_forwa
 // Forward for a few rows (n <= 16 NT): W is read once, straight into the matrix cores' operand, and that is all there is -- no staging, no
 // LDS tiles.  A wave takes 16 RT labels; lane (c, g) reads 16 bytes of label c's row a step (16-bit types: k = 32 s + 8 g ..; fp32, whose
 // products are the fp32 matrix instruction's: k = 16 s + 4 g ..), four consecutive lanes g a contiguous 64 bytes.  Rows that do not
-// begin and end on 16-byte borders (VEC false) are read element by element.
+// begin and end on 16-byte borders (VEC false) have a last step that is read element by element.
 template <int N>
 struct VInt { static constexpr int value = N; };
 template <int D, int RT, int NT, bool VEC, bool ARG>
@@ -451,13 +451,15 @@ __global__ __launch_bounds__(256) void vocab_few_kernel(VocabArgs a) {
         vt_u4 u = {0u, 0u, 0u, 0u};
         if constexpr (VEC) {  // (d is a multiple of EL)
             if (!tail || k < a.d) u = *reinterpret_cast<const vt_u4*>(row + k * (D == PIN_F32 ? 4 : 2));
+        } else if (!tail || k + EL <= a.d) {
+            u = v_read16(row + k * (D == PIN_F32 ? 4 : 2));
         } else if constexpr (D == PIN_F32) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) u[e] = !tail || k + e < a.d ? reinterpret_cast<const unsigned*>(row)[k + e] : 0u;
+            for (int e = 0; e < 4; ++e) u[e] = k + e < a.d ? reinterpret_cast<const unsigned*>(row)[k + e] : 0u;
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                u[e >> 1] |= (!tail || k + e < a.d ? (unsigned)reinterpret_cast<const unsigned short*>(row)[k + e] : 0u) << (16 * (e & 1));
+                u[e >> 1] |= (k + e < a.d ? (unsigned)reinterpret_cast<const unsigned short*>(row)[k + e] : 0u) << (16 * (e & 1));
         }
         return u;
     };
@@ -1349,10 +1351,10 @@ static void v_few(const VocabPlan& p, int mode, hipStream_t s) {
 }
 
 template <int D, int GROUPS>
-static void v_join_partial(const VocabPlan& p, hipStream_t s) {
+static void v_join_partial(const VocabPlan& p, bool x, bool w, hipStream_t s) {
     const VocabArgs& a = p.a;
     const long cols = 256 / GROUPS * 4;
-    const int xb = (int)(((long)a.n * a.dk + cols - 1) / cols), wb = p.kt == 0 && a.dw_splits == 1 ? 0 : (int)(((long)a.V * a.dk + cols - 1) / cols);
+    const int xb = !x ? 0 : (int)(((long)a.n * a.dk + cols - 1) / cols), wb = !w ? 0 : (int)(((long)a.V * a.dk + cols - 1) / cols);
     const int bb = wb == 0 || a.db == nullptr ? 0 : (int)((a.V + cols - 1) / cols);
     V_LAUNCH((vocab_join_kernel<D, GROUPS>), dim3(xb + wb + bb), 0, a, xb, wb, p.kt > 0 ? 1 : 0);
 }
@@ -1405,10 +1407,23 @@ int v_run_typed(const VocabPlan& p, int mode, hipStream_t s) {
             V_TILES((vocab_dw_kernel<D, SEGS>), dim3(width / VT_A, kt, a.dw_splits), a, p0);
         }
     }
-    const int most = a.dx_splits > a.dw_splits ? a.dx_splits : a.dw_splits;
-    if (most > 16) v_join_partial<D, 16>(p, s);
-    else if (most > 2) v_join_partial<D, 4>(p, s);
-    else v_join_partial<D, 1>(p, s);
+    // threads that share a sum's parts: as the parts are many; dx and dW in one launch where they agree
+    auto join = [&](int parts, bool x, bool w) {
+        if (parts > 16) v_join_partial<D, 16>(p, x, w, s);
+        else if (parts > 2) v_join_partial<D, 4>(p, x, w, s);
+        else v_join_partial<D, 1>(p, x, w, s);
+    };
+    const bool w_parts = p.kt > 0 || a.dw_splits > 1;
+    const long w_sum = (long)a.V * a.dk;
+    if (w_parts && a.dx_splits > 2 && a.dw_splits <= 2 && w_sum > (1l << 20)) {  // (a small dW is not worth a launch: 5 us)
+        join(a.dx_splits, true, false);
+        join(a.dw_splits, false, true);
+    } else if (w_parts && a.dw_splits > 2 && a.dx_splits <= 2 && (long)a.n * a.dk > (1l << 20)) {
+        join(a.dx_splits, true, false);
+        join(a.dw_splits, false, true);
+    } else {
+        join(w_parts && a.dw_splits > a.dx_splits ? a.dw_splits : a.dx_splits, true, w_parts);
+    }
     PIN_CHECK_LAUNCH();
     return 0;
 }
