@@ -10,7 +10,7 @@
 // streamed rows, if those are counted in the order (g, i, r) within each 32: D goes from accumulator to operand without leaving the lane,
 // and T^T is laid out in that order by the staging launch (v_stream_row).
 //
-// What bounds it: at 64 dimensions the exponential and the arithmetic around it (one v_exp_f32 of 16 cycles and 3 to 4 instructions of 4
+// What bounds it: at 64 dimensions the exponential and the arithmetic around it (one v_exp_f32 of 8 cycles and 3 to 4 instructions of 4
 // cycles an element and wave, against 2 products of 64), at 256 the matrix cores and, as much, the LDS reads that feed them: each
 // operand read serves the wave's NJ tiles of owners.
 #pragma once
